@@ -1,0 +1,231 @@
+// The C entry points of include/amem_kv.h: what they refuse, the paused gate, and the device they launch on.
+#include <hip/hip_runtime_api.h>
+#include <unistd.h>
+
+#include <mutex>
+
+#include "../../include/amem.h"
+#include "../../include/amem_kv.h"
+#include "ctx.h"
+#include "ipc.h"
+#include "kv.h"
+#include "log.h"
+#include "vmm.h"
+
+namespace amem {
+namespace {
+
+int refuse(const char* what, const char* why) {
+  LOGGER(ERROR, "%s: refused: %s", what, why);
+  return (int)hipErrorInvalidValue;
+}
+#define NEED(cond, why) \
+  do {                  \
+    if (!(cond)) return refuse(what, why); \
+  } while (0)
+
+int log2_of(int x) { return x > 0 && (x & (x - 1)) == 0 ? __builtin_ctz(x) : -1; }
+
+bool fits(int64_t n, int64_t stride) {
+  int64_t bytes;
+  return !__builtin_mul_overflow(n, stride, &bytes) && bytes >= 0 && bytes < ((int64_t)1 << 58);
+}
+
+// Strides that a view of a tensor can have: whole vectors of 16 bytes, forward, below 2^40 elements.
+bool stride_ok(int64_t s, int vector) { return s >= 0 && s < ((int64_t)1 << 40) && s % vector == 0; }
+
+int check_cache(const char* what, const amem_kv_cache* c, bool addresses, KvCache* out) {
+  NEED(c, "cache is NULL");
+  NEED(c->type == AMEM_KV_BF16 || c->type == AMEM_KV_F16 || c->type == AMEM_KV_E4M3, "cache type");
+  NEED(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, "head_dim is not 64, 128 or 256");
+  NEED(c->pages >= 1 && c->kv_heads >= 1 && c->kv_heads <= 1024, "pages or kv_heads out of range");
+  const int page_shift = log2_of(c->page_slots), block_shift = log2_of(c->block_slots);
+  NEED(page_shift >= 0 && page_shift <= 10, "page_slots is not a power of two from 1 to 1024");
+  const bool eight = c->type == AMEM_KV_E4M3;
+  const int element = eight ? 1 : 2;
+  if (eight) {
+    NEED(block_shift >= 4 && block_shift <= 7 && block_shift <= page_shift,
+         "block_slots is not a power of two from 16 to 128 and at most page_slots");
+    NEED(c->scale_page_stride >= 0 && c->scale_head_stride >= 0, "scale strides");
+  } else {
+    NEED(c->block_slots == 0 && c->k_scale == 0 && c->v_scale == 0, "scales with a 16-bit cache");
+  }
+  NEED(stride_ok(c->page_stride, 16 / element) && stride_ok(c->head_stride, 16 / element) &&
+           stride_ok(c->slot_stride, 16 / element),
+       "cache strides are not multiples of 16 bytes");
+  // offsets fit 63 bits with room to add them up
+  NEED(fits(c->pages, c->page_stride) && fits(c->kv_heads, c->head_stride) && fits(c->page_slots, c->slot_stride) &&
+           fits(c->pages, c->scale_page_stride) && fits(c->kv_heads, c->scale_head_stride),
+       "the cache is larger than addresses");
+  NEED(c->reserved == 0, "cache.reserved is not 0");
+  if (addresses) {
+    NEED(c->k && c->v && c->k % 16 == 0 && c->v % 16 == 0, "cache addresses are not aligned to 16 bytes");
+    if (eight) NEED(c->k_scale && c->v_scale && c->k_scale % 4 == 0 && c->v_scale % 4 == 0, "addresses of the scales");
+  }
+  *out = {(uint8_t*)(uintptr_t)c->k, (uint8_t*)(uintptr_t)c->v, (float*)(uintptr_t)c->k_scale, (float*)(uintptr_t)c->v_scale,
+          c->page_stride * element, c->head_stride * element, c->slot_stride * element, c->scale_page_stride,
+          c->scale_head_stride, c->pages, c->kv_heads, page_shift, eight ? block_shift : 0};
+  return 0;
+}
+
+int check_batch(const char* what, const amem_kv_batch* b, const KvCache& c, bool addresses, KvBatch* out) {
+  NEED(b, "batch is NULL");
+  NEED(b->sequences >= 0 && b->sequences <= 1 << 20 && b->tokens >= 0 && b->tokens <= 1 << 24,
+       "sequences or tokens out of range");
+  NEED(b->max_tokens >= 0 && b->max_tokens <= b->tokens, "max_tokens is not between 0 and tokens");
+  NEED(b->table_pages >= 0 && b->table_stride >= b->table_pages, "table_pages or table_stride");
+  NEED(b->max_context >= 0 && b->max_context < 1 << 30 &&
+           b->max_context <= (int64_t)b->table_pages << c.page_shift && fits(b->sequences, b->table_stride),
+       "max_context is above what table_pages hold, or 2^30");
+  NEED(b->reserved == 0, "batch.reserved is not 0");
+  if (addresses && b->sequences) {
+    NEED(b->context && b->context % 4 == 0 && b->cu_tokens % 4 == 0, "addresses of the lengths");
+    NEED(b->table_pages == 0 || (b->page_table && b->page_table % 4 == 0), "address of the page table");
+  }
+  if (!b->cu_tokens && addresses)
+    NEED((int64_t)b->sequences * b->max_tokens == b->tokens, "without cu_tokens there are sequences * max_tokens rows");
+  *out = {(const int*)(uintptr_t)b->page_table, (const int*)(uintptr_t)b->context, (const int*)(uintptr_t)b->cu_tokens,
+          b->table_stride, b->sequences, b->table_pages, b->tokens, b->max_tokens, b->max_context};
+  return 0;
+}
+
+// A tensor [token][head][dim] of 16-bit elements.
+int check_rows(const char* what, const char* why, uint64_t at, int64_t token, int64_t head, int tokens, int heads) {
+  NEED(at && at % 16 == 0 && stride_ok(token, 8) && stride_ok(head, 8) && fits(tokens, token) && fits(heads, head), why);
+  return 0;
+}
+
+// Runs `launch` with the cache's device current, unless the process is paused. The registry's lock is held
+// meanwhile: a pause takes it for its whole length and waits for the device before it releases anything, so what
+// gets enqueued here has run by then, and a call made during a pause finds the process paused.
+template <class Launch>
+int on_device(const char* what, int device, hipStream_t stream, Launch launch) {
+  if (!gpu_present()) {
+    LOGGER(ERROR, "%s: no HIP device", what);
+    return (int)hipErrorNoDevice;
+  }
+  int current = 0;
+  if (hipError_t e = CHECK_HIP(hipGetDevice(&current)); e != hipSuccess) return (int)e;
+  if (stream) {
+    hipDevice_t of;
+    if (hipError_t e = CHECK_HIP(hipStreamGetDevice(stream, &of)); e != hipSuccess) return (int)e;
+    NEED((int)of == device, "the stream is another device's than the cache");
+  }
+  Ctx* c = globals().disabled > 0 ? nullptr : globals().ctx;
+  std::unique_lock<std::mutex> lk;
+  if (c) {
+    lk = std::unique_lock<std::mutex>(c->structure);
+    std::lock_guard<std::mutex> lf(c->fields);
+    if (c->paused) {
+      LOGGER(WARN, "%s: groupID:%d pid:%d is paused: refused", what, amem_groupID_value(), getpid());
+      return (int)hipErrorInvalidValue;
+    }
+  }
+  if (device != current)
+    if (hipError_t e = CHECK_HIP(hipSetDevice(device)); e != hipSuccess) return (int)e;
+  const hipError_t e = CHECK_HIP(launch());
+  if (device != current) (void)CHECK_HIP(hipSetDevice(current));
+  return (int)e;
+}
+
+}  // namespace
+}  // namespace amem
+
+using namespace amem;
+
+extern "C" {
+
+int amem_kv_append(const amem_kv_cache* cache, const amem_kv_batch* batch, const amem_kv_append_args* a, void* stream) {
+  const char* what = "amem_kv_append";
+  KvCache c;
+  KvBatch b;
+  if (int e = check_cache(what, cache, true, &c)) return e;
+  if (int e = check_batch(what, batch, c, true, &b)) return e;
+  NEED(a, "args is NULL");
+  NEED(a->type == AMEM_KV_BF16 || a->type == AMEM_KV_F16, "type is not 16 bits");
+  const bool eight = cache->type == AMEM_KV_E4M3;
+  NEED(eight || cache->type == a->type, "a 16-bit cache has another type than the rows");
+  if (b.tokens) {
+    if (int e = check_rows(what, "address or strides of k", a->k, a->k_token_stride, a->k_head_stride, b.tokens, c.kv_heads)) return e;
+    if (int e = check_rows(what, "address or strides of v", a->v, a->v_token_stride, a->v_head_stride, b.tokens, c.kv_heads)) return e;
+  }
+  NEED(!a->q == !a->q_out, "q and q_out go together");
+  if (a->q) {
+    NEED(a->q_heads >= 1 && a->q_heads <= 1024, "q_heads out of range");
+    if (int e = check_rows(what, "address or strides of q", a->q, a->q_token_stride, a->q_head_stride, b.tokens, a->q_heads)) return e;
+    if (int e = check_rows(what, "address or strides of q_out", a->q_out, a->q_out_token_stride, a->q_out_head_stride, b.tokens, a->q_heads)) return e;
+  }
+  const int pairs = a->rotary_dim / 2;
+  NEED(a->rotary_dim >= 0 && a->rotary_dim <= cache->head_dim && a->rotary_dim % 16 == 0,
+       "rotary_dim is not a multiple of 16 up to head_dim");
+  KvAppend p = {(const uint16_t*)(uintptr_t)a->k, (const uint16_t*)(uintptr_t)a->v, (const uint16_t*)(uintptr_t)a->q,
+                (uint16_t*)(uintptr_t)a->q_out, (const float*)(uintptr_t)a->cos, (const float*)(uintptr_t)a->sin,
+                (const int*)(uintptr_t)a->positions, a->k_token_stride, a->k_head_stride, a->v_token_stride,
+                a->v_head_stride, a->q_token_stride, a->q_head_stride, a->q_out_token_stride, a->q_out_head_stride,
+                a->positions_stride, a->q ? a->q_heads : 0, a->rotary_dim, a->interleaved != 0, a->table_rows, 1,
+                {pairs, pairs, pairs, pairs}};
+  if (pairs) {
+    NEED(a->cos && a->sin && a->cos % 16 == 0 && a->sin % 16 == 0 && a->table_rows >= 1, "the tables of the rotation");
+    NEED(a->axes >= 1 && a->axes <= AMEM_KV_MAX_AXES, "axes out of range");
+    NEED(a->axes == 1 || a->positions, "several axes need positions");
+    NEED(!a->positions || (a->positions % 4 == 0 && (a->axes == 1 || a->positions_stride >= b.tokens)), "positions");
+    if (a->axes > 1) {
+      int64_t end = 0;
+      for (int i = 0; i < a->axes; ++i) {
+        NEED(a->sections[i] >= 0, "sections are not the pairs of the axes");
+        end += a->sections[i];
+        p.axis_end[i] = (int)(end < pairs ? end : pairs);
+      }
+      NEED(end == pairs, "sections are not the pairs of the axes");
+    }
+    p.axes = a->axes;
+  }
+  if (!b.tokens || !b.sequences) return 0;
+  return on_device(what, cache->device, (hipStream_t)stream, [&] {
+    return launch_kv_append(c, b, p, cache->head_dim, a->type == AMEM_KV_F16, eight, (hipStream_t)stream);
+  });
+}
+
+int amem_kv_attention_workspace(const amem_kv_cache* cache, const amem_kv_batch* batch, int q_heads, uint64_t* bytes) {
+  const char* what = "amem_kv_attention_workspace";
+  KvCache c;
+  KvBatch b;
+  if (int e = check_cache(what, cache, false, &c)) return e;
+  if (int e = check_batch(what, batch, c, false, &b)) return e;
+  NEED(q_heads >= 1 && q_heads <= 1024 && q_heads % c.kv_heads == 0, "q_heads is not a multiple of kv_heads");
+  NEED(bytes, "bytes is NULL");
+  *bytes = kv_attend_workspace(c, b, q_heads, batch->max_tokens, cache->head_dim);
+  return 0;
+}
+
+int amem_kv_attention(const amem_kv_cache* cache, const amem_kv_batch* batch, const amem_kv_attention_args* a, void* stream) {
+  const char* what = "amem_kv_attention";
+  KvCache c;
+  KvBatch b;
+  if (int e = check_cache(what, cache, true, &c)) return e;
+  if (int e = check_batch(what, batch, c, true, &b)) return e;
+  NEED(a, "args is NULL");
+  NEED(a->type == AMEM_KV_BF16 || a->type == AMEM_KV_F16, "type is not 16 bits");
+  const bool eight = cache->type == AMEM_KV_E4M3;
+  NEED(eight || cache->type == a->type, "a 16-bit cache has another type than the rows");
+  NEED(a->q_heads >= 1 && a->q_heads <= 1024 && a->q_heads % c.kv_heads == 0, "q_heads is not a multiple of kv_heads");
+  if (b.tokens) {
+    if (int e = check_rows(what, "address or strides of q", a->q, a->q_token_stride, a->q_head_stride, b.tokens, a->q_heads)) return e;
+    if (int e = check_rows(what, "address or strides of out", a->out, a->out_token_stride, a->out_head_stride, b.tokens, a->q_heads)) return e;
+  }
+  NEED(a->lse % 4 == 0, "address of lse");
+  NEED(a->window >= 0, "window is negative");
+  NEED(a->scale - a->scale == 0, "scale is not finite");
+  NEED(a->reserved == 0, "args.reserved is not 0");
+  const uint64_t need = kv_attend_workspace(c, b, a->q_heads, batch->max_tokens, cache->head_dim);
+  NEED(!need || (a->workspace && a->workspace % 16 == 0 && a->workspace_bytes >= need), "workspace is too small or not aligned to 16 bytes");
+  if (!b.tokens || !b.sequences) return 0;
+  const KvAttend p = {(const uint16_t*)(uintptr_t)a->q, (uint16_t*)(uintptr_t)a->out, (float*)(uintptr_t)a->lse,
+                      (uint8_t*)(uintptr_t)a->workspace, a->q_token_stride, a->q_head_stride, a->out_token_stride,
+                      a->out_head_stride, a->scale, a->q_heads, a->causal != 0, a->window, batch->max_tokens};
+  return on_device(what, cache->device, (hipStream_t)stream, [&] {
+    return launch_kv_attend(c, b, p, cache->head_dim, a->type == AMEM_KV_F16, eight, (hipStream_t)stream);
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,255 @@
+"""ctypes binding of include/amem_kv.h: append to a paged key/value cache, and attention over it.
+
+Tensors are whatever has `data_ptr()`, `shape`, `stride()`, `dtype` and `device` (torch's do); nothing here
+imports their library. A program that uses torch imports it before this package loads its own library: the
+process then has one HIP runtime, torch's.
+
+    cache = kv.Cache(k, v)                      # [pages, heads, slots, dim]; 8 bits: also the two tensors of scales
+    batch = kv.Batch(page_table, context, tokens=n, max_tokens=1, max_context=limit)
+    kv.append(cache, batch, new_k, new_v, q, q, rotation=kv.Rotation(cos, sin), stream=stream)
+    kv.attention(cache, batch, q, out, workspace=workspace, stream=stream)
+
+A `Cache`, `Batch` or `Rotation` describes tensors (addresses, sizes, strides) and keeps them alive; what the tensors
+hold may change between calls. `stream` is a hipStream_t as a number, `torch.cuda.current_stream().cuda_stream`
+for instance. Arguments that do not fit raise ValueError before anything is enqueued; what the library refuses
+raises KvError.
+"""
+import ctypes as C
+
+from . import binding
+
+BF16, F16, E4M3 = range(3)
+MAX_AXES = 4
+_TYPES = {"torch.bfloat16": BF16, "torch.float16": F16, "torch.float8_e4m3fn": E4M3}
+
+
+class KvError(RuntimeError):
+    def __init__(self, what, code):
+        super().__init__("%s failed: %d (refused arguments, or paused, if 1; the library's log says why)" % (what, code))
+        self.code = code
+
+
+class CacheInfo(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("k", "v", "k_scale", "v_scale")] + [
+        (n, C.c_int64) for n in ("page_stride", "head_stride", "slot_stride", "scale_page_stride", "scale_head_stride")] + [
+        (n, C.c_int32) for n in ("type", "device", "pages", "kv_heads", "page_slots", "block_slots", "head_dim", "reserved")]
+
+
+class BatchInfo(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("page_table", "context", "cu_tokens")] + [("table_stride", C.c_int64)] + [
+        (n, C.c_int32) for n in ("sequences", "table_pages", "tokens", "max_tokens", "max_context", "reserved")]
+
+
+class AppendArgs(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("k", "v", "q", "q_out", "cos", "sin", "positions")] + [
+        (n, C.c_int64) for n in ("k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride", "q_token_stride",
+                                 "q_head_stride", "q_out_token_stride", "q_out_head_stride", "positions_stride")] + [
+        (n, C.c_int32) for n in ("type", "q_heads", "rotary_dim", "interleaved", "table_rows", "axes")] + [
+        ("sections", C.c_int32 * MAX_AXES)]
+
+
+class AttentionArgs(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("q", "out", "lse", "workspace", "workspace_bytes")] + [
+        (n, C.c_int64) for n in ("q_token_stride", "q_head_stride", "out_token_stride", "out_head_stride")] + [
+        ("scale", C.c_float)] + [(n, C.c_int32) for n in ("type", "q_heads", "causal", "window", "reserved")]
+
+
+_SIGNATURES = {
+    "amem_kv_append": (C.c_int, [C.POINTER(CacheInfo), C.POINTER(BatchInfo), C.POINTER(AppendArgs), C.c_void_p]),
+    "amem_kv_attention": (C.c_int, [C.POINTER(CacheInfo), C.POINTER(BatchInfo), C.POINTER(AttentionArgs), C.c_void_p]),
+    "amem_kv_attention_workspace": (C.c_int, [C.POINTER(CacheInfo), C.POINTER(BatchInfo), C.c_int, C.POINTER(C.c_uint64)]),
+}
+_entry = {}
+
+
+def kv_abi_names():
+    return sorted(_SIGNATURES)
+
+
+def load():
+    """The library, with the entry points of include/amem_kv.h declared."""
+    lib = binding.load()
+    if not _entry:
+        for name, (res, args) in _SIGNATURES.items():
+            fn = getattr(lib, name)
+            fn.restype, fn.argtypes = res, args
+            _entry[name] = fn
+    return lib
+
+
+def _call(name, *args):
+    if not _entry:
+        load()
+    code = _entry[name](*args)
+    if code:
+        raise KvError(name, code)
+
+
+def _need(ok, why):
+    if not ok:
+        raise ValueError(why)
+
+
+def _device(t):
+    d = t.device
+    _need(d.type == "cuda", "a tensor is not on a GPU")
+    return d.index or 0
+
+
+def _is(t, dtype, device, what):
+    _need(str(t.dtype) == dtype, "%s is not %s" % (what, dtype))
+    _need(_device(t) == device, "%s is on another device than the cache" % what)
+
+
+class Cache:
+    """Keys and values [pages, heads, slots, dim], with equal strides and contiguous dims; e4m3 with their scales, float32
+    [pages, heads, blocks], blocks contiguous."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        _need(len(k.shape) == 4 and tuple(k.shape) == tuple(v.shape) and k.stride() == v.stride() and k.dtype == v.dtype,
+              "k and v differ, or are not [pages, heads, slots, dim]")
+        _need(str(k.dtype) in _TYPES, "k is not bfloat16, float16 or float8_e4m3fn")
+        pages, heads, slots, dim = k.shape
+        at = k.stride()
+        _need(at[3] == 1 or dim == 1, "the dims of k are not contiguous")
+        device = _device(k)
+        _need(_device(v) == device, "k and v are on different devices")
+        kind, block = _TYPES[str(k.dtype)], 0
+        _need((kind == E4M3) == (k_scale is not None) == (v_scale is not None), "8 bits have scales, 16 have none")
+        info = CacheInfo(k.data_ptr(), v.data_ptr(), 0, 0, at[0], at[1], at[2], 0, 0, kind, device, pages, heads, slots, 0, dim, 0)
+        if kind == E4M3:
+            for t in (k_scale, v_scale):
+                _is(t, "torch.float32", device, "a tensor of scales")
+            shape = tuple(k_scale.shape)
+            _need(shape == tuple(v_scale.shape) and k_scale.stride() == v_scale.stride() and len(shape) == 3 and shape[:2] == (pages, heads)
+                  and shape[2] > 0 and slots % shape[2] == 0 and (k_scale.stride()[2] == 1 or shape[2] == 1),
+                  "the scales are not [pages, heads, blocks] with contiguous blocks")
+            block = slots // shape[2]
+            info.k_scale, info.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+            info.scale_page_stride, info.scale_head_stride = k_scale.stride()[:2]
+            info.block_slots = block
+        self.info, self.device, self.dim, self.heads, self.kind = info, device, dim, heads, kind
+        self._keep = (k, v, k_scale, v_scale)
+        self._ref = C.byref(info)
+
+
+class Batch:
+    """The sequences of a call: page_table int32 [sequences, pages] (rows may be strided), context int32 [sequences] (tokens
+    in the cache, the new ones included), cu_tokens int32 [sequences + 1] or None where all have max_tokens rows,
+    tokens: rows of the token tensors; max_context: no context is above it (None: what the table's pages hold, for which
+    give page_slots)."""
+
+    def __init__(self, page_table, context, tokens, cu_tokens=None, max_tokens=None, max_context=None, page_slots=None):
+        device = _device(context)
+        n = context.shape[0]
+        for t, what in ((page_table, "page_table"), (context, "context"), (cu_tokens, "cu_tokens")):
+            if t is not None:
+                _is(t, "torch.int32", device, what)
+        _need(len(page_table.shape) == 2 and page_table.shape[0] == n and (page_table.stride()[1] == 1 or page_table.shape[1] < 2),
+              "page_table is not [sequences, pages] with contiguous pages")
+        _need(len(context.shape) == 1 and (n < 2 or context.stride()[0] == 1), "context is not contiguous")
+        if cu_tokens is not None:
+            _need(tuple(cu_tokens.shape) == (n + 1,) and cu_tokens.stride()[0] == 1, "cu_tokens is not [sequences + 1]")
+            max_tokens = tokens if max_tokens is None else max_tokens
+        else:
+            max_tokens = (tokens // n if n else 0) if max_tokens is None else max_tokens
+        if max_context is None:
+            _need(page_slots, "max_context or page_slots is needed")
+            max_context = page_table.shape[1] * page_slots
+        pages = page_table.shape[1]
+        stride = page_table.stride()[0] if n > 1 else pages
+        _need(stride >= pages, "the rows of page_table overlap")
+        self.info = BatchInfo(page_table.data_ptr(), context.data_ptr(), cu_tokens.data_ptr() if cu_tokens is not None else 0,
+                              stride, n, pages, tokens, max_tokens, max_context, 0)
+        self.device, self.tokens = device, tokens
+        self._keep = (page_table, context, cu_tokens)
+        self._ref = C.byref(self.info)
+
+
+class Rotation:
+    """Tables float32 [rows, pairs]; sections: how many pairs each axis has (None: one axis); interleaved: pairs are
+    (2i, 2i + 1) and not (i, i + pairs)."""
+
+    def __init__(self, cos, sin, sections=None, interleaved=False):
+        self.device = _device(cos)
+        for t in (cos, sin):
+            _is(t, "torch.float32", self.device, "a table of the rotation")
+            _need(len(t.shape) == 2 and tuple(t.shape) == tuple(cos.shape) and t.stride() == (t.shape[1], 1), "the tables are not [rows, pairs] and contiguous")
+        sections = tuple(sections) if sections else (cos.shape[1],)
+        _need(len(sections) <= MAX_AXES and sum(sections) == cos.shape[1] and min(sections) >= 0, "sections are not the pairs of the axes")
+        self.axes = len(sections)
+        self.sections = (C.c_int32 * MAX_AXES)(*sections)
+        self.rows, self.dim, self.interleaved = cos.shape[0], 2 * cos.shape[1], int(interleaved)
+        self.cos, self.sin = cos.data_ptr(), sin.data_ptr()
+        self._keep = (cos, sin)
+
+
+def _rows(t, tokens, heads, dim, kind, device, what):
+    """Strides of a tensor [tokens, heads, dim]."""
+    shape, at = t.shape, t.stride()
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != dim or (heads and shape[1] != heads) or at[2] != 1:
+        raise ValueError("%s is not [%d, %s, %d] with contiguous dims" % (what, tokens, heads or "heads", dim))
+    if _TYPES.get(str(t.dtype)) != kind:
+        raise ValueError("%s has another type than the rows" % what)
+    if _device(t) != device:
+        raise ValueError("%s is on another device than the cache" % what)
+    return at
+
+
+def append(cache, batch, k, v, q=None, q_out=None, rotation=None, positions=None, stream=0):
+    """Rows k and v [tokens, heads, dim] into the cache, k rotated; q rotated into q_out."""
+    n, dim, device = batch.tokens, cache.dim, cache.device
+    kind = _TYPES.get(str(k.dtype))
+    _need(kind in (BF16, F16), "k is not bfloat16 or float16")
+    _need(batch.device == device and (rotation is None or rotation.device == device), "tensors are on different devices")
+    ak = _rows(k, n, cache.heads, dim, kind, device, "k")
+    av = _rows(v, n, cache.heads, dim, kind, device, "v")
+    a = AppendArgs(k.data_ptr(), v.data_ptr(), 0, 0, 0, 0, 0, ak[0], ak[1], av[0], av[1], 0, 0, 0, 0, 0, kind)
+    if q is not None:
+        _need(q_out is not None, "q without q_out")
+        a.q_heads = q.shape[1]
+        a.q_token_stride, a.q_head_stride = _rows(q, n, 0, dim, kind, device, "q")[:2]
+        a.q_out_token_stride, a.q_out_head_stride = _rows(q_out, n, q.shape[1], dim, kind, device, "q_out")[:2]
+        a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
+    if rotation is not None:
+        _need(rotation.axes == 1 or positions is not None, "several axes need positions")
+        a.cos, a.sin, a.rotary_dim, a.interleaved = rotation.cos, rotation.sin, rotation.dim, rotation.interleaved
+        a.table_rows, a.axes, a.sections = rotation.rows, rotation.axes, rotation.sections
+        if positions is not None:
+            _is(positions, "torch.int32", device, "positions")
+            shape, at = tuple(positions.shape), positions.stride()
+            _need(shape == (rotation.axes, n) or (rotation.axes == 1 and shape == (n,)), "positions are not [axes, tokens]")
+            _need(n < 2 or at[-1] == 1, "positions are not contiguous")
+            a.positions, a.positions_stride = positions.data_ptr(), at[0] if rotation.axes > 1 else n
+    else:
+        _need(positions is None, "positions without rotation")
+    _call("amem_kv_append", cache._ref, batch._ref, C.byref(a), stream)
+
+
+def attention_workspace(cache, batch, q_heads):
+    """Bytes of workspace that `attention` needs for these sizes."""
+    n = C.c_uint64()
+    _call("amem_kv_attention_workspace", cache._ref, batch._ref, q_heads, C.byref(n))
+    return n.value
+
+
+def attention(cache, batch, q, out, lse=None, scale=None, causal=True, window=0, workspace=None, stream=0):
+    """out [tokens, heads, dim] = attention of q over the cache; lse float32 [tokens, heads]; scale: dim ** -0.5 if None;
+    workspace: a contiguous tensor of at least attention_workspace() bytes."""
+    n, dim, device = batch.tokens, cache.dim, cache.device
+    kind, heads = _TYPES.get(str(q.dtype)), q.shape[1]
+    _need(kind in (BF16, F16), "q is not bfloat16 or float16")
+    _need(batch.device == device, "the batch is on another device than the cache")
+    aq = _rows(q, n, 0, dim, kind, device, "q")
+    ao = _rows(out, n, heads, dim, kind, device, "out")
+    lse_at = at = size = 0
+    if lse is not None:
+        _is(lse, "torch.float32", device, "lse")
+        _need(tuple(lse.shape) == (n, heads) and lse.is_contiguous(), "lse is not [tokens, heads] and contiguous")
+        lse_at = lse.data_ptr()
+    if workspace is not None:
+        _need(_device(workspace) == device and workspace.is_contiguous(), "workspace is on another device, or strided")
+        at, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    a = AttentionArgs(q.data_ptr(), out.data_ptr(), lse_at, at, size, aq[0], aq[1], ao[0], ao[1],
+                      dim ** -0.5 if scale is None else scale, kind, heads, int(causal), window, 0)
+    _call("amem_kv_attention", cache._ref, batch._ref, C.byref(a), stream)
