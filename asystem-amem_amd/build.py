@@ -12,7 +12,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIBNAME = "libamem_nccl.so.1"
 HOOK_NAME = "libamem_rccl_hook.so"
-HIP_SOURCES = ["kernels.hip", "kv_append.hip", "kv_attention.hip"]
+HIP_SOURCES = ["kernels.hip", "kv_append.hip", "kv_attend_few.hip", "kv_attention.hip"]
 CXX_SOURCES = ["capi.cpp", "engine.cpp", "ipc.cpp", "kv_api.cpp", "log.cpp", "slab_pool.cpp", "vmm.cpp"]
 # The packed-fp32 target feature is switched off for all device code of this project.
 DEVICE_FLAGS = ["--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]

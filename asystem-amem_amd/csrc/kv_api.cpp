@@ -57,6 +57,7 @@ int check_cache(const char* what, const amem_kv_cache* c, bool addresses, KvCach
   NEED(fits(c->pages, c->page_stride) && fits(c->kv_heads, c->head_stride) && fits(c->page_slots, c->slot_stride) &&
            fits(c->pages, c->scale_page_stride) && fits(c->kv_heads, c->scale_head_stride),
        "the cache is larger than addresses");
+  NEED((c->slot_stride * element) << page_shift < (int64_t)1 << 31, "the slots of a page are 2^31 bytes or more apart");
   NEED(c->reserved == 0, "cache.reserved is not 0");
   if (addresses) {
     NEED(c->k && c->v && c->k % 16 == 0 && c->v % 16 == 0, "cache addresses are not aligned to 16 bytes");
@@ -193,6 +194,7 @@ int amem_kv_attention_workspace(const amem_kv_cache* cache, const amem_kv_batch*
   if (int e = check_cache(what, cache, false, &c)) return e;
   if (int e = check_batch(what, batch, c, false, &b)) return e;
   NEED(q_heads >= 1 && q_heads <= 1024 && q_heads % c.kv_heads == 0, "q_heads is not a multiple of kv_heads");
+  NEED((int64_t)b.tokens * q_heads < 1 << 30, "tokens * q_heads is 2^30 or more");
   NEED(bytes, "bytes is NULL");
   *bytes = kv_attend_workspace(c, b, q_heads, batch->max_tokens, cache->head_dim);
   return 0;
@@ -213,6 +215,7 @@ int amem_kv_attention(const amem_kv_cache* cache, const amem_kv_batch* batch, co
     if (int e = check_rows(what, "address or strides of q", a->q, a->q_token_stride, a->q_head_stride, b.tokens, a->q_heads)) return e;
     if (int e = check_rows(what, "address or strides of out", a->out, a->out_token_stride, a->out_head_stride, b.tokens, a->q_heads)) return e;
   }
+  NEED((int64_t)b.tokens * a->q_heads < 1 << 30, "tokens * q_heads is 2^30 or more");
   NEED(a->lse % 4 == 0, "address of lse");
   NEED(a->window >= 0, "window is negative");
   NEED(a->scale - a->scale == 0, "scale is not finite");

@@ -1,0 +1,581 @@
+// Attention over a paged key/value cache for few rows: single tokens, drafted tokens, up to 64 rows that share a
+// key/value head (the rows of a sequence are its new tokens times the query heads of that head's group).
+//
+//   s_p = scale q.k_p,  m = max s_p,  l = sum exp(s_p - m),  out = sum exp(s_p - m) v_p / l,  lse = m + log l
+//
+// Bound by reading keys and values once; the arithmetic has to hide behind that. Four waves of a workgroup take tiles of a
+// stretch of positions in turn, each with m, l and a sum of its own, and join them in LDS at the end. Longer
+// contexts are cut into several stretches (workgroups), whose parts a second kernel joins.
+//
+// Both products run on the matrix unit as (keys x dims)(dims x rows) and (dims x keys)(keys x rows), so that a lane
+// holds scores and sums of one row: the softmax needs two exchanges between lanes a tile. Keys go from memory to the
+// operand's registers; values pass through LDS, wave by wave, to be read as columns. A tile's registers are
+// loaded again for the next tile as soon as the matrix unit, or LDS, has taken them.
+#include <algorithm>
+
+#include "kv_device.h"
+
+namespace amem {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kTarget = 2048;  // workgroups that a call is cut into, where its contexts are long enough
+
+// How a call's rows and positions are dealt out.
+struct Few {
+  int stretch;   // positions of a workgroup, a multiple of kWaves * 64
+  int splits;    // most stretches of a unit
+  float* sums;   // [unit][kv head][split][row][dim]
+  float* stats;  // [unit][kv head][split][row]{m, l}, m in units of log 2
+};
+
+// A unit: some rows of one sequence (row r is head r % group of new token r / group), and the positions they see.
+struct Unit {
+  int s, first, rows;  // the sequence, the first of its rows, how many
+  int lo, to;          // positions that some row sees: [lo, to)
+  int from;            // lo, down to a multiple of 64
+  int all_from, all_to;  // positions that every row sees
+};
+
+__device__ __forceinline__ void row_range(const KvAttend& a, const KvSeq& q, int token, int& from, int& to) {
+  const int pos = q.context - q.n + token;
+  to = a.causal && pos + 1 < q.context ? pos + 1 : q.context;
+  from = a.window && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
+}
+
+__device__ __forceinline__ bool find_unit(const KvBatch& b, const KvAttend& a, int group, int shift, int index, KvSeq& q, Unit& u) {
+  u.s = b.cu_tokens ? find_sequence(b, index, shift, 1, group) : 0;
+  if (!b.cu_tokens) {
+    // every sequence has the same number of units
+    const int each = ((b.uniform * group - 1) >> shift) + 1;
+    u.s = index / each;
+    index -= u.s * each;
+    if (u.s >= b.sequences) return false;
+  } else {
+    if (u.s < 0) return false;
+    index -= kv_unit_base(b, u.s, shift, 1, group);
+  }
+  q = kv_seq(b, u.s);
+  u.first = index << shift;
+  u.rows = q.n * group - u.first;
+  if (u.rows <= 0) return false;
+  if (u.rows > 1 << shift) u.rows = 1 << shift;
+  row_range(a, q, u.first / group, u.lo, u.all_to);
+  row_range(a, q, (u.first + u.rows - 1) / group, u.all_from, u.to);
+  u.from = u.lo & ~63;
+  return true;
+}
+
+// D dims, 16 bits of fp16 (HALF) or bf16, a cache of e4m3 (EIGHT), NB blocks of 16 rows, pages of at least 16 slots (WIDE).
+template <int D, bool HALF, bool EIGHT, int NB, bool WIDE>
+__global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_few(KvCache c, KvBatch b, KvAttend a, Few few) {
+  constexpr int kElement = EIGHT ? 1 : 2;
+  constexpr int kTile = EIGHT ? 64 : 32;               // positions of a tile
+  constexpr int kGroups = kTile / 16;                  // of 16 positions: rows of an operand, and never over a page's end
+  constexpr int kLoads = D * kElement / 64;            // 16-byte loads of a lane for a group's keys
+  constexpr int kRowLanes = D * kElement / 16;         // lanes that read a position's values
+  constexpr int kRowsALoad = kWave / kRowLanes;
+  constexpr int kValueLoads = kTile / kRowsALoad;
+  // a row of values in LDS: its pad puts the rows that are read together on different banks
+  constexpr int kPitch = D * kElement + (EIGHT ? 16 : 32);
+  constexpr int kBlocks = D / 16;
+  constexpr bool kHalfP = EIGHT || HALF;  // weights are fp16 where the values' type allows it
+  // fp16 weights are held 2^8 times larger, which keeps small ones out of the subnormal numbers
+  constexpr float kLift = kHalfP ? 8.0f : 0.0f;
+  constexpr int kLds = kWaves * kTile * kPitch, kJoin = kWaves * 16 * (D + 4) * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kLds > kJoin ? kLds : kJoin];
+  __shared__ float lds_m[kWaves][16 * NB], lds_l[kWaves][16 * NB];
+
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int group = a.q_heads / c.kv_heads, kvh = blockIdx.y, split = blockIdx.z;
+  constexpr int shift = NB == 1 ? 4 : NB == 2 ? 5 : 6;
+  KvSeq q;
+  Unit u;
+  if (!find_unit(b, a, group, shift, blockIdx.x, q, u)) return;
+  const int begin = u.from + split * few.stretch;
+  if (split && (begin >= u.to || q.bad)) return;
+  const int end = begin + few.stretch < u.to ? begin + few.stretch : u.to;
+  const int col = lane & 15, quad = lane >> 4;
+
+  // queries: the operand of a block of rows, dims in the order of the keys' registers
+  u32x4 qr[NB][D / 32];
+  int row_from[NB], row_to[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    int r = n * 16 + col;
+    if (r >= u.rows) r = u.rows - 1;
+    r += u.first;
+    const int token = r / group;
+    row_range(a, q, token, row_from[n], row_to[n]);
+    const uint16_t* p = a.q + (q.row + token) * a.q_token + (kvh * group + r % group) * a.q_head;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) {
+      const int d = EIGHT ? (t / 2) * 64 + quad * 16 + (t % 2) * 8 : t * 32 + quad * 8;
+      qr[n][t] = *(const u32x4*)(p + d);
+    }
+  }
+
+  float m[NB], l[NB];
+  f32x4 sum[NB][kBlocks];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    m[n] = -kInf;
+    l[n] = 0;
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) sum[n][i] = f32x4{0, 0, 0, 0};
+  }
+  float unit_scale = 0;  // the sums are in multiples of it; the largest scale of values so far (8 bits)
+
+  uint8_t* const mine = lds + wave * kTile * kPitch;
+  const uint8_t* const keys = c.k + (int64_t)kvh * c.head_stride;
+  const int64_t values_off = c.v - c.k;
+  const int slot_mask = (1 << c.page_shift) - 1;
+  // where this lane writes its values, and reads columns. 8 bits: a lane reads eight rows as one column, which are to be
+  // the positions of its eight weights, so position r of 32 goes to row 8 ((r % 16) / 4) + 4 (r / 16) + r % 4
+  const int value_row = lane / kRowLanes, value_col = lane % kRowLanes * 16;
+  auto lds_row = [](int r) { return EIGHT ? (r & ~31) + 8 * ((r & 15) >> 2) + 4 * ((r & 31) >> 4) + (r & 3) : r; };
+  const int write_at = lds_row(value_row) * kPitch + value_col;
+  const int read_at = EIGHT ? (8 * quad + (col >> 1)) * kPitch + (col & 1) * 8 : (4 * quad + (col >> 2)) * kPitch + (col & 3) * 8;
+
+  u32x4 kreg[kGroups][kLoads], vreg[kValueLoads];
+  int page = 0, page_next = 0;           // of position base + lane
+  float ks = 0, vs = 0, ks_next = 0, vs_next = 0;
+
+  auto look_up = [&](int base) {  // page of base + lane: 0 where there is none, -1 where it is out of range
+    const int p = base + lane;
+    return p < u.to && (kTile == kWave || lane < kTile) ? kv_page(c, b, u.s, p) : 0;
+  };
+  auto row_of = [&](int page, int p) {
+    return keys + ((int64_t)(page < 0 ? 0 : page) * c.page_stride + (int64_t)(p & slot_mask) * c.slot_stride);
+  };
+  // offsets of this lane in a group that lies in one page: 32 bits, since a page's rows span less than 2^31 bytes
+  const uint32_t key_off = (uint32_t)(col * (int)c.slot_stride + quad * 16);
+  const uint32_t value_off = (uint32_t)((value_row & 15) * (int)c.slot_stride + value_col);
+  auto load_keys = [&](int base, int page) {
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      if constexpr (WIDE) {
+        const uint8_t* at = row_of(__builtin_amdgcn_readlane(page, g * 16), base + g * 16);
+#pragma unroll
+        for (int t = 0; t < kLoads; ++t) kreg[g][t] = *(const u32x4*)(at + t * 64 + key_off);
+      } else {
+        const uint8_t* at = row_of(__shfl(page, g * 16 + col, kWave), base + g * 16 + col) + quad * 16;
+#pragma unroll
+        for (int t = 0; t < kLoads; ++t) kreg[g][t] = *(const u32x4*)(at + t * 64);
+      }
+    }
+  };
+  auto load_values = [&](int base, int page) {
+#pragma unroll
+    for (int i = 0; i < kValueLoads; ++i) {
+      if constexpr (WIDE) {
+        const int r = i * kRowsALoad;
+        const uint8_t* at = row_of(__builtin_amdgcn_readlane(page, r & ~15), base + r) + values_off;
+        vreg[i] = *(const u32x4*)(at + value_off);
+      } else {
+        const int r = i * kRowsALoad + value_row;
+        vreg[i] = *(const u32x4*)(row_of(__shfl(page, r, kWave), base + r) + values_off + value_col);
+      }
+    }
+  };
+  auto load_scales = [&](int base, int page, float& k, float& v) {
+    if constexpr (EIGHT) {
+      const int p = base + lane;
+      k = v = 0;
+      if (p < u.to && (p | 15) >= u.lo) {  // a hidden group's scale may be anything
+        const int64_t at = kv_scale_offset(c, page < 0 ? 0 : page, kvh, p);
+        k = c.k_scale[at];
+        v = c.v_scale[at];
+      }
+    }
+  };
+
+  int base = begin + wave * kTile;
+  constexpr int kStep = kWaves * kTile;
+  if (base < end) {
+    page = look_up(base);
+    load_keys(base, page);
+    load_scales(base, page, ks, vs);
+    load_values(base, page);
+    if (base + kStep < end) page_next = look_up(base + kStep);
+  }
+  for (; base < end; base += kStep) {
+    const bool more = base + kStep < end;
+    const bool whole = base >= u.all_from && base + kTile <= u.all_to;
+    f32x4 score[NB][kGroups];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t) {
+          if constexpr (EIGHT) x = mfma16<HALF>(widen<HALF>(u32x2{kreg[g][t / 2][t % 2 * 2], kreg[g][t / 2][t % 2 * 2 + 1]}), qr[n][t], x);
+          else x = mfma16<HALF>(kreg[g][t], qr[n][t], x);
+        }
+        score[n][g] = x;
+      }
+    if (more) load_keys(base + kStep, page_next);
+
+    // scores in units of log 2
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const float f = a.scale * kLog2e * (EIGHT ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), g * 16)) : 1.0f);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) score[n][g] *= f;
+    }
+    // values that no row sees are stored as zeros, since a weight of zero does not hide infinities and NaN
+    bool odd = false;  // some positions have such values, and may be hidden from some rows
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < kValueLoads; ++i) {
+        const int p = base + i * kRowsALoad + value_row;
+        if (p < u.lo || p >= u.to) vreg[i] = u32x4{0, 0, 0, 0};
+        // those are taken out of the product and added one by one below
+        const uint64_t lanes = __ballot(not_finite<HALF, EIGHT>(vreg[i]));
+        if (lanes) {
+          odd = true;
+          if (lanes >> (value_row * kRowLanes) & ((1ull << kRowLanes) - 1)) vreg[i] = u32x4{0, 0, 0, 0};
+        }
+      }
+      const uint64_t bad = __ballot(page < 0);
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = g * 16 + quad * 4 + i, p = base + k;
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            if (bad >> k & 1) score[n][g][i] = __builtin_nanf("");
+            if (p < row_from[n] || p >= row_to[n]) score[n][g][i] = -kInf;
+          }
+        }
+    } else if (__any(page < 0)) {
+      const uint64_t bad = __ballot(page < 0);
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+            if (bad >> (g * 16 + quad * 4 + i) & 1) score[n][g][i] = __builtin_nanf("");
+    }
+#pragma unroll
+    for (int i = 0; i < kValueLoads; ++i) *(u32x4*)(mine + write_at + lds_row(i * kRowsALoad) * kPitch) = vreg[i];
+    __builtin_amdgcn_wave_barrier();
+    const float vs_now = vs;
+    const int page_now = page;
+    if (more) {
+      load_scales(base + kStep, page_next, ks_next, vs_next);
+      load_values(base + kStep, page_next);
+      page = page_next;
+      ks = ks_next;
+      vs = vs_next;
+      if (base + 2 * kStep < end) page_next = look_up(base + 2 * kStep);
+    }
+
+    // running maximum; where it grows, what has been summed shrinks
+    bool grew = false;
+    float shrink[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      float top = score[n][0][0];
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = __builtin_elementwise_maximum(top, score[n][g][i]);  // NaN stays
+      top = __builtin_elementwise_maximum(top, __shfl_xor(top, 16, kWave));
+      top = __builtin_elementwise_maximum(top, __shfl_xor(top, 32, kWave));
+      const float now = __builtin_elementwise_maximum(m[n], top);
+      shrink[n] = now == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - now);
+      grew |= now != m[n];
+      m[n] = now;
+    }
+    float f_scale[kGroups];
+    if constexpr (EIGHT) {
+      float top = 0;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        f_scale[g] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs_now), g * 16));
+        top = __builtin_elementwise_maximum(top, f_scale[g]);
+      }
+      if (!(top <= unit_scale)) {
+        const float f = unit_scale / top;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int i = 0; i < kBlocks; ++i) sum[n][i] *= f;
+        unit_scale = top;
+      }
+      const float f = unit_scale > 0 ? 1.0f / unit_scale : 0.0f;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) f_scale[g] *= f;
+    }
+    if (__any(grew)) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        l[n] *= shrink[n];
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) sum[n][i] *= shrink[n];
+      }
+    }
+    u32x4 w[NB][kGroups / 2];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const float top = (m[n] == -kInf ? 0.0f : m[n]) - kLift;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = __builtin_amdgcn_exp2f(score[n][g][i] - top);
+          l[n] += x[i];
+          if constexpr (EIGHT) x[i] *= f_scale[g];
+          score[n][g][i] = x[i];
+        }
+        w[n][g / 2][g % 2 * 2] = pack<kHalfP>(x[0], x[1]);
+        w[n][g / 2][g % 2 * 2 + 1] = pack<kHalfP>(x[2], x[3]);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < kTile / 32; ++t)
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) {
+        const uint8_t* p = mine + read_at + t * 32 * kPitch + i * 16 * kElement;
+        u32x4 v;
+        if constexpr (EIGHT) {
+          v = widen<true>(read_columns8(p));
+        } else {
+          const u32x2 lo = read_columns16(p), hi = read_columns16(p + 16 * kPitch);
+          v = u32x4{lo[0], lo[1], hi[0], hi[1]};
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n) sum[n][i] = mfma16<kHalfP>(v, w[n][t], sum[n][i]);
+      }
+    __builtin_amdgcn_wave_barrier();
+    if (odd) {
+      // one position after the other: its values through LDS, its weights from the lanes that hold them
+#pragma unroll 1
+      for (int k = 0; k < kTile; ++k) {
+        const int p = base + k;
+        if (p < u.lo || p >= u.to) continue;
+        const uint8_t* at = row_of(__builtin_amdgcn_readlane(page_now, k), p) + values_off;
+        u32x4 v = {0, 0, 0, 0};
+        if (lane < kRowLanes) v = *(const u32x4*)(at + lane * 16);
+        if (!__any(not_finite<HALF, EIGHT>(v))) continue;
+        if (lane < kRowLanes) *(u32x4*)(mine + lane * 16) = v;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          float x = 0;
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (g == k / 16 && e == k % 4) x = score[n][g][e];
+          x = __shfl(x, (k % 16 / 4) * 16 + col, kWave);
+          if (p < row_from[n] || p >= row_to[n]) continue;
+#pragma unroll
+          for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i = d * 16 + quad * 4 + e;
+              if constexpr (EIGHT) sum[n][d][e] += x * __builtin_amdgcn_cvt_f32_fp8((int)mine[i], 0);
+              else sum[n][d][e] += x * to_float<HALF>(((const uint16_t*)mine)[i]);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+  }
+
+  // the four waves' parts become one
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    l[n] += __shfl_xor(l[n], 16, kWave);
+    l[n] += __shfl_xor(l[n], 32, kWave);
+    if (lane < 16) {
+      lds_m[wave][n * 16 + lane] = m[n];
+      lds_l[wave][n * 16 + lane] = l[n];
+    }
+  }
+  const int64_t part = ((int64_t)blockIdx.x * c.kv_heads + kvh) * few.splits + split;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    __syncthreads();
+    float top = lds_m[0][n * 16 + col];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) top = __builtin_elementwise_maximum(top, lds_m[i][n * 16 + col]);
+    const float f = (m[n] == top ? 1.0f : __builtin_amdgcn_exp2f(m[n] - top)) * (EIGHT && unit_scale > 0 ? unit_scale : 1.0f);
+    float* at = (float*)lds + (wave * 16 + col) * (D + 4) + quad * 4;
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) *(f32x4*)(at + i * 16) = sum[n][i] * f;
+    __syncthreads();
+    constexpr int kVectors = 16 * D / 4;
+#pragma unroll
+    for (int v0 = 0; v0 < kVectors; v0 += kWaves * kWave) {
+      const int v = v0 + threadIdx.x, r = v / (D / 4), d = v % (D / 4) * 4;
+      if (kVectors % (kWaves * kWave) && v >= kVectors) break;
+      if (n * 16 + r >= u.rows) continue;
+      float mm = lds_m[0][n * 16 + r];
+#pragma unroll
+      for (int i = 1; i < kWaves; ++i) mm = __builtin_elementwise_maximum(mm, lds_m[i][n * 16 + r]);
+      float ll = 0;
+      f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) {
+        const float mi = lds_m[i][n * 16 + r];
+        ll += lds_l[i][n * 16 + r] * (mi == mm ? 1.0f : __builtin_amdgcn_exp2f(mi - mm));
+        x += *(const f32x4*)((const float*)lds + (i * 16 + r) * (D + 4) + d);
+      }
+      if (few.splits > 1) {
+        const int64_t row = part * (16 * NB) + n * 16 + r;
+        *(f32x4*)(few.sums + row * D + d) = x;
+        if (d == 0) {
+          few.stats[row * 2] = mm;
+          few.stats[row * 2 + 1] = ll;
+        }
+        continue;
+      }
+      const int rr = u.first + n * 16 + r, token = rr / group, head = kvh * group + rr % group;
+      const float inverse = q.bad ? __builtin_nanf("") : ll == 0 ? 0.0f : 1.0f / ll;
+      if (ll == 0) x = f32x4{0, 0, 0, 0};
+      *(u32x2*)(a.out + (q.row + token) * a.out_token + head * a.out_head + d) =
+          u32x2{pack<HALF>(x[0] * inverse, x[1] * inverse), pack<HALF>(x[2] * inverse, x[3] * inverse)};
+      if (a.lse && d == 0)
+        a.lse[(int64_t)(q.row + token) * a.q_heads + head] = q.bad ? __builtin_nanf("") : ll == 0 ? -kInf : ((mm - kLift) + __builtin_amdgcn_logf(ll)) * kLn2;
+    }
+  }
+}
+
+// Joins the stretches of a row: one workgroup for a row and query head, the waves take stretches in turn.
+template <int D, bool HALF>
+__global__ __launch_bounds__(kWaves * kWave) void join_stretches(KvCache c, KvBatch b, KvAttend a, Few few, int shift, float lift) {
+  const int group = a.q_heads / c.kv_heads, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int rows = 1 << shift, kvh = blockIdx.y, row = blockIdx.x & (rows - 1), index = blockIdx.x >> shift;
+  KvSeq q;
+  Unit u;
+  if (!find_unit(b, a, group, shift, index, q, u) || row >= u.rows) return;
+  int parts = (u.to - u.from + few.stretch - 1) / few.stretch;
+  parts = q.bad || parts < 1 ? 1 : parts > few.splits ? few.splits : parts;
+  const int64_t first = ((int64_t)index * c.kv_heads + kvh) * few.splits;
+  constexpr int N = D / kWave;
+  float m = -kInf, l = 0, x[N] = {};
+  for (int i = wave; i < parts; i += kWaves) {
+    const int64_t at = (first + i) * rows + row;
+    const float mi = few.stats[at * 2], li = few.stats[at * 2 + 1];
+    const float now = __builtin_elementwise_maximum(m, mi);
+    const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now), g = mi == now ? 1.0f : __builtin_amdgcn_exp2f(mi - now);
+    m = now;
+    l = l * f + li * g;
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = x[j] * f + few.sums[at * D + j * kWave + lane] * g;
+  }
+  __shared__ float part[kWaves][D], stat[kWaves][2];
+#pragma unroll
+  for (int j = 0; j < N; ++j) part[wave][j * kWave + lane] = x[j];
+  if (lane == 0) { stat[wave][0] = m; stat[wave][1] = l; }
+  __syncthreads();
+  m = stat[0][0];
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) m = __builtin_elementwise_maximum(m, stat[i][0]);
+  float f[kWaves];
+  l = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    f[i] = stat[i][0] == m ? 1.0f : __builtin_amdgcn_exp2f(stat[i][0] - m);
+    l += stat[i][1] * f[i];
+  }
+  const int rr = u.first + row, token = rr / group, head = kvh * group + rr % group;
+  for (int d = threadIdx.x; d < D; d += kWaves * kWave) {
+    float y = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) y += part[i][d] * f[i];
+    y = q.bad ? __builtin_nanf("") : l == 0 ? 0.0f : y / l;
+    a.out[(q.row + token) * a.out_token + head * a.out_head + d] = from_float<HALF>(y);
+  }
+  if (a.lse && threadIdx.x == 0)
+    a.lse[(int64_t)(q.row + token) * a.q_heads + head] = q.bad ? __builtin_nanf("") : l == 0 ? -kInf : ((m - lift) + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+int units_of(const KvBatch& b, int group, int shift) {
+  return b.cu_tokens ? kv_units(b, shift, 1, group) : b.sequences * (((b.uniform * group - 1) >> shift) + 1);
+}
+
+// Blocks of 16 rows that a workgroup takes: enough for all rows of a sequence's key/value head, so that its keys and
+// values are read once.
+int blocks_of(int group, int max_tokens, int head_dim) {
+  const int64_t rows = (int64_t)group * max_tokens;
+  return rows <= 16 ? 1 : rows <= 32 || head_dim == 256 ? 2 : 4;
+}
+
+// Stretches are as long as leaves about kTarget workgroups (eight for each compute unit, of which it holds two to four at a
+// time), and at least a tile for each wave.
+void plan(const KvCache& c, const KvBatch& b, int group, int blocks, int window, Few* few) {
+  const int shift = blocks == 1 ? 4 : blocks == 2 ? 5 : 6;
+  int64_t span = b.max_context;
+  const int64_t seen = (int64_t)window + (16 * blocks) / group + 1 + 64;
+  if (window && seen < span) span = seen;
+  const int64_t all = (int64_t)units_of(b, group, shift) * c.kv_heads * span;
+  const int64_t step = kWaves * 64;
+  int64_t stretch = ((all + kTarget - 1) / kTarget + step - 1) / step * step;
+  if (stretch < step) stretch = step;
+  few->stretch = (int)stretch;
+  few->splits = span > stretch ? (int)((span + stretch - 1) / stretch) : 1;
+}
+
+template <int D, bool HALF, bool EIGHT, int NB>
+hipError_t launch_few(const KvCache& c, const KvBatch& b, const KvAttend& a, const Few& few, hipStream_t stream) {
+  const int group = a.q_heads / c.kv_heads, shift = NB == 1 ? 4 : NB == 2 ? 5 : 6;
+  const int units = units_of(b, group, shift);
+  const dim3 grid(units, c.kv_heads, few.splits);
+  if constexpr (!EIGHT) {
+    if (c.page_shift < 4) attend_few<D, HALF, EIGHT, NB, false><<<grid, kWaves * kWave, 0, stream>>>(c, b, a, few);
+    else attend_few<D, HALF, EIGHT, NB, true><<<grid, kWaves * kWave, 0, stream>>>(c, b, a, few);
+  } else {
+    attend_few<D, HALF, EIGHT, NB, true><<<grid, kWaves * kWave, 0, stream>>>(c, b, a, few);
+  }
+  if (hipError_t e = hipGetLastError(); e != hipSuccess || few.splits == 1) return e;
+  join_stretches<D, HALF><<<dim3(units << shift, c.kv_heads), kWaves * kWave, 0, stream>>>(c, b, a, few, shift, EIGHT || HALF ? 8.0f : 0.0f);
+  return hipGetLastError();
+}
+
+template <int D, bool HALF, bool EIGHT>
+hipError_t launch_blocks(const KvCache& c, const KvBatch& b, const KvAttend& a, const Few& few, int blocks, hipStream_t stream) {
+  if (blocks == 1) return launch_few<D, HALF, EIGHT, 1>(c, b, a, few, stream);
+  if (blocks == 2) return launch_few<D, HALF, EIGHT, 2>(c, b, a, few, stream);
+  if constexpr (D < 256) return launch_few<D, HALF, EIGHT, 4>(c, b, a, few, stream);
+  return hipErrorInvalidValue;
+}
+
+template <int D>
+hipError_t launch_dims(const KvCache& c, const KvBatch& b, const KvAttend& a, bool half, bool eight, const Few& few, int blocks, hipStream_t stream) {
+  if (half) return eight ? launch_blocks<D, true, true>(c, b, a, few, blocks, stream) : launch_blocks<D, true, false>(c, b, a, few, blocks, stream);
+  return eight ? launch_blocks<D, false, true>(c, b, a, few, blocks, stream) : launch_blocks<D, false, false>(c, b, a, few, blocks, stream);
+}
+
+}  // namespace
+
+uint64_t kv_attend_few_workspace(const KvCache& c, const KvBatch& b, int q_heads, int max_tokens, int head_dim) {
+  // for any window: plan() has at most that many splits
+  const int group = q_heads / c.kv_heads, blocks = blocks_of(group, max_tokens, head_dim);
+  const int shift = blocks == 1 ? 4 : blocks == 2 ? 5 : 6;
+  const int64_t units = (int64_t)units_of(b, group, shift) * c.kv_heads;
+  if (!units) return 0;
+  const int64_t splits = std::min<int64_t>((b.max_context + kWaves * 64 - 1) / (kWaves * 64), (kTarget + units - 1) / units);
+  return splits < 2 ? 0 : (uint64_t)(units * splits * (16 * blocks)) * (head_dim + 2) * 4;
+}
+
+hipError_t launch_kv_attend_few(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream) {
+  const int group = a.q_heads / c.kv_heads, blocks = blocks_of(group, a.max_tokens, head_dim);
+  Few few;
+  plan(c, b, group, blocks, a.window, &few);
+  const int shift = blocks == 1 ? 4 : blocks == 2 ? 5 : 6;
+  few.sums = (float*)a.workspace;
+  few.stats = few.sums + (int64_t)units_of(b, group, shift) * c.kv_heads * few.splits * (16 * blocks) * head_dim;
+  if (head_dim == 64) return launch_dims<64>(c, b, a, half, eight, few, blocks, stream);
+  if (head_dim == 128) return launch_dims<128>(c, b, a, half, eight, few, blocks, stream);
+  return launch_dims<256>(c, b, a, half, eight, few, blocks, stream);
+}
+
+}  // namespace amem

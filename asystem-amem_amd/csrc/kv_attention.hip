@@ -95,9 +95,16 @@ hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, bool ha
 
 }  // namespace
 
-uint64_t kv_attend_workspace(const KvCache&, const KvBatch&, int, int, int) { return 0; }
+static bool few_rows(int q_heads, int kv_heads, int max_tokens, int head_dim) {
+  return (int64_t)(q_heads / kv_heads) * max_tokens <= (head_dim == 256 ? 32 : 64);
+}
+
+uint64_t kv_attend_workspace(const KvCache& c, const KvBatch& b, int q_heads, int max_tokens, int head_dim) {
+  return few_rows(q_heads, c.kv_heads, max_tokens, head_dim) ? kv_attend_few_workspace(c, b, q_heads, max_tokens, head_dim) : 0;
+}
 
 hipError_t launch_kv_attend(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream) {
+  if (few_rows(a.q_heads, c.kv_heads, a.max_tokens, head_dim)) return launch_kv_attend_few(c, b, a, head_dim, half, eight, stream);
   if (head_dim == 64) return launch<64>(c, b, a, half, eight, stream);
   if (head_dim == 128) return launch<128>(c, b, a, half, eight, stream);
   return launch<256>(c, b, a, half, eight, stream);
