@@ -8,9 +8,9 @@
 // contexts are cut into several stretches (workgroups), whose parts a second kernel joins.
 //
 // Both products run on the matrix unit as (keys x dims)(dims x rows) and (dims x keys)(keys x rows), so that a lane
-// holds scores and sums of one row: the softmax needs two exchanges between lanes a tile. Keys go from memory to the
-// operand's registers; values pass through LDS, wave by wave, to be read as columns. A tile's registers are
-// loaded again for the next tile as soon as the matrix unit, or LDS, has taken them.
+// holds scores and sums of one row: the softmax needs two exchanges between lanes a tile. Keys and values are loaded as
+// they lie, whole lines by one instruction, past the caches (nothing reads them twice), and pass through LDS, wave
+// by wave, to become operands. A tile's registers are loaded again for the next tile as soon as LDS has them.
 #include <algorithm>
 
 #include "kv_device.h"
@@ -19,11 +19,12 @@ namespace amem {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kTarget = 2048;  // workgroups that a call is cut into, where its contexts are long enough
+constexpr int kTarget = 512;  // workgroups that a call is cut into, where its contexts are long enough
 
 // How a call's rows and positions are dealt out.
 struct Few {
   int stretch;   // positions of a workgroup, a multiple of kWaves * 64
+  int units;
   int splits;    // most stretches of a unit
   float* sums;   // [unit][kv head][split][row][dim]
   float* stats;  // [unit][kv head][split][row]{m, l}, m in units of log 2
@@ -43,20 +44,10 @@ __device__ __forceinline__ void row_range(const KvAttend& a, const KvSeq& q, int
   from = a.window && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
 }
 
-__device__ __forceinline__ bool find_unit(const KvBatch& b, const KvAttend& a, int group, int shift, int index, KvSeq& q, Unit& u) {
-  u.s = b.cu_tokens ? find_sequence(b, index, shift, 1, group) : 0;
-  if (!b.cu_tokens) {
-    // every sequence has the same number of units
-    const int each = ((b.uniform * group - 1) >> shift) + 1;
-    u.s = index / each;
-    index -= u.s * each;
-    if (u.s >= b.sequences) return false;
-  } else {
-    if (u.s < 0) return false;
-    index -= kv_unit_base(b, u.s, shift, 1, group);
-  }
-  q = kv_seq(b, u.s);
-  u.first = index << shift;
+// The unit of sequence s that starts at row `tile` << shift; false if there are no rows.
+__device__ __forceinline__ bool unit_at(const KvBatch& b, const KvAttend& a, int group, int shift, int s, int tile, const KvSeq& q, Unit& u) {
+  u.s = s;
+  u.first = tile << shift;
   u.rows = q.n * group - u.first;
   if (u.rows <= 0) return false;
   if (u.rows > 1 << shift) u.rows = 1 << shift;
@@ -66,17 +57,36 @@ __device__ __forceinline__ bool find_unit(const KvBatch& b, const KvAttend& a, i
   return true;
 }
 
+__device__ __forceinline__ bool find_unit(const KvBatch& b, const KvAttend& a, int group, int shift, int index, KvSeq& q, Unit& u) {
+  int s;
+  if (b.cu_tokens) {
+    s = find_sequence(b, index, shift, 1, group);
+    if (s < 0) return false;
+    index -= kv_unit_base(b, s, shift, 1, group);
+  } else {
+    const int each = ((b.uniform * group - 1) >> shift) + 1;
+    s = index / each;
+    index -= s * each;
+  }
+  q = kv_seq(b, s);
+  return unit_at(b, a, group, shift, s, index, q, u);
+}
+
+// Where a stretch's part of a unit is kept.
+__device__ __forceinline__ int64_t part_of(const KvCache& c, const KvBatch& b, const Few& few, int unit, int kvh, int split) {
+  return ((int64_t)unit * c.kv_heads + kvh) * few.splits + split;
+}
+
 // D dims, 16 bits of fp16 (HALF) or bf16, a cache of e4m3 (EIGHT), NB blocks of 16 rows, pages of at least 16 slots (WIDE).
 template <int D, bool HALF, bool EIGHT, int NB, bool WIDE>
 __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_few(KvCache c, KvBatch b, KvAttend a, Few few) {
   constexpr int kElement = EIGHT ? 1 : 2;
   constexpr int kTile = EIGHT ? 64 : 32;               // positions of a tile
   constexpr int kGroups = kTile / 16;                  // of 16 positions: rows of an operand, and never over a page's end
-  constexpr int kLoads = D * kElement / 64;            // 16-byte loads of a lane for a group's keys
-  constexpr int kRowLanes = D * kElement / 16;         // lanes that read a position's values
+  constexpr int kRowLanes = D * kElement / 16;         // lanes that load a position's key, or value
   constexpr int kRowsALoad = kWave / kRowLanes;
-  constexpr int kValueLoads = kTile / kRowsALoad;
-  // a row of values in LDS: its pad puts the rows that are read together on different banks
+  constexpr int kRowLoads = kTile / kRowsALoad;
+  // a row in LDS: its pad puts the rows that are read together on different banks
   constexpr int kPitch = D * kElement + (EIGHT ? 16 : 32);
   constexpr int kBlocks = D / 16;
   constexpr bool kHalfP = EIGHT || HALF;  // weights are fp16 where the values' type allows it
@@ -87,11 +97,12 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
   __shared__ float lds_m[kWaves][16 * NB], lds_l[kWaves][16 * NB];
 
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int group = a.q_heads / c.kv_heads, kvh = blockIdx.y, split = blockIdx.z;
+  // heads first: their rows of a page are neighbours
+  const int group = a.q_heads / c.kv_heads, kvh = blockIdx.x % c.kv_heads, unit = blockIdx.x / c.kv_heads % few.units, split = blockIdx.x / c.kv_heads / few.units;
   constexpr int shift = NB == 1 ? 4 : NB == 2 ? 5 : 6;
   KvSeq q;
   Unit u;
-  if (!find_unit(b, a, group, shift, blockIdx.x, q, u)) return;
+  if (!find_unit(b, a, group, shift, unit, q, u)) return;
   const int begin = u.from + split * few.stretch;
   if (split && (begin >= u.to || q.bad)) return;
   const int end = begin + few.stretch < u.to ? begin + few.stretch : u.to;
@@ -128,7 +139,7 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
 
   uint8_t* const mine = lds + wave * kTile * kPitch;
   const uint8_t* const keys = c.k + (int64_t)kvh * c.head_stride;
-  const int64_t values_off = c.v - c.k;
+  const uint8_t* const values = c.v + (int64_t)kvh * c.head_stride;
   const int slot_mask = (1 << c.page_shift) - 1;
   // where this lane writes its values, and reads columns. 8 bits: a lane reads eight rows as one column, which are to be
   // the positions of its eight weights, so position r of 32 goes to row 8 ((r % 16) / 4) + 4 (r / 16) + r % 4
@@ -137,7 +148,7 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
   const int write_at = lds_row(value_row) * kPitch + value_col;
   const int read_at = EIGHT ? (8 * quad + (col >> 1)) * kPitch + (col & 1) * 8 : (4 * quad + (col >> 2)) * kPitch + (col & 3) * 8;
 
-  u32x4 kreg[kGroups][kLoads], vreg[kValueLoads];
+  u32x4 kreg[kRowLoads], vreg[kRowLoads];
   int page = 0, page_next = 0;           // of position base + lane
   float ks = 0, vs = 0, ks_next = 0, vs_next = 0;
 
@@ -146,36 +157,17 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
     return p < u.to && (kTile == kWave || lane < kTile) ? kv_page(c, b, u.s, p) : 0;
   };
   auto row_of = [&](int page, int p) {
-    return keys + ((int64_t)(page < 0 ? 0 : page) * c.page_stride + (int64_t)(p & slot_mask) * c.slot_stride);
+    return (int64_t)(page < 0 ? 0 : page) * c.page_stride + (int64_t)(p & slot_mask) * c.slot_stride;
   };
-  // offsets of this lane in a group that lies in one page: 32 bits, since a page's rows span less than 2^31 bytes
-  const uint32_t key_off = (uint32_t)(col * (int)c.slot_stride + quad * 16);
-  const uint32_t value_off = (uint32_t)((value_row & 15) * (int)c.slot_stride + value_col);
-  auto load_keys = [&](int base, int page) {
+  // this lane's offset in a group that lies in one page: 32 bits, since a page's rows span less than 2^31 bytes
+  const uint32_t lane_off = (uint32_t)((value_row & 15) * (int)c.slot_stride + value_col);
+  auto load_rows = [&](const uint8_t* from, int base, int page, u32x4 (&to)[kRowLoads]) {
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      if constexpr (WIDE) {
-        const uint8_t* at = row_of(__builtin_amdgcn_readlane(page, g * 16), base + g * 16);
-#pragma unroll
-        for (int t = 0; t < kLoads; ++t) kreg[g][t] = *(const u32x4*)(at + t * 64 + key_off);
-      } else {
-        const uint8_t* at = row_of(__shfl(page, g * 16 + col, kWave), base + g * 16 + col) + quad * 16;
-#pragma unroll
-        for (int t = 0; t < kLoads; ++t) kreg[g][t] = *(const u32x4*)(at + t * 64);
-      }
-    }
-  };
-  auto load_values = [&](int base, int page) {
-#pragma unroll
-    for (int i = 0; i < kValueLoads; ++i) {
-      if constexpr (WIDE) {
-        const int r = i * kRowsALoad;
-        const uint8_t* at = row_of(__builtin_amdgcn_readlane(page, r & ~15), base + r) + values_off;
-        vreg[i] = *(const u32x4*)(at + value_off);
-      } else {
-        const int r = i * kRowsALoad + value_row;
-        vreg[i] = *(const u32x4*)(row_of(__shfl(page, r, kWave), base + r) + values_off + value_col);
-      }
+    for (int i = 0; i < kRowLoads; ++i) {
+      const uint8_t* at;
+      if constexpr (WIDE) at = from + row_of(__builtin_amdgcn_readlane(page, i * kRowsALoad & ~15), base + i * kRowsALoad) + lane_off;
+      else at = from + row_of(__shfl(page, i * kRowsALoad + value_row, kWave), base + i * kRowsALoad + value_row) + value_col;
+      to[i] = __builtin_nontemporal_load((const u32x4*)at);
     }
   };
   auto load_scales = [&](int base, int page, float& k, float& v) {
@@ -194,28 +186,38 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
   constexpr int kStep = kWaves * kTile;
   if (base < end) {
     page = look_up(base);
-    load_keys(base, page);
+    load_rows(keys, base, page, kreg);
     load_scales(base, page, ks, vs);
-    load_values(base, page);
+    load_rows(values, base, page, vreg);
     if (base + kStep < end) page_next = look_up(base + kStep);
   }
   for (; base < end; base += kStep) {
     const bool more = base + kStep < end;
     const bool whole = base >= u.all_from && base + kTile <= u.all_to;
+#pragma unroll
+    for (int i = 0; i < kRowLoads; ++i) *(u32x4*)(mine + (i * kRowsALoad + value_row) * kPitch + value_col) = kreg[i];
+    __builtin_amdgcn_wave_barrier();
+    if (more) load_rows(keys, base + kStep, page_next, kreg);
     f32x4 score[NB][kGroups];
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g)
+    for (int g = 0; g < kGroups; ++g) {
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        f32x4 x = {0, 0, 0, 0};
+      for (int n = 0; n < NB; ++n) score[n][g] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int t = 0; t < D / 32; ++t) {
-          if constexpr (EIGHT) x = mfma16<HALF>(widen<HALF>(u32x2{kreg[g][t / 2][t % 2 * 2], kreg[g][t / 2][t % 2 * 2 + 1]}), qr[n][t], x);
-          else x = mfma16<HALF>(kreg[g][t], qr[n][t], x);
+      for (int t = 0; t < D * kElement / 64; ++t) {
+        const u32x4 k = *(const u32x4*)(mine + (g * 16 + col) * kPitch + t * 64 + quad * 16);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          if constexpr (EIGHT) {
+            score[n][g] = mfma16<HALF>(widen<HALF>(u32x2{k[0], k[1]}), qr[n][2 * t], score[n][g]);
+            score[n][g] = mfma16<HALF>(widen<HALF>(u32x2{k[2], k[3]}), qr[n][2 * t + 1], score[n][g]);
+          } else {
+            score[n][g] = mfma16<HALF>(k, qr[n][t], score[n][g]);
+          }
         }
-        score[n][g] = x;
       }
-    if (more) load_keys(base + kStep, page_next);
+    }
+    __builtin_amdgcn_wave_barrier();
 
     // scores in units of log 2
 #pragma unroll
@@ -228,7 +230,7 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
     bool odd = false;  // some positions have such values, and may be hidden from some rows
     if (!whole) {
 #pragma unroll
-      for (int i = 0; i < kValueLoads; ++i) {
+      for (int i = 0; i < kRowLoads; ++i) {
         const int p = base + i * kRowsALoad + value_row;
         if (p < u.lo || p >= u.to) vreg[i] = u32x4{0, 0, 0, 0};
         // those are taken out of the product and added one by one below
@@ -261,13 +263,13 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
             if (bad >> (g * 16 + quad * 4 + i) & 1) score[n][g][i] = __builtin_nanf("");
     }
 #pragma unroll
-    for (int i = 0; i < kValueLoads; ++i) *(u32x4*)(mine + write_at + lds_row(i * kRowsALoad) * kPitch) = vreg[i];
+    for (int i = 0; i < kRowLoads; ++i) *(u32x4*)(mine + write_at + lds_row(i * kRowsALoad) * kPitch) = vreg[i];
     __builtin_amdgcn_wave_barrier();
     const float vs_now = vs;
     const int page_now = page;
     if (more) {
       load_scales(base + kStep, page_next, ks_next, vs_next);
-      load_values(base + kStep, page_next);
+      load_rows(values, base + kStep, page_next, vreg);
       page = page_next;
       ks = ks_next;
       vs = vs_next;
@@ -359,7 +361,7 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
       for (int k = 0; k < kTile; ++k) {
         const int p = base + k;
         if (p < u.lo || p >= u.to) continue;
-        const uint8_t* at = row_of(__builtin_amdgcn_readlane(page_now, k), p) + values_off;
+        const uint8_t* at = values + row_of(__builtin_amdgcn_readlane(page_now, k), p);
         u32x4 v = {0, 0, 0, 0};
         if (lane < kRowLanes) v = *(const u32x4*)(at + lane * 16);
         if (!__any(not_finite<HALF, EIGHT>(v))) continue;
@@ -399,7 +401,7 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
       lds_l[wave][n * 16 + lane] = l[n];
     }
   }
-  const int64_t part = ((int64_t)blockIdx.x * c.kv_heads + kvh) * few.splits + split;
+  const int64_t part = part_of(c, b, few, unit, kvh, split);
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     __syncthreads();
@@ -448,54 +450,62 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
   }
 }
 
-// Joins the stretches of a row: one workgroup for a row and query head, the waves take stretches in turn.
-template <int D, bool HALF>
+// Joins the stretches of a row and query head: W waves take the stretches in turn (one wave where they are few, since then
+// rows are many).
+template <int D, bool HALF, int W>
 __global__ __launch_bounds__(kWaves * kWave) void join_stretches(KvCache c, KvBatch b, KvAttend a, Few few, int shift, float lift) {
-  const int group = a.q_heads / c.kv_heads, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const int rows = 1 << shift, kvh = blockIdx.y, row = blockIdx.x & (rows - 1), index = blockIdx.x >> shift;
-  KvSeq q;
-  Unit u;
-  if (!find_unit(b, a, group, shift, index, q, u) || row >= u.rows) return;
-  int parts = (u.to - u.from + few.stretch - 1) / few.stretch;
-  parts = q.bad || parts < 1 ? 1 : parts > few.splits ? few.splits : parts;
-  const int64_t first = ((int64_t)index * c.kv_heads + kvh) * few.splits;
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int index = blockIdx.x * (kWaves / W) + wave / W, turn = wave % W;
+  const int row = index / a.q_heads, head = index % a.q_heads, group = a.q_heads / c.kv_heads, kvh = head / group;
   constexpr int N = D / kWave;
   float m = -kInf, l = 0, x[N] = {};
-  for (int i = wave; i < parts; i += kWaves) {
-    const int64_t at = (first + i) * rows + row;
-    const float mi = few.stats[at * 2], li = few.stats[at * 2 + 1];
-    const float now = __builtin_elementwise_maximum(m, mi);
-    const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now), g = mi == now ? 1.0f : __builtin_amdgcn_exp2f(mi - now);
-    m = now;
-    l = l * f + li * g;
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = x[j] * f + few.sums[at * D + j * kWave + lane] * g;
+  KvSeq q;
+  Unit u;
+  const int s = row >= b.tokens ? -1 : b.cu_tokens ? find_sequence(b, row, 0, 0) : row / b.uniform;
+  bool mine = s >= 0;
+  if (mine) {
+    q = kv_seq(b, s);
+    mine = row >= q.row && row < q.row + q.n;
   }
-  __shared__ float part[kWaves][D], stat[kWaves][2];
+  if (mine) {
+    const int r = (row - q.row) * group + head % group;
+    const int unit = (b.cu_tokens ? kv_unit_base(b, s, shift, 1, group) : s * (((b.uniform * group - 1) >> shift) + 1)) + (r >> shift);
+    unit_at(b, a, group, shift, s, r >> shift, q, u);
+    int parts = (u.to - u.from + few.stretch - 1) / few.stretch;
+    parts = q.bad || parts < 1 ? 1 : parts > few.splits ? few.splits : parts;
+    for (int i = turn; i < parts; i += W) {
+      const int64_t at = (part_of(c, b, few, unit, kvh, i) << shift) + (r & ((1 << shift) - 1));
+      const float mi = few.stats[at * 2], li = few.stats[at * 2 + 1];
+      const float now = __builtin_elementwise_maximum(m, mi);
+      const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now), g = mi == now ? 1.0f : __builtin_amdgcn_exp2f(mi - now);
+      m = now;
+      l = l * f + li * g;
 #pragma unroll
-  for (int j = 0; j < N; ++j) part[wave][j * kWave + lane] = x[j];
-  if (lane == 0) { stat[wave][0] = m; stat[wave][1] = l; }
-  __syncthreads();
-  m = stat[0][0];
-#pragma unroll
-  for (int i = 1; i < kWaves; ++i) m = __builtin_elementwise_maximum(m, stat[i][0]);
-  float f[kWaves];
-  l = 0;
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
-    f[i] = stat[i][0] == m ? 1.0f : __builtin_amdgcn_exp2f(stat[i][0] - m);
-    l += stat[i][1] * f[i];
+      for (int j = 0; j < N; ++j) x[j] = x[j] * f + few.sums[at * D + lane * N + j] * g;
+    }
   }
-  const int rr = u.first + row, token = rr / group, head = kvh * group + rr % group;
-  for (int d = threadIdx.x; d < D; d += kWaves * kWave) {
-    float y = 0;
+  if constexpr (W > 1) {
+    __shared__ float part[W][D], stat[W][2];
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) y += part[i][d] * f[i];
-    y = q.bad ? __builtin_nanf("") : l == 0 ? 0.0f : y / l;
-    a.out[(q.row + token) * a.out_token + head * a.out_head + d] = from_float<HALF>(y);
+    for (int j = 0; j < N; ++j) part[turn][lane * N + j] = x[j];
+    if (lane == 0) { stat[turn][0] = m; stat[turn][1] = l; }
+    __syncthreads();
+    if (turn) return;
+#pragma unroll
+    for (int i = 1; i < W; ++i) {
+      const float mi = stat[i][0], now = __builtin_elementwise_maximum(m, mi);
+      const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now), g = mi == now ? 1.0f : __builtin_amdgcn_exp2f(mi - now);
+      m = now;
+      l = l * f + stat[i][1] * g;
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = x[j] * f + part[i][lane * N + j] * g;
+    }
   }
-  if (a.lse && threadIdx.x == 0)
-    a.lse[(int64_t)(q.row + token) * a.q_heads + head] = q.bad ? __builtin_nanf("") : l == 0 ? -kInf : ((m - lift) + __builtin_amdgcn_logf(l)) * kLn2;
+  if (!mine) return;
+  uint16_t* at = a.out + row * a.out_token + head * a.out_head + lane * N;
+#pragma unroll
+  for (int j = 0; j < N; ++j) at[j] = from_float<HALF>(q.bad ? __builtin_nanf("") : l == 0 ? 0.0f : x[j] / l);
+  if (a.lse && lane == 0) a.lse[(int64_t)row * a.q_heads + head] = q.bad ? __builtin_nanf("") : l == 0 ? -kInf : ((m - lift) + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 int units_of(const KvBatch& b, int group, int shift) {
@@ -516,7 +526,8 @@ void plan(const KvCache& c, const KvBatch& b, int group, int blocks, int window,
   int64_t span = b.max_context;
   const int64_t seen = (int64_t)window + (16 * blocks) / group + 1 + 64;
   if (window && seen < span) span = seen;
-  const int64_t all = (int64_t)units_of(b, group, shift) * c.kv_heads * span;
+  few->units = units_of(b, group, shift);
+  const int64_t all = (int64_t)few->units * c.kv_heads * span;
   const int64_t step = kWaves * 64;
   int64_t stretch = ((all + kTarget - 1) / kTarget + step - 1) / step * step;
   if (stretch < step) stretch = step;
@@ -527,8 +538,7 @@ void plan(const KvCache& c, const KvBatch& b, int group, int blocks, int window,
 template <int D, bool HALF, bool EIGHT, int NB>
 hipError_t launch_few(const KvCache& c, const KvBatch& b, const KvAttend& a, const Few& few, hipStream_t stream) {
   const int group = a.q_heads / c.kv_heads, shift = NB == 1 ? 4 : NB == 2 ? 5 : 6;
-  const int units = units_of(b, group, shift);
-  const dim3 grid(units, c.kv_heads, few.splits);
+  const uint32_t grid = (uint32_t)few.units * c.kv_heads * few.splits;
   if constexpr (!EIGHT) {
     if (c.page_shift < 4) attend_few<D, HALF, EIGHT, NB, false><<<grid, kWaves * kWave, 0, stream>>>(c, b, a, few);
     else attend_few<D, HALF, EIGHT, NB, true><<<grid, kWaves * kWave, 0, stream>>>(c, b, a, few);
@@ -536,7 +546,10 @@ hipError_t launch_few(const KvCache& c, const KvBatch& b, const KvAttend& a, con
     attend_few<D, HALF, EIGHT, NB, true><<<grid, kWaves * kWave, 0, stream>>>(c, b, a, few);
   }
   if (hipError_t e = hipGetLastError(); e != hipSuccess || few.splits == 1) return e;
-  join_stretches<D, HALF><<<dim3(units << shift, c.kv_heads), kWaves * kWave, 0, stream>>>(c, b, a, few, shift, EIGHT || HALF ? 8.0f : 0.0f);
+  const int rows = b.tokens * a.q_heads;
+  const float lift = EIGHT || HALF ? 8.0f : 0.0f;
+  if (few.splits > 8) join_stretches<D, HALF, kWaves><<<rows, kWaves * kWave, 0, stream>>>(c, b, a, few, shift, lift);
+  else join_stretches<D, HALF, 1><<<(rows + kWaves - 1) / kWaves, kWaves * kWave, 0, stream>>>(c, b, a, few, shift, lift);
   return hipGetLastError();
 }
 
@@ -570,9 +583,8 @@ hipError_t launch_kv_attend_few(const KvCache& c, const KvBatch& b, const KvAtte
   const int group = a.q_heads / c.kv_heads, blocks = blocks_of(group, a.max_tokens, head_dim);
   Few few;
   plan(c, b, group, blocks, a.window, &few);
-  const int shift = blocks == 1 ? 4 : blocks == 2 ? 5 : 6;
   few.sums = (float*)a.workspace;
-  few.stats = few.sums + (int64_t)units_of(b, group, shift) * c.kv_heads * few.splits * (16 * blocks) * head_dim;
+  few.stats = few.sums + (int64_t)few.units * c.kv_heads * few.splits * (16 * blocks) * head_dim;
   if (head_dim == 64) return launch_dims<64>(c, b, a, half, eight, few, blocks, stream);
   if (head_dim == 128) return launch_dims<128>(c, b, a, half, eight, few, blocks, stream);
   return launch_dims<256>(c, b, a, half, eight, few, blocks, stream);
