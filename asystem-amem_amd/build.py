@@ -6,13 +6,14 @@ tree; nothing is installed. Run as `python asystem-amem_amd/build.py`.
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIBNAME = "libamem_nccl.so.1"
 HOOK_NAME = "libamem_rccl_hook.so"
-HIP_SOURCES = ["kernels.hip", "kv_append.hip", "kv_attend_few.hip", "kv_attention.hip"]
+HIP_SOURCES = ["kernels.hip", "kv_append.hip", "kv_attend_few.hip", "kv_attend_many.hip", "kv_attention.hip"]
 CXX_SOURCES = ["capi.cpp", "engine.cpp", "ipc.cpp", "kv_api.cpp", "log.cpp", "slab_pool.cpp", "vmm.cpp"]
 # The packed-fp32 target feature is switched off for all device code of this project.
 DEVICE_FLAGS = ["--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
@@ -28,15 +29,16 @@ def build(verbose=True):
     os.makedirs(LIBDIR, exist_ok=True)
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
-    objs = []
+    objs, cmds = [], []
     for src in HIP_SOURCES + CXX_SOURCES:
         obj = os.path.join(objdir, src.rsplit(".", 1)[0] + ".o")
         cmd = [hipcc] + COMMON
         if src.endswith(".hip"):
             cmd += DEVICE_FLAGS
-        cmd += ["-c", os.path.join(CSRC, src), "-o", obj]
-        _run(cmd, verbose)
+        cmds.append(cmd + ["-c", os.path.join(CSRC, src), "-o", obj])
         objs.append(obj)
+    with ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:   # the kernels take most of the time
+        list(pool.map(lambda cmd: _run(cmd, verbose), cmds))
     out = lib_path()
     cmd = [hipcc, "-shared", "-fPIC", "-Wl,-soname," + LIBNAME, "--offload-arch=gfx950", "-o", out] + objs + ["-lpthread"]
     _run(cmd, verbose)

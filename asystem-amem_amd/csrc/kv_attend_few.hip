@@ -13,7 +13,7 @@
 // by wave, to become operands. A tile's registers are loaded again for the next tile as soon as LDS has them.
 #include <algorithm>
 
-#include "kv_device.h"
+#include "kv_parts.h"
 
 namespace amem {
 namespace {
@@ -21,65 +21,9 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kTarget = 512;  // workgroups that a call is cut into, where its contexts are long enough
 
-// How a call's rows and positions are dealt out.
-struct Few {
-  int stretch;   // positions of a workgroup, a multiple of kWaves * 64
-  int units;
-  int splits;    // most stretches of a unit
-  float* sums;   // [unit][kv head][split][row][dim]
-  float* stats;  // [unit][kv head][split][row]{m, l}, m in units of log 2
-};
-
-// A unit: some rows of one sequence (row r is head r % group of new token r / group), and the positions they see.
-struct Unit {
-  int s, first, rows;  // the sequence, the first of its rows, how many
-  int lo, to;          // positions that some row sees: [lo, to)
-  int from;            // lo, down to a multiple of 64
-  int all_from, all_to;  // positions that every row sees
-};
-
-__device__ __forceinline__ void row_range(const KvAttend& a, const KvSeq& q, int token, int& from, int& to) {
-  const int pos = q.context - q.n + token;
-  to = a.causal && pos + 1 < q.context ? pos + 1 : q.context;
-  from = a.window && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
-}
-
-// The unit of sequence s that starts at row `tile` << shift; false if there are no rows.
-__device__ __forceinline__ bool unit_at(const KvBatch& b, const KvAttend& a, int group, int shift, int s, int tile, const KvSeq& q, Unit& u) {
-  u.s = s;
-  u.first = tile << shift;
-  u.rows = q.n * group - u.first;
-  if (u.rows <= 0) return false;
-  if (u.rows > 1 << shift) u.rows = 1 << shift;
-  row_range(a, q, u.first / group, u.lo, u.all_to);
-  row_range(a, q, (u.first + u.rows - 1) / group, u.all_from, u.to);
-  u.from = u.lo & ~63;
-  return true;
-}
-
-__device__ __forceinline__ bool find_unit(const KvBatch& b, const KvAttend& a, int group, int shift, int index, KvSeq& q, Unit& u) {
-  int s;
-  if (b.cu_tokens) {
-    s = find_sequence(b, index, shift, 1, group);
-    if (s < 0) return false;
-    index -= kv_unit_base(b, s, shift, 1, group);
-  } else {
-    const int each = ((b.uniform * group - 1) >> shift) + 1;
-    s = index / each;
-    index -= s * each;
-  }
-  q = kv_seq(b, s);
-  return unit_at(b, a, group, shift, s, index, q, u);
-}
-
-// Where a stretch's part of a unit is kept.
-__device__ __forceinline__ int64_t part_of(const KvCache& c, const KvBatch& b, const Few& few, int unit, int kvh, int split) {
-  return ((int64_t)unit * c.kv_heads + kvh) * few.splits + split;
-}
-
 // D dims, 16 bits of fp16 (HALF) or bf16, a cache of e4m3 (EIGHT), NB blocks of 16 rows, pages of at least 16 slots (WIDE).
 template <int D, bool HALF, bool EIGHT, int NB, bool WIDE>
-__global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_few(KvCache c, KvBatch b, KvAttend a, Few few) {
+__global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_few(KvCache c, KvBatch b, KvAttend a, Parts few) {
   constexpr int kElement = EIGHT ? 1 : 2;
   constexpr int kTile = EIGHT ? 64 : 32;               // positions of a tile
   constexpr int kGroups = kTile / 16;                  // of 16 positions: rows of an operand, and never over a page's end
@@ -401,7 +345,7 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
       lds_l[wave][n * 16 + lane] = l[n];
     }
   }
-  const int64_t part = part_of(c, b, few, unit, kvh, split);
+  const int64_t part = part_of(c, few, unit, kvh, split);
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     __syncthreads();
@@ -450,68 +394,6 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
   }
 }
 
-// Joins the stretches of a row and query head: W waves take the stretches in turn (one wave where they are few, since then
-// rows are many).
-template <int D, bool HALF, int W>
-__global__ __launch_bounds__(kWaves * kWave) void join_stretches(KvCache c, KvBatch b, KvAttend a, Few few, int shift, float lift) {
-  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int index = blockIdx.x * (kWaves / W) + wave / W, turn = wave % W;
-  const int row = index / a.q_heads, head = index % a.q_heads, group = a.q_heads / c.kv_heads, kvh = head / group;
-  constexpr int N = D / kWave;
-  float m = -kInf, l = 0, x[N] = {};
-  KvSeq q;
-  Unit u;
-  const int s = row >= b.tokens ? -1 : b.cu_tokens ? find_sequence(b, row, 0, 0) : row / b.uniform;
-  bool mine = s >= 0;
-  if (mine) {
-    q = kv_seq(b, s);
-    mine = row >= q.row && row < q.row + q.n;
-  }
-  if (mine) {
-    const int r = (row - q.row) * group + head % group;
-    const int unit = (b.cu_tokens ? kv_unit_base(b, s, shift, 1, group) : s * (((b.uniform * group - 1) >> shift) + 1)) + (r >> shift);
-    unit_at(b, a, group, shift, s, r >> shift, q, u);
-    int parts = (u.to - u.from + few.stretch - 1) / few.stretch;
-    parts = q.bad || parts < 1 ? 1 : parts > few.splits ? few.splits : parts;
-    for (int i = turn; i < parts; i += W) {
-      const int64_t at = (part_of(c, b, few, unit, kvh, i) << shift) + (r & ((1 << shift) - 1));
-      const float mi = few.stats[at * 2], li = few.stats[at * 2 + 1];
-      const float now = __builtin_elementwise_maximum(m, mi);
-      const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now), g = mi == now ? 1.0f : __builtin_amdgcn_exp2f(mi - now);
-      m = now;
-      l = l * f + li * g;
-#pragma unroll
-      for (int j = 0; j < N; ++j) x[j] = x[j] * f + few.sums[at * D + lane * N + j] * g;
-    }
-  }
-  if constexpr (W > 1) {
-    __shared__ float part[W][D], stat[W][2];
-#pragma unroll
-    for (int j = 0; j < N; ++j) part[turn][lane * N + j] = x[j];
-    if (lane == 0) { stat[turn][0] = m; stat[turn][1] = l; }
-    __syncthreads();
-    if (turn) return;
-#pragma unroll
-    for (int i = 1; i < W; ++i) {
-      const float mi = stat[i][0], now = __builtin_elementwise_maximum(m, mi);
-      const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now), g = mi == now ? 1.0f : __builtin_amdgcn_exp2f(mi - now);
-      m = now;
-      l = l * f + stat[i][1] * g;
-#pragma unroll
-      for (int j = 0; j < N; ++j) x[j] = x[j] * f + part[i][lane * N + j] * g;
-    }
-  }
-  if (!mine) return;
-  uint16_t* at = a.out + row * a.out_token + head * a.out_head + lane * N;
-#pragma unroll
-  for (int j = 0; j < N; ++j) at[j] = from_float<HALF>(q.bad ? __builtin_nanf("") : l == 0 ? 0.0f : x[j] / l);
-  if (a.lse && lane == 0) a.lse[(int64_t)row * a.q_heads + head] = q.bad ? __builtin_nanf("") : l == 0 ? -kInf : ((m - lift) + __builtin_amdgcn_logf(l)) * kLn2;
-}
-
-int units_of(const KvBatch& b, int group, int shift) {
-  return b.cu_tokens ? kv_units(b, shift, 1, group) : b.sequences * (((b.uniform * group - 1) >> shift) + 1);
-}
-
 // Blocks of 16 rows that a workgroup takes: enough for all rows of a sequence's key/value head, so that its keys and
 // values are read once.
 int blocks_of(int group, int max_tokens, int head_dim) {
@@ -521,7 +403,7 @@ int blocks_of(int group, int max_tokens, int head_dim) {
 
 // Stretches are as long as leaves about kTarget workgroups (eight for each compute unit, of which it holds two to four at a
 // time), and at least a tile for each wave.
-void plan(const KvCache& c, const KvBatch& b, int group, int blocks, int window, Few* few) {
+void plan(const KvCache& c, const KvBatch& b, int group, int blocks, int window, Parts* few) {
   const int shift = blocks == 1 ? 4 : blocks == 2 ? 5 : 6;
   int64_t span = b.max_context;
   const int64_t seen = (int64_t)window + (16 * blocks) / group + 1 + 64;
@@ -536,7 +418,7 @@ void plan(const KvCache& c, const KvBatch& b, int group, int blocks, int window,
 }
 
 template <int D, bool HALF, bool EIGHT, int NB>
-hipError_t launch_few(const KvCache& c, const KvBatch& b, const KvAttend& a, const Few& few, hipStream_t stream) {
+hipError_t launch_few(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& few, hipStream_t stream) {
   const int group = a.q_heads / c.kv_heads, shift = NB == 1 ? 4 : NB == 2 ? 5 : 6;
   const uint32_t grid = (uint32_t)few.units * c.kv_heads * few.splits;
   if constexpr (!EIGHT) {
@@ -546,15 +428,11 @@ hipError_t launch_few(const KvCache& c, const KvBatch& b, const KvAttend& a, con
     attend_few<D, HALF, EIGHT, NB, true><<<grid, kWaves * kWave, 0, stream>>>(c, b, a, few);
   }
   if (hipError_t e = hipGetLastError(); e != hipSuccess || few.splits == 1) return e;
-  const int rows = b.tokens * a.q_heads;
-  const float lift = EIGHT || HALF ? 8.0f : 0.0f;
-  if (few.splits > 8) join_stretches<D, HALF, kWaves><<<rows, kWaves * kWave, 0, stream>>>(c, b, a, few, shift, lift);
-  else join_stretches<D, HALF, 1><<<(rows + kWaves - 1) / kWaves, kWaves * kWave, 0, stream>>>(c, b, a, few, shift, lift);
-  return hipGetLastError();
+  return launch_join(c, b, a, few, shift, EIGHT || HALF ? 8.0f : 0.0f, D, HALF, stream);
 }
 
 template <int D, bool HALF, bool EIGHT>
-hipError_t launch_blocks(const KvCache& c, const KvBatch& b, const KvAttend& a, const Few& few, int blocks, hipStream_t stream) {
+hipError_t launch_blocks(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& few, int blocks, hipStream_t stream) {
   if (blocks == 1) return launch_few<D, HALF, EIGHT, 1>(c, b, a, few, stream);
   if (blocks == 2) return launch_few<D, HALF, EIGHT, 2>(c, b, a, few, stream);
   if constexpr (D < 256) return launch_few<D, HALF, EIGHT, 4>(c, b, a, few, stream);
@@ -562,7 +440,7 @@ hipError_t launch_blocks(const KvCache& c, const KvBatch& b, const KvAttend& a, 
 }
 
 template <int D>
-hipError_t launch_dims(const KvCache& c, const KvBatch& b, const KvAttend& a, bool half, bool eight, const Few& few, int blocks, hipStream_t stream) {
+hipError_t launch_dims(const KvCache& c, const KvBatch& b, const KvAttend& a, bool half, bool eight, const Parts& few, int blocks, hipStream_t stream) {
   if (half) return eight ? launch_blocks<D, true, true>(c, b, a, few, blocks, stream) : launch_blocks<D, true, false>(c, b, a, few, blocks, stream);
   return eight ? launch_blocks<D, false, true>(c, b, a, few, blocks, stream) : launch_blocks<D, false, false>(c, b, a, few, blocks, stream);
 }
@@ -581,7 +459,7 @@ uint64_t kv_attend_few_workspace(const KvCache& c, const KvBatch& b, int q_heads
 
 hipError_t launch_kv_attend_few(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream) {
   const int group = a.q_heads / c.kv_heads, blocks = blocks_of(group, a.max_tokens, head_dim);
-  Few few;
+  Parts few;
   plan(c, b, group, blocks, a.window, &few);
   few.sums = (float*)a.workspace;
   few.stats = few.sums + (int64_t)few.units * c.kv_heads * few.splits * (16 * blocks) * head_dim;

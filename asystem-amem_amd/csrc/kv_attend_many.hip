@@ -1,0 +1,397 @@
+// Attention over a paged key/value cache for many rows: prompts, and chunks of them.
+//
+//   s_p = scale q.k_p,  m = max s_p,  l = sum exp(s_p - m),  out = sum exp(s_p - m) v_p / l,  lse = m + log l
+//
+// Bound by the matrix unit. A workgroup takes 128 rows that share a key/value head (32 for each of its four waves) through
+// the positions they see, 64 at a time: its threads load a tile of keys and values while the one before is worked on, and
+// put it into LDS as 16-bit numbers, where every wave reads all of it. Two tiles are held there, so that one barrier a
+// tile is enough. Products are (keys x dims)(dims x rows) and (dims x keys)(keys x rows): a lane holds scores and sums
+// of one row, the weights go from the first product's result to the second's operand without leaving their lane, and
+// values are read from LDS as columns.
+#include <algorithm>
+
+#include "kv_parts.h"
+
+namespace amem {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kShift = 7;      // log2 of a unit's rows
+constexpr int kTile = 64;      // positions
+constexpr int kTarget = 512;   // workgroups that fit at once; contexts are cut until there are as many
+
+// Eight e4m3 codes times a power of two as 16-bit numbers.
+template <bool HALF>
+__device__ __forceinline__ u32x4 widen_scaled(u32x2 x, float scale) {
+  u32x4 y;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (HALF) {
+      y[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[i], scale, false));
+      y[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[i], scale, true));
+    } else {
+      y[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], scale, false));
+      y[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], scale, true));
+    }
+  }
+  return y;
+}
+
+__device__ __forceinline__ float lane_value(float x, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
+}
+
+// D dims, 16 bits of fp16 (HALF) or bf16, a cache of e4m3 (EIGHT).
+template <int D, bool HALF, bool EIGHT>
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend_many(KvCache c, KvBatch b, KvAttend a, Parts parts) {
+  constexpr int kElement = EIGHT ? 1 : 2;
+  constexpr int kRowLanes = D * kElement / 16;    // threads that load a position's key, or value
+  constexpr int kRowsAPass = kThreads / kRowLanes;
+  constexpr int kPasses = kTile / kRowsAPass;
+  static_assert(kPasses >= 1, "a pass is at most a tile");
+  // pads: the rows that are read together are on different banks
+  constexpr int kKeyPitch = D * 2 + 16, kValuePitch = D * 2 + 64, kBuffer = kTile * (kKeyPitch + kValuePitch);
+  constexpr bool kHalfP = EIGHT || HALF;  // weights are fp16 where the values' type allows it
+  // fp16 weights are held 2^8 times larger, which keeps small ones out of the subnormal numbers
+  constexpr float kLift = kHalfP ? 8.0f : 0.0f;
+  // Scales of keys go into the keys where 16 bits hold every product (bf16), else into the scores.
+  constexpr bool kFold = EIGHT && !HALF;
+  constexpr int kDims = D / 32;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kBuffer];
+  __shared__ uint64_t lds_odd[2][kPasses * kWaves];
+
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  // heads first, so that the units of a head, which read the same keys, run on one die where heads are a multiple of eight;
+  // the last units, which see most, before the others
+  const int group = a.q_heads / c.kv_heads, kvh = blockIdx.x % c.kv_heads;
+  const int unit = parts.units - 1 - blockIdx.x / c.kv_heads % parts.units, split = blockIdx.x / c.kv_heads / parts.units;
+  KvSeq q;
+  Unit u;
+  if (!find_unit(b, a, group, kShift, unit, q, u)) return;
+  const int begin = u.from + split * parts.stretch;
+  if (split && (begin >= u.to || q.bad)) return;
+  const int end = begin + parts.stretch < u.to ? begin + parts.stretch : u.to;
+  const int col = lane & 31, half = lane >> 5;
+
+  // this wave's rows, and the positions that some, and all, of them see
+  const int wave_first = u.first + wave * 32;
+  const bool active = wave * 32 < u.rows;
+  const int wave_last = std::min(wave_first + 31, u.first + u.rows - 1);
+  int wave_lo = 0, wave_to = 0, all_from = 0, all_to = 0, row_from = 0, row_to = 0, token = 0, head = 0;
+  u32x4 qr[D / 16];
+  if (active) {
+    row_range(a, q, wave_first / group, wave_lo, all_to);
+    row_range(a, q, wave_last / group, all_from, wave_to);
+    const int r = std::min(wave_first + col, wave_last);
+    token = r / group;
+    head = kvh * group + r % group;
+    row_range(a, q, token, row_from, row_to);
+    const uint16_t* p = a.q + (q.row + token) * a.q_token + head * a.q_head;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) qr[t] = *(const u32x4*)(p + t * 16 + half * 8);
+  }
+
+  float m = -kInf, l = 0;
+  f32x16 sum[kDims];
+#pragma unroll
+  for (int i = 0; i < kDims; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sum[i][j] = 0;
+  float unit_scale = 0;  // the sums are in multiples of it (8 bits)
+
+  // ---- loading: a thread's rows of a tile
+  const int my_row = tid / kRowLanes, my_col = tid % kRowLanes * 16;
+  const int slot_mask = (1 << c.page_shift) - 1;
+  const uint8_t* const keys = c.k + (int64_t)kvh * c.head_stride + my_col;
+  const uint8_t* const values = c.v + (int64_t)kvh * c.head_stride + my_col;
+  u32x4 kreg[kPasses], vreg[kPasses];
+  int page[kPasses], group_page = 0;  // of the tile to be loaded next: 0 where there is none, -1 where it is out of range
+  bool missing[kPasses];              // of the tile in the registers
+  float ks = 0, vs = 0;               // of the tile in the registers, lane g has group g's
+  auto look_up = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int p = base + i * kRowsAPass + my_row;
+      page[i] = p < u.to ? kv_page(c, b, u.s, p) : 0;
+    }
+    if constexpr (EIGHT) {
+      const int p = base + (lane & 3) * 16;
+      group_page = p < u.to ? kv_page(c, b, u.s, p) : 0;
+    }
+  };
+  auto load = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int p = base + i * kRowsAPass + my_row;
+      missing[i] = page[i] < 0;
+      const int64_t at = (int64_t)(page[i] < 0 ? 0 : page[i]) * c.page_stride + (int64_t)(p & slot_mask) * c.slot_stride;
+      kreg[i] = *(const u32x4*)(keys + at);
+      vreg[i] = *(const u32x4*)(values + at);
+    }
+    if constexpr (EIGHT) {
+      const int p = base + (lane & 3) * 16;
+      ks = vs = 0;
+      if (p < u.to && (p | 15) >= u.lo) {  // a hidden group's scale may be anything
+        const int64_t at = kv_scale_offset(c, group_page < 0 ? 0 : group_page, kvh, p);
+        ks = c.k_scale[at];
+        vs = c.v_scale[at];
+      }
+    }
+  };
+  auto partial = [&](int base) { return base < u.all_from || base + kTile > u.all_to; };
+  // The registers' tile into LDS. Keys of a page that is out of range become NaN, which every row that sees them gets.
+  float key_scale[4] = {1, 1, 1, 1}, stored_scale = 0;  // of the tile stored last
+  auto store = [&](int base, int buffer) {
+    uint8_t* const at = lds + buffer * kBuffer;
+    float value_scale[4];
+    if constexpr (EIGHT) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        key_scale[g] = lane_value(ks, g);
+        value_scale[g] = lane_value(vs, g);
+        stored_scale = __builtin_elementwise_maximum(stored_scale, value_scale[g]);
+      }
+      const float f = stored_scale > 0 ? 1.0f / stored_scale : 0.0f;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) value_scale[g] *= f;
+    }
+    const bool edge = partial(base);
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int r = i * kRowsAPass + my_row;
+      u32x4 k = kreg[i], v = vreg[i];
+      if (missing[i]) k = u32x4{~0u, ~0u, ~0u, ~0u};
+      if (edge) {
+        // a weight of zero does not hide infinities and NaN: values that no row sees become zeros here, and those that
+        // only some rows see are taken out of the product and added one by one
+        if (base + r < u.lo || base + r >= u.to) v = u32x4{0, 0, 0, 0};
+        const uint64_t lanes = __ballot(not_finite<HALF, EIGHT>(v));
+        if (lane == 0) lds_odd[buffer][i * kWaves + wave] = lanes;
+        if (lanes >> (lane / kRowLanes * kRowLanes) & ((1ull << kRowLanes) - 1)) v = u32x4{0, 0, 0, 0};
+      }
+      if constexpr (EIGHT) {
+        const int g = r >> 4;
+        const float fk = kFold ? (g & 2 ? (g & 1 ? key_scale[3] : key_scale[2]) : (g & 1 ? key_scale[1] : key_scale[0])) : 1.0f;
+        const float fv = g & 2 ? (g & 1 ? value_scale[3] : value_scale[2]) : (g & 1 ? value_scale[1] : value_scale[0]);
+        uint8_t* ka = at + r * kKeyPitch + my_col * 2;
+        uint8_t* va = at + kTile * kKeyPitch + r * kValuePitch + my_col * 2;
+        *(u32x4*)ka = widen_scaled<HALF>(u32x2{k[0], k[1]}, fk);
+        *(u32x4*)(ka + 16) = widen_scaled<HALF>(u32x2{k[2], k[3]}, fk);
+        *(u32x4*)va = widen_scaled<true>(u32x2{v[0], v[1]}, fv);
+        *(u32x4*)(va + 16) = widen_scaled<true>(u32x2{v[2], v[3]}, fv);
+      } else {
+        *(u32x4*)(at + r * kKeyPitch + my_col) = k;
+        *(u32x4*)(at + kTile * kKeyPitch + r * kValuePitch + my_col) = v;
+      }
+    }
+  };
+
+  if (begin < end) {
+    look_up(begin);
+    load(begin);
+    look_up(begin + kTile);
+    store(begin, 0);
+    load(begin + kTile);
+    look_up(begin + 2 * kTile);
+  }
+  int buffer = 0;
+  for (int base = begin; base < end; base += kTile, buffer ^= 1) {
+    __syncthreads();
+    const bool work = active && base < wave_to && base + kTile > wave_lo;
+    const uint8_t* const tile = lds + buffer * kBuffer;
+    f32x16 score[2];
+    float f[4];
+    if constexpr (EIGHT && !kFold) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) f[g] = a.scale * kLog2e * key_scale[g];
+    }
+    const float tile_scale = stored_scale;
+    if (work) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) score[g][j] = 0;
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t)
+          score[g] = mfma32<HALF>(*(const u32x4*)(tile + (g * 32 + col) * kKeyPitch + t * 32 + half * 16), qr[t], score[g]);
+      }
+    }
+    if (base + kTile < end) {
+      store(base + kTile, buffer ^ 1);
+      load(base + 2 * kTile);
+      look_up(base + 3 * kTile);
+    }
+    if (!work) continue;
+
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) score[g][j] *= EIGHT && !kFold ? f[2 * g + j / 8] : a.scale * kLog2e;
+    const bool edge = base < all_from || base + kTile > all_to;
+    if (edge) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int p = base + g * 32 + j / 4 * 8 + half * 4 + j % 4;
+          if (p < row_from || p >= row_to) score[g][j] = -kInf;
+        }
+    }
+    float top = score[0][0];
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) top = __builtin_elementwise_maximum(top, score[g][j]);  // NaN stays
+    top = __builtin_elementwise_maximum(top, __shfl_xor(top, 32, kWave));
+    const float now = __builtin_elementwise_maximum(m, top);
+    if (__any(now != m)) {
+      const float shrink = now == m ? 1.0f : __builtin_amdgcn_exp2f(m - now);
+      l *= shrink;
+#pragma unroll
+      for (int i = 0; i < kDims; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sum[i][j] *= shrink;
+      m = now;
+    }
+    if (EIGHT && !(tile_scale <= unit_scale)) {
+      const float x = unit_scale / tile_scale;
+#pragma unroll
+      for (int i = 0; i < kDims; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sum[i][j] *= x;
+      unit_scale = tile_scale;
+    }
+    const float sub = (m == -kInf ? 0.0f : m) - kLift;
+    u32x4 w[4];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        score[g][j] = __builtin_amdgcn_exp2f(score[g][j] - sub);
+        l += score[g][j];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[2 * g + j / 4][j % 4] = pack<kHalfP>(score[g][2 * j], score[g][2 * j + 1]);
+    }
+    // lane m of 16 gives the address of position m / 4 of four, dims 4 (m % 4) on, of the block of 16 dims that these lanes take
+    const uint8_t* const columns = tile + kTile * kKeyPitch + (4 * half + (lane & 15) / 4) * kValuePitch + ((lane >> 4 & 1) * 16 + (lane & 3) * 4) * 2;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < kDims; ++i) {
+        const uint8_t* p = columns + t * 16 * kValuePitch + i * 64;
+        const u32x2 lo = read_columns16(p), hi = read_columns16(p + 8 * kValuePitch);
+        sum[i] = mfma32<kHalfP>(u32x4{lo[0], lo[1], hi[0], hi[1]}, w[t], sum[i]);
+      }
+    if (edge) {
+#pragma unroll 1
+      for (int n = 0; n < kPasses * kWaves; ++n) {
+        const uint64_t lanes = lds_odd[buffer][n];
+        if (!lanes) continue;
+#pragma unroll 1
+        for (int j = 0; j < kWave / kRowLanes; ++j) {
+          if (!(lanes >> (j * kRowLanes) & ((1ull << kRowLanes) - 1))) continue;
+          const int k = n / kWaves * kRowsAPass + n % kWaves * (kWave / kRowLanes) + j, p = base + k;
+          const int where = kv_page(c, b, u.s, p);  // seen by some row, so below u.to
+          if (where < 0) continue;                  // its key is NaN already
+          const uint8_t* v = c.v + kv_offset(c, where, kvh, p);
+          float x = 0;
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (k >> 5 == g && (k & 31) / 8 * 4 + k % 4 == e) x = score[g][e];
+          x = __shfl(x, (k >> 2 & 1) * 32 + col, kWave);
+          if (p < row_from || p >= row_to) continue;
+          if constexpr (EIGHT) x *= c.v_scale[kv_scale_offset(c, where, kvh, p)] * (unit_scale > 0 ? 1.0f / unit_scale : 0.0f);
+#pragma unroll
+          for (int i = 0; i < kDims; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int d = i * 32 + e / 4 * 8 + half * 4 + e % 4;
+              if constexpr (EIGHT) sum[i][e] += x * __builtin_amdgcn_cvt_f32_fp8((int)v[d], 0);
+              else sum[i][e] += x * to_float<HALF>(((const uint16_t*)v)[d]);
+            }
+        }
+      }
+    }
+  }
+  if (!active) return;
+
+  l += __shfl_xor(l, 32, kWave);
+  const float back = EIGHT && unit_scale > 0 ? unit_scale : 1.0f;
+  const int r = wave * 32 + col;
+  if (r >= u.rows) return;
+  if (parts.splits > 1) {
+    const int64_t row = (part_of(c, parts, unit, kvh, split) << kShift) + r;
+#pragma unroll
+    for (int i = 0; i < kDims; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *(f32x4*)(parts.sums + row * D + i * 32 + j * 8 + half * 4) =
+            f32x4{sum[i][4 * j], sum[i][4 * j + 1], sum[i][4 * j + 2], sum[i][4 * j + 3]} * back;
+    if (half == 0) {
+      parts.stats[row * 2] = m;
+      parts.stats[row * 2 + 1] = l;
+    }
+    return;
+  }
+  const float inverse = q.bad ? __builtin_nanf("") : l == 0 ? 0.0f : back / l;
+  uint16_t* const out = a.out + (q.row + token) * a.out_token + head * a.out_head;
+#pragma unroll
+  for (int i = 0; i < kDims; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4 x = f32x4{sum[i][4 * j], sum[i][4 * j + 1], sum[i][4 * j + 2], sum[i][4 * j + 3]} * inverse;
+      *(u32x2*)(out + i * 32 + j * 8 + half * 4) = u32x2{pack<HALF>(x[0], x[1]), pack<HALF>(x[2], x[3])};
+    }
+  if (a.lse && half == 0)
+    a.lse[(int64_t)(q.row + token) * a.q_heads + head] = q.bad ? __builtin_nanf("") : l == 0 ? -kInf : ((m - kLift) + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// Contexts are cut only where units are fewer than fit at once, and never below 512 positions: a part costs its rows' sums
+// written and read once more.
+void plan(const KvCache& c, const KvBatch& b, int group, int window, Parts* parts) {
+  parts->units = units_of(b, group, kShift);
+  int64_t span = b.max_context;
+  const int64_t seen = (int64_t)window + (1 << kShift) / group + 1 + 64;
+  if (window && seen < span) span = seen;
+  const int64_t all = (int64_t)parts->units * c.kv_heads * span;
+  const int64_t stretch = std::max<int64_t>(((all + kTarget - 1) / kTarget + 511) / 512 * 512, 512);
+  parts->stretch = (int)stretch;
+  parts->splits = span > stretch ? (int)((span + stretch - 1) / stretch) : 1;
+}
+
+template <int D>
+hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, bool half, bool eight, const Parts& parts, hipStream_t stream) {
+  const uint32_t grid = (uint32_t)parts.units * c.kv_heads * parts.splits;
+  if (half && eight) attend_many<D, true, true><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  else if (half) attend_many<D, true, false><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  else if (eight) attend_many<D, false, true><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  else attend_many<D, false, false><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess || parts.splits == 1) return e;
+  return launch_join(c, b, a, parts, kShift, half || eight ? 8.0f : 0.0f, D, half, stream);
+}
+
+}  // namespace
+
+uint64_t kv_attend_many_workspace(const KvCache& c, const KvBatch& b, int q_heads, int head_dim) {
+  // for any window: plan() has at most that many splits
+  const int64_t units = (int64_t)units_of(b, q_heads / c.kv_heads, kShift) * c.kv_heads;
+  if (!units) return 0;
+  const int64_t splits = std::min<int64_t>((b.max_context + 511) / 512, (kTarget + units - 1) / units);
+  return splits < 2 ? 0 : (uint64_t)((units * splits) << kShift) * (head_dim + 2) * 4;
+}
+
+hipError_t launch_kv_attend_many(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream) {
+  Parts parts;
+  plan(c, b, a.q_heads / c.kv_heads, a.window, &parts);
+  parts.sums = (float*)a.workspace;
+  parts.stats = parts.sums + (((int64_t)parts.units * c.kv_heads * parts.splits) << kShift) * head_dim;
+  if (head_dim == 64) return launch<64>(c, b, a, half, eight, parts, stream);
+  if (head_dim == 128) return launch<128>(c, b, a, half, eight, parts, stream);
+  return launch<256>(c, b, a, half, eight, parts, stream);
+}
+
+}  // namespace amem

@@ -1,113 +1,100 @@
-// Attention over a paged key/value cache.
-//
-//   s_p = scale q.k_p,  m = max s_p,  l = sum exp(s_p - m),  out = sum exp(s_p - m) v_p / l,  lse = m + log l
-//
-// in one pass over the keys: m, l and the sum so far are carried along, and both are multiplied by
-// exp(m_old - m_new) when a tile of keys raises m.
-#include "kv_device.h"
+// Attention over a paged key/value cache: which kernel takes a call, and the join of the parts of rows whose positions were
+// dealt out to several workgroups.
+#include "kv_parts.h"
 
 namespace amem {
 namespace {
 
-template <bool HALF, bool EIGHT>
-__device__ __forceinline__ float element(const uint8_t* at, int d) {
-  if constexpr (EIGHT) return __builtin_amdgcn_cvt_f32_fp8((int)at[d], 0);
-  else return to_float<HALF>(((const uint16_t*)at)[d]);
-}
+constexpr int kJoinWaves = 4;
 
-// One wave for a row and head: a lane takes a key of each 64, then D / 64 dims of the sum.
-template <int D, bool HALF, bool EIGHT>
-__global__ __launch_bounds__(kWave) void attend_row(KvCache c, KvBatch b, KvAttend a) {
-  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-  const int s = find_sequence(b, row, 0, 0);
-  if (s < 0) return;
-  const KvSeq q = kv_seq(b, s);
-  if (row < q.row || row >= q.row + q.n) return;
-  const int pos = q.context - q.n + row - q.row;
-  const int kvh = h / (a.q_heads / c.kv_heads);
-  int from = 0, to = q.context;
-  if (a.causal && pos + 1 < to) to = pos + 1;
-  if (a.window && pos - a.window + 1 > 0) from = pos - a.window + 1;
-  __shared__ float qs[D], ps[kWave];
-  __shared__ const uint8_t* vs[kWave];
-  const uint16_t* qp = a.q + row * a.q_token + h * a.q_head;
-  for (int d = lane; d < D; d += kWave) qs[d] = to_float<HALF>(qp[d]);
-  __syncthreads();
-  float m = -__builtin_inff(), l = 0, o[D / kWave] = {};
-  bool bad = q.bad;
-  for (int p0 = from; p0 < to; p0 += kWave) {
-    const int p = p0 + lane;
-    float x = -__builtin_inff(), vscale = 1;
-    const uint8_t* v = nullptr;
-    int page = 0;
-    if (p < to) page = kv_page(c, b, s, p);
-    if (__any(page < 0)) { bad = true; break; }
-    if (p < to) {
-      const uint8_t* k = c.k + kv_offset(c, page, kvh, p);
-      v = c.v + kv_offset(c, page, kvh, p);
-      x = 0;
-      for (int d = 0; d < D; ++d) x += qs[d] * element<HALF, EIGHT>(k, d);
-      x *= a.scale;
-      if constexpr (EIGHT) {
-        const int64_t at = kv_scale_offset(c, page, kvh, p);
-        x *= c.k_scale[at];
-        vscale = c.v_scale[at];
-      }
-    }
-    float top = x;
-#pragma unroll
-    for (int i = kWave / 2; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i, kWave));
-    if (__any(x != x)) top = __builtin_nanf("");
-    const float now = top > m || top != top ? top : m;
-    if (now == -__builtin_inff()) continue;
-    const float shrink = expf(m - now), w = expf(x - now);
-    float sum = w;
-#pragma unroll
-    for (int i = kWave / 2; i; i >>= 1) sum += __shfl_xor(sum, i, kWave);
-    l = l * shrink + sum;
-    m = now;
-    ps[lane] = w * vscale;
-    vs[lane] = v;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < D / kWave; ++i) o[i] *= shrink;
-    for (int j = 0; j < kWave && p0 + j < to; ++j)
-#pragma unroll
-      for (int i = 0; i < D / kWave; ++i) o[i] += ps[j] * element<HALF, EIGHT>(vs[j], lane + i * kWave);
-    __syncthreads();
+// Joins the stretches of a row and query head: W waves take the stretches in turn (one wave where they are few, since then
+// rows are many).
+template <int D, bool HALF, int W>
+__global__ __launch_bounds__(kJoinWaves * kWave) void join_stretches(KvCache c, KvBatch b, KvAttend a, Parts parts, int shift, float lift) {
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int index = blockIdx.x * (kJoinWaves / W) + wave / W, turn = wave % W;
+  const int row = index / a.q_heads, head = index % a.q_heads, group = a.q_heads / c.kv_heads, kvh = head / group;
+  constexpr int N = D / kWave;
+  float m = -kInf, l = 0, x[N] = {};
+  KvSeq q;
+  Unit u;
+  const int s = row >= b.tokens ? -1 : b.cu_tokens ? find_sequence(b, row, 0, 0) : row / b.uniform;
+  bool mine = s >= 0;
+  if (mine) {
+    q = kv_seq(b, s);
+    mine = row >= q.row && row < q.row + q.n;
   }
-  const float nan = __builtin_nanf("");
+  if (mine) {
+    const int r = (row - q.row) * group + head % group;
+    const int unit = (b.cu_tokens ? kv_unit_base(b, s, shift, 1, group) : s * (((b.uniform * group - 1) >> shift) + 1)) + (r >> shift);
+    unit_at(b, a, group, shift, s, r >> shift, q, u);
+    int count = (u.to - u.from + parts.stretch - 1) / parts.stretch;
+    count = q.bad || count < 1 ? 1 : count > parts.splits ? parts.splits : count;
+    for (int i = turn; i < count; i += W) {
+      const int64_t at = (part_of(c, parts, unit, kvh, i) << shift) + (r & ((1 << shift) - 1));
+      const float mi = parts.stats[at * 2], li = parts.stats[at * 2 + 1];
+      const float now = __builtin_elementwise_maximum(m, mi);
+      const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now), g = mi == now ? 1.0f : __builtin_amdgcn_exp2f(mi - now);
+      m = now;
+      l = l * f + li * g;
 #pragma unroll
-  for (int i = 0; i < D / kWave; ++i)
-    a.out[row * a.out_token + h * a.out_head + lane + i * kWave] = from_float<HALF>(bad ? nan : l == 0 ? 0 : o[i] / l);
-  if (a.lse && lane == 0) a.lse[(int64_t)row * a.q_heads + h] = bad ? nan : l == 0 ? -__builtin_inff() : m + logf(l);
+      for (int j = 0; j < N; ++j) x[j] = x[j] * f + parts.sums[at * D + lane * N + j] * g;
+    }
+  }
+  if constexpr (W > 1) {
+    __shared__ float part[W][D], stat[W][2];
+#pragma unroll
+    for (int j = 0; j < N; ++j) part[turn][lane * N + j] = x[j];
+    if (lane == 0) { stat[turn][0] = m; stat[turn][1] = l; }
+    __syncthreads();
+    if (turn) return;
+#pragma unroll
+    for (int i = 1; i < W; ++i) {
+      const float mi = stat[i][0], now = __builtin_elementwise_maximum(m, mi);
+      const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now), g = mi == now ? 1.0f : __builtin_amdgcn_exp2f(mi - now);
+      m = now;
+      l = l * f + stat[i][1] * g;
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = x[j] * f + part[i][lane * N + j] * g;
+    }
+  }
+  if (!mine) return;
+  uint16_t* at = a.out + row * a.out_token + head * a.out_head + lane * N;
+#pragma unroll
+  for (int j = 0; j < N; ++j) at[j] = from_float<HALF>(q.bad ? __builtin_nanf("") : l == 0 ? 0.0f : x[j] / l);
+  if (a.lse && lane == 0) a.lse[(int64_t)row * a.q_heads + head] = q.bad ? __builtin_nanf("") : l == 0 ? -kInf : ((m - lift) + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-template <int D>
-hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, bool half, bool eight, hipStream_t stream) {
-  const dim3 grid(b.tokens, a.q_heads);
-  if (half && eight) attend_row<D, true, true><<<grid, kWave, 0, stream>>>(c, b, a);
-  else if (half) attend_row<D, true, false><<<grid, kWave, 0, stream>>>(c, b, a);
-  else if (eight) attend_row<D, false, true><<<grid, kWave, 0, stream>>>(c, b, a);
-  else attend_row<D, false, false><<<grid, kWave, 0, stream>>>(c, b, a);
+template <int D, bool HALF>
+hipError_t join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int shift, float lift, hipStream_t stream) {
+  const int rows = b.tokens * a.q_heads;
+  if (parts.splits > 8) join_stretches<D, HALF, kJoinWaves><<<rows, kJoinWaves * kWave, 0, stream>>>(c, b, a, parts, shift, lift);
+  else join_stretches<D, HALF, 1><<<(rows + kJoinWaves - 1) / kJoinWaves, kJoinWaves * kWave, 0, stream>>>(c, b, a, parts, shift, lift);
   return hipGetLastError();
+}
+
+// Up to 64 rows that share a key/value head (32 of 256 dims) are few: there the reading of the cache bounds, and beyond it
+// the matrix unit.
+bool few_rows(int q_heads, int kv_heads, int max_tokens, int head_dim) {
+  return (int64_t)(q_heads / kv_heads) * max_tokens <= (head_dim == 256 ? 32 : 64);
 }
 
 }  // namespace
 
-static bool few_rows(int q_heads, int kv_heads, int max_tokens, int head_dim) {
-  return (int64_t)(q_heads / kv_heads) * max_tokens <= (head_dim == 256 ? 32 : 64);
+hipError_t launch_join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int shift, float lift, int head_dim, bool half, hipStream_t stream) {
+  if (head_dim == 64) return half ? join<64, true>(c, b, a, parts, shift, lift, stream) : join<64, false>(c, b, a, parts, shift, lift, stream);
+  if (head_dim == 128) return half ? join<128, true>(c, b, a, parts, shift, lift, stream) : join<128, false>(c, b, a, parts, shift, lift, stream);
+  return half ? join<256, true>(c, b, a, parts, shift, lift, stream) : join<256, false>(c, b, a, parts, shift, lift, stream);
 }
 
 uint64_t kv_attend_workspace(const KvCache& c, const KvBatch& b, int q_heads, int max_tokens, int head_dim) {
-  return few_rows(q_heads, c.kv_heads, max_tokens, head_dim) ? kv_attend_few_workspace(c, b, q_heads, max_tokens, head_dim) : 0;
+  return few_rows(q_heads, c.kv_heads, max_tokens, head_dim) ? kv_attend_few_workspace(c, b, q_heads, max_tokens, head_dim)
+                                                             : kv_attend_many_workspace(c, b, q_heads, head_dim);
 }
 
 hipError_t launch_kv_attend(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream) {
   if (few_rows(a.q_heads, c.kv_heads, a.max_tokens, head_dim)) return launch_kv_attend_few(c, b, a, head_dim, half, eight, stream);
-  if (head_dim == 64) return launch<64>(c, b, a, half, eight, stream);
-  if (head_dim == 128) return launch<128>(c, b, a, half, eight, stream);
-  return launch<256>(c, b, a, half, eight, stream);
+  return launch_kv_attend_many(c, b, a, head_dim, half, eight, stream);
 }
 
 }  // namespace amem

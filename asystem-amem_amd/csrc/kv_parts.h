@@ -1,0 +1,77 @@
+// How attention deals out its work: units of rows that share a key/value head, and stretches of the positions they see.
+#ifndef AMEM_KV_PARTS_H_
+#define AMEM_KV_PARTS_H_
+
+#include "kv_device.h"
+
+namespace amem {
+
+// How a call's rows and positions are dealt out.
+struct Parts {
+  int stretch;   // positions of a workgroup, a multiple of 64
+  int units;
+  int splits;    // most stretches of a unit
+  float* sums;   // [unit][kv head][split][row][dim]
+  float* stats;  // [unit][kv head][split][row]{m, l}, m in units of log 2
+};
+
+namespace {
+
+// A unit: some rows of one sequence (row r is head r % group of new token r / group), and the positions they see.
+struct Unit {
+  int s, first, rows;  // the sequence, the first of its rows, how many
+  int lo, to;          // positions that some row sees: [lo, to)
+  int from;            // lo, down to a multiple of 64
+  int all_from, all_to;  // positions that every row sees
+};
+
+__device__ __forceinline__ void row_range(const KvAttend& a, const KvSeq& q, int token, int& from, int& to) {
+  const int pos = q.context - q.n + token;
+  to = a.causal && pos + 1 < q.context ? pos + 1 : q.context;
+  from = a.window && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
+}
+
+// The unit of sequence s that starts at row `tile` << shift; false if there are no rows.
+__device__ __forceinline__ bool unit_at(const KvBatch& b, const KvAttend& a, int group, int shift, int s, int tile, const KvSeq& q, Unit& u) {
+  u.s = s;
+  u.first = tile << shift;
+  u.rows = q.n * group - u.first;
+  if (u.rows <= 0) return false;
+  if (u.rows > 1 << shift) u.rows = 1 << shift;
+  row_range(a, q, u.first / group, u.lo, u.all_to);
+  row_range(a, q, (u.first + u.rows - 1) / group, u.all_from, u.to);
+  u.from = u.lo & ~63;
+  return true;
+}
+
+__device__ __forceinline__ bool find_unit(const KvBatch& b, const KvAttend& a, int group, int shift, int index, KvSeq& q, Unit& u) {
+  int s;
+  if (b.cu_tokens) {
+    s = find_sequence(b, index, shift, 1, group);
+    if (s < 0) return false;
+    index -= kv_unit_base(b, s, shift, 1, group);
+  } else {
+    const int each = ((b.uniform * group - 1) >> shift) + 1;
+    s = index / each;
+    index -= s * each;
+  }
+  q = kv_seq(b, s);
+  return unit_at(b, a, group, shift, s, index, q, u);
+}
+
+// Where a stretch's part of a unit is kept.
+__device__ __forceinline__ int64_t part_of(const KvCache& c, const Parts& parts, int unit, int kvh, int split) {
+  return ((int64_t)unit * c.kv_heads + kvh) * parts.splits + split;
+}
+
+inline int units_of(const KvBatch& b, int group, int shift) {
+  return b.cu_tokens ? kv_units(b, shift, 1, group) : b.sequences * (((b.uniform * group - 1) >> shift) + 1);
+}
+
+}  // namespace
+
+// Joins the stretches of every row: kv_attention.hip. `shift`: log2 of a unit's rows; `lift`: what the kernel added to m.
+hipError_t launch_join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int shift, float lift, int head_dim, bool half, hipStream_t stream);
+
+}  // namespace amem
+#endif
