@@ -93,13 +93,12 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
   const int read_at = EIGHT ? (8 * quad + (col >> 1)) * kPitch + (col & 1) * 8 : (4 * quad + (col >> 2)) * kPitch + (col & 3) * 8;
 
   u32x4 kreg[kRowLoads], vreg[kRowLoads];
-  int page = 0, page_next = 0;           // of position base + lane
+  int page = 0, page_next = 0, page_after = 0;  // of position base + lane of this tile (-1: out of range), the next and the one behind it
   float ks = 0, vs = 0, ks_next = 0, vs_next = 0;
 
-  auto look_up = [&](int base) {  // page of base + lane: 0 where there is none, -1 where it is out of range
-    const int p = base + lane;
-    return p < u.to && (kTile == kWave || lane < kTile) ? kv_page(c, b, u.s, p) : 0;
-  };
+  // What the page table has for position base + lane, behind the last position that one's. Nothing is done with it here: that
+  // would wait for all loads under way.
+  auto look_up = [&](int base) { return kv_table(c, b, u.s, std::min(base + (lane & (kTile - 1)), u.to - 1)); };
   auto row_of = [&](int page, int p) {
     return (int64_t)(page < 0 ? 0 : page) * c.page_stride + (int64_t)(p & slot_mask) * c.slot_stride;
   };
@@ -130,10 +129,11 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
   constexpr int kStep = kWaves * kTile;
   if (base < end) {
     page = look_up(base);
+    page_next = look_up(base + kStep);
+    page = kv_checked(c, page);
     load_rows(keys, base, page, kreg);
     load_scales(base, page, ks, vs);
     load_rows(values, base, page, vreg);
-    if (base + kStep < end) page_next = look_up(base + kStep);
   }
   for (; base < end; base += kStep) {
     const bool more = base + kStep < end;
@@ -141,6 +141,9 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
 #pragma unroll
     for (int i = 0; i < kRowLoads; ++i) *(u32x4*)(mine + (i * kRowsALoad + value_row) * kPitch + value_col) = kreg[i];
     __builtin_amdgcn_wave_barrier();
+    // before the loads that it must not wait for
+    page_after = look_up(base + 2 * kStep);
+    page_next = kv_checked(c, page_next);
     if (more) load_rows(keys, base + kStep, page_next, kreg);
     f32x4 score[NB][kGroups];
 #pragma unroll
@@ -217,7 +220,7 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
       page = page_next;
       ks = ks_next;
       vs = vs_next;
-      if (base + 2 * kStep < end) page_next = look_up(base + 2 * kStep);
+      page_next = page_after;
     }
 
     // running maximum; where it grows, what has been summed shrinks

@@ -89,8 +89,11 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend_many(KvCach
     row_range(a, q, token, row_from, row_to);
     const uint16_t* p = a.q + (q.row + token) * a.q_token + head * a.q_head;
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) qr[t] = *(const u32x4*)(p + t * 16 + half * 8);
+    for (int t = 0; t < D / 16; ++t) qr[t] = *(const u32x4*)(p + t * 16 + half * 8) ^ (a.scale < 0 ? 0x80008000u : 0u);
   }
+  // weights are exp2(score * factor - top), so the factor has to be above zero for the largest score to give the largest
+  // product: its sign is in the queries, and a scale of zero becomes one that is as good as zero
+  const float factor = fmaxf(fabsf(a.scale) * kLog2e, 0x1p-100f);
 
   float m = -kInf, l = 0;
   f32x16 sum[kDims];
@@ -106,37 +109,29 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend_many(KvCach
   const uint8_t* const keys = c.k + (int64_t)kvh * c.head_stride + my_col;
   const uint8_t* const values = c.v + (int64_t)kvh * c.head_stride + my_col;
   u32x4 kreg[kPasses], vreg[kPasses];
-  int page[kPasses], group_page = 0;  // of the tile to be loaded next: 0 where there is none, -1 where it is out of range
+  int page[kPasses], group_page = 0;  // of the tile to be loaded next, as the page table has them
   bool missing[kPasses];              // of the tile in the registers
   float ks = 0, vs = 0;               // of the tile in the registers, lane g has group g's
+  // Nothing is done with a page here: that would wait for all loads under way. Behind the last position it is that one's.
   auto look_up = [&](int base) {
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int p = base + i * kRowsAPass + my_row;
-      page[i] = p < u.to ? kv_page(c, b, u.s, p) : 0;
-    }
-    if constexpr (EIGHT) {
-      const int p = base + (lane & 3) * 16;
-      group_page = p < u.to ? kv_page(c, b, u.s, p) : 0;
-    }
+    for (int i = 0; i < kPasses; ++i) page[i] = kv_table(c, b, u.s, std::min(base + i * kRowsAPass + my_row, u.to - 1));
+    if constexpr (EIGHT) group_page = kv_table(c, b, u.s, std::min(base + (lane & 3) * 16, u.to - 1));
   };
   auto load = [&](int base) {
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       const int p = base + i * kRowsAPass + my_row;
-      missing[i] = page[i] < 0;
-      const int64_t at = (int64_t)(page[i] < 0 ? 0 : page[i]) * c.page_stride + (int64_t)(p & slot_mask) * c.slot_stride;
+      missing[i] = kv_checked(c, page[i]) < 0;
+      const int64_t at = (int64_t)(missing[i] ? 0 : page[i]) * c.page_stride + (int64_t)(p & slot_mask) * c.slot_stride;
       kreg[i] = *(const u32x4*)(keys + at);
       vreg[i] = *(const u32x4*)(values + at);
     }
     if constexpr (EIGHT) {
       const int p = base + (lane & 3) * 16;
-      ks = vs = 0;
-      if (p < u.to && (p | 15) >= u.lo) {  // a hidden group's scale may be anything
-        const int64_t at = kv_scale_offset(c, group_page < 0 ? 0 : group_page, kvh, p);
-        ks = c.k_scale[at];
-        vs = c.v_scale[at];
-      }
+      const int64_t at = kv_scale_offset(c, kv_checked(c, group_page) < 0 ? 0 : group_page, kvh, p);
+      ks = c.k_scale[at];
+      vs = c.v_scale[at];
     }
   };
   auto partial = [&](int base) { return base < u.all_from || base + kTile > u.all_to; };
@@ -148,8 +143,9 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend_many(KvCach
     if constexpr (EIGHT) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        key_scale[g] = lane_value(ks, g);
-        value_scale[g] = lane_value(vs, g);
+        const bool seen = base + g * 16 < u.to && base + g * 16 + 15 >= u.lo;  // a hidden group's scale may be anything
+        key_scale[g] = seen ? lane_value(ks, g) : 0;
+        value_scale[g] = seen ? lane_value(vs, g) : 0;
         stored_scale = __builtin_elementwise_maximum(stored_scale, value_scale[g]);
       }
       const float f = stored_scale > 0 ? 1.0f / stored_scale : 0.0f;
@@ -204,18 +200,19 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend_many(KvCach
     float f[4];
     if constexpr (EIGHT && !kFold) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) f[g] = a.scale * kLog2e * key_scale[g];
+      for (int g = 0; g < 4; ++g) f[g] = key_scale[g];
     }
     const float tile_scale = stored_scale;
     if (work) {
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
+      for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int j = 0; j < 16; ++j) score[g][j] = 0;
 #pragma unroll
-        for (int t = 0; t < D / 16; ++t)
+      for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
           score[g] = mfma32<HALF>(*(const u32x4*)(tile + (g * 32 + col) * kKeyPitch + t * 32 + half * 16), qr[t], score[g]);
-      }
     }
     if (base + kTile < end) {
       store(base + kTile, buffer ^ 1);
@@ -224,10 +221,12 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend_many(KvCach
     }
     if (!work) continue;
 
+    if constexpr (EIGHT && !kFold) {
 #pragma unroll
-    for (int g = 0; g < 2; ++g)
+      for (int g = 0; g < 2; ++g)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) score[g][j] *= EIGHT && !kFold ? f[2 * g + j / 8] : a.scale * kLog2e;
+        for (int j = 0; j < 16; ++j) score[g][j] *= f[2 * g + j / 8];
+    }
     const bool edge = base < all_from || base + kTile > all_to;
     if (edge) {
 #pragma unroll
@@ -244,7 +243,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend_many(KvCach
 #pragma unroll
       for (int j = 0; j < 16; ++j) top = __builtin_elementwise_maximum(top, score[g][j]);  // NaN stays
     top = __builtin_elementwise_maximum(top, __shfl_xor(top, 32, kWave));
-    const float now = __builtin_elementwise_maximum(m, top);
+    const float now = __builtin_elementwise_maximum(m, top * factor);
     if (__any(now != m)) {
       const float shrink = now == m ? 1.0f : __builtin_amdgcn_exp2f(m - now);
       l *= shrink;
@@ -268,7 +267,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend_many(KvCach
     for (int g = 0; g < 2; ++g) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        score[g][j] = __builtin_amdgcn_exp2f(score[g][j] - sub);
+        score[g][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[g][j], factor, -sub));
         l += score[g][j];
       }
 #pragma unroll

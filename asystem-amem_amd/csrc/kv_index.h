@@ -60,11 +60,15 @@ AMEM_HD KvSeq kv_seq(const KvBatch& b, int s) {
   return q;
 }
 
-// The page that holds position `p` (0 <= p < context of a sequence that is not bad), or -1.
-AMEM_HD int kv_page(const KvCache& c, const KvBatch& b, int s, int p) {
-  const int page = b.page_table[(int64_t)s * b.table_stride + (p >> c.page_shift)];
-  return page >= 0 && page < c.pages ? page : -1;
+// What the page table has for position `p` (0 <= p < context of a sequence that is not bad): to be checked before it is used.
+AMEM_HD int kv_table(const KvCache& c, const KvBatch& b, int s, int p) {
+  return b.page_table[(int64_t)s * b.table_stride + (p >> c.page_shift)];
 }
+
+AMEM_HD int kv_checked(const KvCache& c, int page) { return page >= 0 && page < c.pages ? page : -1; }
+
+// The page that holds position `p`, or -1.
+AMEM_HD int kv_page(const KvCache& c, const KvBatch& b, int s, int p) { return kv_checked(c, kv_table(c, b, s, p)); }
 
 // Byte offset of a slot's dims; `page` as kv_page gives it and not -1.
 AMEM_HD int64_t kv_offset(const KvCache& c, int page, int head, int p) {
