@@ -73,7 +73,7 @@ int check_batch(const char* what, const amem_kv_batch* b, const KvCache& c, bool
   NEED(b, "batch is NULL");
   NEED(b->sequences >= 0 && b->sequences <= 1 << 20 && b->tokens >= 0 && b->tokens <= 1 << 24,
        "sequences or tokens out of range");
-  NEED((int64_t)b->sequences * c.kv_heads <= 1 << 28, "sequences * kv_heads out of range");
+  NEED((int64_t)(b->tokens / 16 + 2 * b->sequences) * c.kv_heads <= 1 << 28, "tokens or sequences times kv_heads out of range");
   NEED(b->max_tokens >= 0 && b->max_tokens <= b->tokens, "max_tokens is not between 0 and tokens");
   NEED(b->table_pages >= 0 && b->table_stride >= b->table_pages, "table_pages or table_stride");
   NEED(b->max_context >= 0 && b->max_context < 1 << 30 &&

@@ -42,8 +42,8 @@ __device__ __forceinline__ float lane_value(float x, int lane) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
 }
 
-// D dims, 16 bits of fp16 (HALF) or bf16, a cache of e4m3 (EIGHT).
-template <int D, bool HALF, bool EIGHT>
+// D dims, 16 bits of fp16 (HALF) or bf16, a cache of e4m3 (EIGHT), pages of at least 16 slots (WIDE).
+template <int D, bool HALF, bool EIGHT, bool WIDE>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend_many(KvCache c, KvBatch b, KvAttend a, Parts parts) {
   constexpr int kElement = EIGHT ? 1 : 2;
   constexpr int kRowLanes = D * kElement / 16;    // threads that load a position's key, or value
@@ -106,30 +106,59 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend_many(KvCach
   // ---- loading: a thread's rows of a tile
   const int my_row = tid / kRowLanes, my_col = tid % kRowLanes * 16;
   const int slot_mask = (1 << c.page_shift) - 1;
-  const uint8_t* const keys = c.k + (int64_t)kvh * c.head_stride + my_col;
-  const uint8_t* const values = c.v + (int64_t)kvh * c.head_stride + my_col;
+  const uint8_t* const keys = c.k + (int64_t)kvh * c.head_stride;
+  const uint8_t* const values = c.v + (int64_t)kvh * c.head_stride;
   u32x4 kreg[kPasses], vreg[kPasses];
-  int page[kPasses], group_page = 0;  // of the tile to be loaded next, as the page table has them
-  bool missing[kPasses];              // of the tile in the registers
-  float ks = 0, vs = 0;               // of the tile in the registers, lane g has group g's
+  // Pages of the tile to be loaded next, as the page table has them. WIDE: 16 positions lie in one page, and lane g has that
+  // of group g; else each of the thread's rows has its own.
+  int page[WIDE ? 1 : kPasses];
+  uint32_t missing = 0;  // groups, or rows, of the tile in the registers whose page is out of range
+  float ks = 0, vs = 0;  // of the tile in the registers, lane g has group g's
   // Nothing is done with a page here: that would wait for all loads under way. Behind the last position it is that one's.
   auto look_up = [&](int base) {
+    if constexpr (WIDE) {
+      page[0] = kv_table(c, b, u.s, std::min(base + (lane & 3) * 16, u.to - 1));
+    } else {
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) page[i] = kv_table(c, b, u.s, std::min(base + i * kRowsAPass + my_row, u.to - 1));
-    if constexpr (EIGHT) group_page = kv_table(c, b, u.s, std::min(base + (lane & 3) * 16, u.to - 1));
+      for (int i = 0; i < kPasses; ++i) page[i] = kv_table(c, b, u.s, std::min(base + i * kRowsAPass + my_row, u.to - 1));
+    }
   };
+  // this thread's offset in a group: 32 bits, since a page's rows span less than 2^31 bytes
+  const uint32_t my_off = (uint32_t)((my_row & 15) * (int)c.slot_stride + my_col);
   auto load = [&](int base) {
+    missing = 0;
+    if constexpr (WIDE) {
+      int64_t at[4];
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int p = base + i * kRowsAPass + my_row;
-      missing[i] = kv_checked(c, page[i]) < 0;
-      const int64_t at = (int64_t)(missing[i] ? 0 : page[i]) * c.page_stride + (int64_t)(p & slot_mask) * c.slot_stride;
-      kreg[i] = *(const u32x4*)(keys + at);
-      vreg[i] = *(const u32x4*)(values + at);
+      for (int g = 0; g < 4; ++g) {
+        int where = kv_checked(c, __builtin_amdgcn_readlane(page[0], g));
+        if (where < 0) missing |= 1u << g;
+        where = where < 0 ? 0 : where;
+        at[g] = (int64_t)where * c.page_stride + (int64_t)(base + g * 16 & slot_mask) * c.slot_stride;
+      }
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        constexpr int kGroupsAPass = (kRowsAPass + 15) / 16;
+        const int g0 = i * kRowsAPass / 16, r0 = i * kRowsAPass % 16;
+        int64_t from = at[g0];
+#pragma unroll
+        for (int g = 1; g < kGroupsAPass; ++g) from = my_row >> 4 >= g ? at[g0 + g] : from;
+        from += r0 * c.slot_stride;
+        kreg[i] = *(const u32x4*)(keys + from + my_off);
+        vreg[i] = *(const u32x4*)(values + from + my_off);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int p = base + i * kRowsAPass + my_row, where = kv_checked(c, page[i]);
+        if (where < 0) missing |= 1u << i;
+        const int64_t at = (int64_t)(where < 0 ? 0 : where) * c.page_stride + (int64_t)(p & slot_mask) * c.slot_stride + my_col;
+        kreg[i] = *(const u32x4*)(keys + at);
+        vreg[i] = *(const u32x4*)(values + at);
+      }
     }
     if constexpr (EIGHT) {
-      const int p = base + (lane & 3) * 16;
-      const int64_t at = kv_scale_offset(c, kv_checked(c, group_page) < 0 ? 0 : group_page, kvh, p);
+      const int64_t at = kv_scale_offset(c, kv_checked(c, page[0]) < 0 ? 0 : page[0], kvh, base + (lane & 3) * 16);
       ks = c.k_scale[at];
       vs = c.v_scale[at];
     }
@@ -157,7 +186,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend_many(KvCach
     for (int i = 0; i < kPasses; ++i) {
       const int r = i * kRowsAPass + my_row;
       u32x4 k = kreg[i], v = vreg[i];
-      if (missing[i]) k = u32x4{~0u, ~0u, ~0u, ~0u};
+      if (missing && missing >> (WIDE ? r >> 4 : i) & 1) k = u32x4{~0u, ~0u, ~0u, ~0u};
       if (edge) {
         // a weight of zero does not hide infinities and NaN: values that no row sees become zeros here, and those that
         // only some rows see are taken out of the product and added one by one
@@ -365,10 +394,13 @@ void plan(const KvCache& c, const KvBatch& b, int group, int window, Parts* part
 template <int D>
 hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, bool half, bool eight, const Parts& parts, hipStream_t stream) {
   const uint32_t grid = (uint32_t)parts.units * c.kv_heads * parts.splits;
-  if (half && eight) attend_many<D, true, true><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-  else if (half) attend_many<D, true, false><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-  else if (eight) attend_many<D, false, true><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-  else attend_many<D, false, false><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  const bool wide = c.page_shift >= 4;
+  if (half && eight) attend_many<D, true, true, true><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  else if (eight) attend_many<D, false, true, true><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  else if (half && wide) attend_many<D, true, false, true><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  else if (half) attend_many<D, true, false, false><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  else if (wide) attend_many<D, false, false, true><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  else attend_many<D, false, false, false><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || parts.splits == 1) return e;
   return launch_join(c, b, a, parts, kShift, half || eight ? 8.0f : 0.0f, D, half, stream);
 }
