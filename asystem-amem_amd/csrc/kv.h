@@ -36,7 +36,7 @@ struct KvAttend {
 // `half`: the 16-bit type is fp16, else bf16; `eight`: the cache holds e4m3.
 hipError_t launch_kv_append(const KvCache& c, const KvBatch& b, const KvAppend& a, int head_dim, bool half, bool eight, hipStream_t stream);
 hipError_t launch_kv_attend(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream);
-// Few rows: at most 64 that share a key/value head (more are right, and slow).
+// Few rows: at most 32 that share a key/value head, or 64 of 64 dims (more are right, and slow).
 hipError_t launch_kv_attend_few(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream);
 uint64_t kv_attend_few_workspace(const KvCache& c, const KvBatch& b, int q_heads, int max_tokens, int head_dim);
 hipError_t launch_kv_attend_many(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream);

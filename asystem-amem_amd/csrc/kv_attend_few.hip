@@ -1,4 +1,4 @@
-// Attention over a paged key/value cache for few rows: single tokens, drafted tokens, up to 64 rows that share a
+// Attention over a paged key/value cache for few rows: single tokens, drafted tokens, up to 32 rows (64 of 64 dims) that share a
 // key/value head (the rows of a sequence are its new tokens times the query heads of that head's group).
 //
 //   s_p = scale q.k_p,  m = max s_p,  l = sum exp(s_p - m),  out = sum exp(s_p - m) v_p / l,  lse = m + log l
@@ -19,13 +19,18 @@ namespace amem {
 namespace {
 
 constexpr int kWaves = 4;
+constexpr int kLeast = 256;   // positions of a workgroup, at least: shorter ones and no join would both be slower, down to a context of 500
 constexpr int kTarget = 512;  // workgroups that a call is cut into, where its contexts are long enough
+
+// Whether a wave has a SIMD, and all of its registers, to itself: where two would spill.
+template <int D, bool EIGHT, int NB>
+constexpr bool kOneWave = D == 256 && !(EIGHT && NB == 1);
 
 // D dims, 16 bits of fp16 (HALF) or bf16, a cache of e4m3 (EIGHT), NB blocks of 16 rows, pages of at least 16 slots (WIDE).
 template <int D, bool HALF, bool EIGHT, int NB, bool WIDE>
-__global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_few(KvCache c, KvBatch b, KvAttend a, Parts few) {
+__global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) void attend_few(KvCache c, KvBatch b, KvAttend a, Parts few) {
   constexpr int kElement = EIGHT ? 1 : 2;
-  constexpr int kTile = EIGHT ? 64 : 32;               // positions of a tile
+  constexpr int kTile = EIGHT && NB == 1 && D == 64 ? 64 : 32;  // positions of a tile
   constexpr int kGroups = kTile / 16;                  // of 16 positions: rows of an operand, and never over a page's end
   constexpr int kRowLanes = D * kElement / 16;         // lanes that load a position's key, or value
   constexpr int kRowsALoad = kWave / kRowLanes;
@@ -52,22 +57,32 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
   const int end = begin + few.stretch < u.to ? begin + few.stretch : u.to;
   const int col = lane & 15, quad = lane >> 4;
 
-  // queries: the operand of a block of rows, dims in the order of the keys' registers
-  u32x4 qr[NB][D / 32];
+  // Queries, the operand of a block of rows: dims in the order of the keys' operand. More than one block leaves no registers
+  // for them; they are in LDS then, read once a tile.
+  constexpr bool kQueriesInLds = NB > 1;
+  constexpr int kQueryPitch = D * 2 + 16;
+  __shared__ __attribute__((aligned(16))) uint8_t lds_q[kQueriesInLds ? 16 * NB * kQueryPitch : 16];
+  u32x4 qr[kQueriesInLds ? 1 : D / 32];
   int row_from[NB], row_to[NB];
+  auto query = [&](int r) {
+    if (r >= u.rows) r = u.rows - 1;
+    r += u.first;
+    return a.q + (q.row + r / group) * a.q_token + (kvh * group + r % group) * a.q_head;
+  };
+  auto dim_of = [&](int t) { return EIGHT ? (t / 2) * 64 + quad * 16 + (t % 2) * 8 : t * 32 + quad * 8; };
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     int r = n * 16 + col;
     if (r >= u.rows) r = u.rows - 1;
-    r += u.first;
-    const int token = r / group;
-    row_range(a, q, token, row_from[n], row_to[n]);
-    const uint16_t* p = a.q + (q.row + token) * a.q_token + (kvh * group + r % group) * a.q_head;
+    row_range(a, q, (u.first + r) / group, row_from[n], row_to[n]);
+  }
+  if constexpr (kQueriesInLds) {
+    for (int i = threadIdx.x; i < 16 * NB * (D / 8); i += kWaves * kWave)
+      *(u32x4*)(lds_q + i / (D / 8) * kQueryPitch + i % (D / 8) * 16) = *(const u32x4*)(query(i / (D / 8)) + i % (D / 8) * 8);
+    __syncthreads();
+  } else {
 #pragma unroll
-    for (int t = 0; t < D / 32; ++t) {
-      const int d = EIGHT ? (t / 2) * 64 + quad * 16 + (t % 2) * 8 : t * 32 + quad * 8;
-      qr[n][t] = *(const u32x4*)(p + d);
-    }
+    for (int t = 0; t < D / 32; ++t) qr[t] = *(const u32x4*)(query(col) + dim_of(t));
   }
 
   float m[NB], l[NB];
@@ -94,7 +109,7 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
 
   u32x4 kreg[kRowLoads], vreg[kRowLoads];
   int page = 0, page_next = 0, page_after = 0;  // of position base + lane of this tile (-1: out of range), the next and the one behind it
-  float ks = 0, vs = 0, ks_next = 0, vs_next = 0;
+  float ks = 0, vs = 0;
 
   // What the page table has for position base + lane, behind the last position that one's. Nothing is done with it here: that
   // would wait for all loads under way.
@@ -104,24 +119,27 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
   };
   // this lane's offset in a group that lies in one page: 32 bits, since a page's rows span less than 2^31 bytes
   const uint32_t lane_off = (uint32_t)((value_row & 15) * (int)c.slot_stride + value_col);
-  auto load_rows = [&](const uint8_t* from, int base, int page, u32x4 (&to)[kRowLoads]) {
+  // Loads are never skipped, which would make the compiler keep the registers' old contents and copy them about: behind the last
+  // tile (`more` false) all of them read one line.
+  auto load_rows = [&](const uint8_t* from, int base, int page, bool more, u32x4 (&to)[kRowLoads]) {
 #pragma unroll
     for (int i = 0; i < kRowLoads; ++i) {
       const uint8_t* at;
-      if constexpr (WIDE) at = from + row_of(__builtin_amdgcn_readlane(page, i * kRowsALoad & ~15), base + i * kRowsALoad) + lane_off;
-      else at = from + row_of(__shfl(page, i * kRowsALoad + value_row, kWave), base + i * kRowsALoad + value_row) + value_col;
+      if constexpr (WIDE) {
+        const int64_t row = row_of(__builtin_amdgcn_readlane(page, i * kRowsALoad & ~15), base + i * kRowsALoad);
+        at = from + (more ? row : 0) + (more ? lane_off : 0);
+      } else {
+        const int64_t row = row_of(__shfl(page, i * kRowsALoad + value_row, kWave), base + i * kRowsALoad + value_row) + value_col;
+        at = from + (more ? row : 0);
+      }
       to[i] = __builtin_nontemporal_load((const u32x4*)at);
     }
   };
   auto load_scales = [&](int base, int page, float& k, float& v) {
     if constexpr (EIGHT) {
-      const int p = base + lane;
-      k = v = 0;
-      if (p < u.to && (p | 15) >= u.lo) {  // a hidden group's scale may be anything
-        const int64_t at = kv_scale_offset(c, page < 0 ? 0 : page, kvh, p);
-        k = c.k_scale[at];
-        v = c.v_scale[at];
-      }
+      const int64_t at = kv_scale_offset(c, page < 0 ? 0 : page, kvh, base + lane);
+      k = c.k_scale[at];
+      v = c.v_scale[at];
     }
   };
 
@@ -131,9 +149,9 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
     page = look_up(base);
     page_next = look_up(base + kStep);
     page = kv_checked(c, page);
-    load_rows(keys, base, page, kreg);
+    load_rows(keys, base, page, true, kreg);
     load_scales(base, page, ks, vs);
-    load_rows(values, base, page, vreg);
+    load_rows(values, base, page, true, vreg);
   }
   for (; base < end; base += kStep) {
     const bool more = base + kStep < end;
@@ -144,24 +162,28 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
     // before the loads that it must not wait for
     page_after = look_up(base + 2 * kStep);
     page_next = kv_checked(c, page_next);
-    if (more) load_rows(keys, base + kStep, page_next, kreg);
+    load_rows(keys, base + kStep, page_next, more, kreg);
     f32x4 score[NB][kGroups];
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
+    for (int g = 0; g < kGroups; ++g)
 #pragma unroll
       for (int n = 0; n < NB; ++n) score[n][g] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int t = 0; t < D * kElement / 64; ++t) {
-        const u32x4 k = *(const u32x4*)(mine + (g * 16 + col) * kPitch + t * 64 + quad * 16);
+    for (int t = 0; t < D / 32; ++t) {
+      u32x4 qt[NB];
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          if constexpr (EIGHT) {
-            score[n][g] = mfma16<HALF>(widen<HALF>(u32x2{k[0], k[1]}), qr[n][2 * t], score[n][g]);
-            score[n][g] = mfma16<HALF>(widen<HALF>(u32x2{k[2], k[3]}), qr[n][2 * t + 1], score[n][g]);
-          } else {
-            score[n][g] = mfma16<HALF>(k, qr[n][t], score[n][g]);
-          }
-        }
+      for (int n = 0; n < NB; ++n) {
+        if constexpr (kQueriesInLds) qt[n] = *(const u32x4*)(lds_q + (n * 16 + col) * kQueryPitch + dim_of(t) * 2);
+        else qt[n] = qr[t];
+      }
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const uint8_t* p = mine + (g * 16 + col) * kPitch;
+        u32x4 k;
+        if constexpr (EIGHT) k = widen<HALF>(*(const u32x2*)(p + t / 2 * 64 + quad * 16 + t % 2 * 8));
+        else k = *(const u32x4*)(p + t * 64 + quad * 16);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) score[n][g] = mfma16<HALF>(k, qt[n], score[n][g]);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -169,24 +191,11 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
     // scores in units of log 2
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      const float f = a.scale * kLog2e * (EIGHT ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), g * 16)) : 1.0f);
+      const float f = a.scale * kLog2e * (EIGHT ? lane_value(ks, g * 16) : 1.0f);
 #pragma unroll
       for (int n = 0; n < NB; ++n) score[n][g] *= f;
     }
-    // values that no row sees are stored as zeros, since a weight of zero does not hide infinities and NaN
-    bool odd = false;  // some positions have such values, and may be hidden from some rows
     if (!whole) {
-#pragma unroll
-      for (int i = 0; i < kRowLoads; ++i) {
-        const int p = base + i * kRowsALoad + value_row;
-        if (p < u.lo || p >= u.to) vreg[i] = u32x4{0, 0, 0, 0};
-        // those are taken out of the product and added one by one below
-        const uint64_t lanes = __ballot(not_finite<HALF, EIGHT>(vreg[i]));
-        if (lanes) {
-          odd = true;
-          if (lanes >> (value_row * kRowLanes) & ((1ull << kRowLanes) - 1)) vreg[i] = u32x4{0, 0, 0, 0};
-        }
-      }
       const uint64_t bad = __ballot(page < 0);
 #pragma unroll
       for (int g = 0; g < kGroups; ++g)
@@ -209,19 +218,31 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
           for (int n = 0; n < NB; ++n)
             if (bad >> (g * 16 + quad * 4 + i) & 1) score[n][g][i] = __builtin_nanf("");
     }
+    // values that no row sees are stored as zeros, since a weight of zero does not hide infinities and NaN
+    bool odd = false;  // some positions have such values, and may be hidden from some rows
+    if (whole) {
 #pragma unroll
-    for (int i = 0; i < kRowLoads; ++i) *(u32x4*)(mine + write_at + lds_row(i * kRowsALoad) * kPitch) = vreg[i];
-    __builtin_amdgcn_wave_barrier();
-    const float vs_now = vs;
-    const int page_now = page;
-    if (more) {
-      load_scales(base + kStep, page_next, ks_next, vs_next);
-      load_rows(values, base + kStep, page_next, vreg);
-      page = page_next;
-      ks = ks_next;
-      vs = vs_next;
-      page_next = page_after;
+      for (int i = 0; i < kRowLoads; ++i) *(u32x4*)(mine + write_at + lds_row(i * kRowsALoad) * kPitch) = vreg[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRowLoads; ++i) {
+        const int p = base + i * kRowsALoad + value_row;
+        u32x4 v = vreg[i];
+        if (p < u.lo || p >= u.to) v = u32x4{0, 0, 0, 0};
+        // those are taken out of the product and added one by one below
+        const uint64_t lanes = __ballot(not_finite<HALF, EIGHT>(v));
+        odd |= lanes != 0;
+        if (lanes >> (value_row * kRowLanes) & ((1ull << kRowLanes) - 1)) v = u32x4{0, 0, 0, 0};
+        *(u32x4*)(mine + write_at + lds_row(i * kRowsALoad) * kPitch) = v;
+      }
     }
+    __builtin_amdgcn_wave_barrier();
+    const int page_now = page;
+    page = page_next;
+    page_next = page_after;
+    float ks_next = 0, vs_next = 0;
+    load_scales(base + kStep, page, ks_next, vs_next);
+    load_rows(values, base + kStep, page, more, vreg);
 
     // running maximum; where it grows, what has been summed shrinks
     bool grew = false;
@@ -245,7 +266,8 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
       float top = 0;
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        f_scale[g] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs_now), g * 16));
+        const bool seen = base + g * 16 < u.to && base + g * 16 + 15 >= u.lo;  // a hidden group's scale may be anything
+        f_scale[g] = seen ? lane_value(vs, g * 16) : 0;
         top = __builtin_elementwise_maximum(top, f_scale[g]);
       }
       if (!(top <= unit_scale)) {
@@ -336,6 +358,8 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
         __builtin_amdgcn_wave_barrier();
       }
     }
+    ks = ks_next;
+    vs = vs_next;
   }
 
   // the four waves' parts become one
@@ -401,11 +425,10 @@ __global__ __launch_bounds__(kWaves * kWave, NB * D >= 512 ? 1 : 2) void attend_
 // values are read once.
 int blocks_of(int group, int max_tokens, int head_dim) {
   const int64_t rows = (int64_t)group * max_tokens;
-  return rows <= 16 ? 1 : rows <= 32 || head_dim == 256 ? 2 : 4;
+  return rows <= 16 ? 1 : rows <= 32 || head_dim > 64 ? 2 : 4;
 }
 
-// Stretches are as long as leaves about kTarget workgroups (eight for each compute unit, of which it holds two to four at a
-// time), and at least a tile for each wave.
+// Stretches are as long as leaves about kTarget workgroups, and at least kLeast positions.
 void plan(const KvCache& c, const KvBatch& b, int group, int blocks, int window, Parts* few) {
   const int shift = blocks == 1 ? 4 : blocks == 2 ? 5 : 6;
   int64_t span = b.max_context;
@@ -414,8 +437,7 @@ void plan(const KvCache& c, const KvBatch& b, int group, int blocks, int window,
   few->units = units_of(b, group, shift);
   const int64_t all = (int64_t)few->units * c.kv_heads * span;
   const int64_t step = kWaves * 64;
-  int64_t stretch = ((all + kTarget - 1) / kTarget + step - 1) / step * step;
-  if (stretch < step) stretch = step;
+  const int64_t stretch = std::max<int64_t>(((all + kTarget - 1) / kTarget + step - 1) / step * step, kLeast);
   few->stretch = (int)stretch;
   few->splits = span > stretch ? (int)((span + stretch - 1) / stretch) : 1;
 }
@@ -438,8 +460,8 @@ template <int D, bool HALF, bool EIGHT>
 hipError_t launch_blocks(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& few, int blocks, hipStream_t stream) {
   if (blocks == 1) return launch_few<D, HALF, EIGHT, 1>(c, b, a, few, stream);
   if (blocks == 2) return launch_few<D, HALF, EIGHT, 2>(c, b, a, few, stream);
-  if constexpr (D < 256) return launch_few<D, HALF, EIGHT, 4>(c, b, a, few, stream);
-  return hipErrorInvalidValue;
+  if constexpr (D == 64) return launch_few<D, HALF, EIGHT, 4>(c, b, a, few, stream);
+  else return launch_few<D, HALF, EIGHT, 2>(c, b, a, few, stream);
 }
 
 template <int D>
@@ -456,7 +478,7 @@ uint64_t kv_attend_few_workspace(const KvCache& c, const KvBatch& b, int q_heads
   const int shift = blocks == 1 ? 4 : blocks == 2 ? 5 : 6;
   const int64_t units = (int64_t)units_of(b, group, shift) * c.kv_heads;
   if (!units) return 0;
-  const int64_t splits = std::min<int64_t>((b.max_context + kWaves * 64 - 1) / (kWaves * 64), (kTarget + units - 1) / units);
+  const int64_t splits = std::min<int64_t>((b.max_context + kLeast - 1) / kLeast, (kTarget + units - 1) / units);
   return splits < 2 ? 0 : (uint64_t)(units * splits * (16 * blocks)) * (head_dim + 2) * 4;
 }
 

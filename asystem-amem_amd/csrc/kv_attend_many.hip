@@ -38,10 +38,6 @@ __device__ __forceinline__ u32x4 widen_scaled(u32x2 x, float scale) {
   return y;
 }
 
-__device__ __forceinline__ float lane_value(float x, int lane) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
-}
-
 // D dims, 16 bits of fp16 (HALF) or bf16, a cache of e4m3 (EIGHT), pages of at least 16 slots (WIDE).
 template <int D, bool HALF, bool EIGHT, bool WIDE>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend_many(KvCache c, KvBatch b, KvAttend a, Parts parts) {

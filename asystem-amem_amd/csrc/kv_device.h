@@ -73,6 +73,10 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   else return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)lo, (__bf16)hi});
 }
 
+__device__ __forceinline__ float lane_value(float x, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
+}
+
 // Whether any of 16 bytes of values is an infinity or NaN.
 template <bool HALF, bool EIGHT>
 __device__ __forceinline__ bool not_finite(u32x4 x) {

@@ -15,12 +15,22 @@ for instance. Arguments that do not fit raise ValueError before anything is enqu
 raises KvError.
 """
 import ctypes as C
+import struct
 
 from . import binding
 
 BF16, F16, E4M3 = range(3)
 MAX_AXES = 4
-_TYPES = {"torch.bfloat16": BF16, "torch.float16": F16, "torch.float8_e4m3fn": E4M3}
+_TYPES = {"torch.bfloat16": BF16, "torch.float16": F16, "torch.float8_e4m3fn": E4M3, "torch.float32": -2, "torch.int32": -3}
+_kinds = {}     # by the dtypes themselves, as they are met
+
+
+def _kind(t):
+    kind = _kinds.get(t.dtype)
+    if kind is None:
+        kind = _kinds[t.dtype] = _TYPES.get(str(t.dtype), -1)
+    return kind
+
 
 
 class KvError(RuntimeError):
@@ -54,9 +64,14 @@ class AttentionArgs(C.Structure):
         ("scale", C.c_float)] + [(n, C.c_int32) for n in ("type", "q_heads", "causal", "window", "reserved")]
 
 
+# The two records of a call's arguments as bytes: a quarter of what filling the structures takes.
+_append_args = struct.Struct("=7Q9q10i").pack
+_attention_args = struct.Struct("=5Q4qf5i").pack
+
+# the records by address: a structure's byref, or bytes
 _SIGNATURES = {
-    "amem_kv_append": (C.c_int, [C.POINTER(CacheInfo), C.POINTER(BatchInfo), C.POINTER(AppendArgs), C.c_void_p]),
-    "amem_kv_attention": (C.c_int, [C.POINTER(CacheInfo), C.POINTER(BatchInfo), C.POINTER(AttentionArgs), C.c_void_p]),
+    "amem_kv_append": (C.c_int, [C.c_void_p] * 4),
+    "amem_kv_attention": (C.c_int, [C.c_void_p] * 4),
     "amem_kv_attention_workspace": (C.c_int, [C.POINTER(CacheInfo), C.POINTER(BatchInfo), C.c_int, C.POINTER(C.c_uint64)]),
 }
 _entry = {}
@@ -77,6 +92,13 @@ def load():
     return lib
 
 
+def _packed(pack, *values):
+    try:
+        return pack(*values)
+    except (struct.error, OverflowError) as e:
+        raise ValueError("an argument is no number of its type: %s" % e) from None
+
+
 def _call(name, *args):
     if not _entry:
         load()
@@ -91,14 +113,15 @@ def _need(ok, why):
 
 
 def _device(t):
-    d = t.device
-    _need(d.type == "cuda", "a tensor is not on a GPU")
-    return d.index or 0
+    _need(t.device.type == "cuda", "a tensor is not on a GPU")
+    return t.device
 
 
 def _is(t, dtype, device, what):
-    _need(str(t.dtype) == dtype, "%s is not %s" % (what, dtype))
-    _need(_device(t) == device, "%s is on another device than the cache" % what)
+    if _kind(t) != _TYPES["torch." + dtype]:
+        raise ValueError("%s is not %s" % (what, dtype))
+    if t.device != device:
+        raise ValueError("%s is on another device than the cache" % what)
 
 
 class Cache:
@@ -108,18 +131,18 @@ class Cache:
     def __init__(self, k, v, k_scale=None, v_scale=None):
         _need(len(k.shape) == 4 and tuple(k.shape) == tuple(v.shape) and k.stride() == v.stride() and k.dtype == v.dtype,
               "k and v differ, or are not [pages, heads, slots, dim]")
-        _need(str(k.dtype) in _TYPES, "k is not bfloat16, float16 or float8_e4m3fn")
+        kind, block = _kind(k), 0
+        _need(kind >= 0, "k is not bfloat16, float16 or float8_e4m3fn")
         pages, heads, slots, dim = k.shape
         at = k.stride()
         _need(at[3] == 1 or dim == 1, "the dims of k are not contiguous")
         device = _device(k)
         _need(_device(v) == device, "k and v are on different devices")
-        kind, block = _TYPES[str(k.dtype)], 0
         _need((kind == E4M3) == (k_scale is not None) == (v_scale is not None), "8 bits have scales, 16 have none")
-        info = CacheInfo(k.data_ptr(), v.data_ptr(), 0, 0, at[0], at[1], at[2], 0, 0, kind, device, pages, heads, slots, 0, dim, 0)
+        info = CacheInfo(k.data_ptr(), v.data_ptr(), 0, 0, at[0], at[1], at[2], 0, 0, kind, device.index or 0, pages, heads, slots, 0, dim, 0)
         if kind == E4M3:
             for t in (k_scale, v_scale):
-                _is(t, "torch.float32", device, "a tensor of scales")
+                _is(t, "float32", device, "a tensor of scales")
             shape = tuple(k_scale.shape)
             _need(shape == tuple(v_scale.shape) and k_scale.stride() == v_scale.stride() and len(shape) == 3 and shape[:2] == (pages, heads)
                   and shape[2] > 0 and slots % shape[2] == 0 and (k_scale.stride()[2] == 1 or shape[2] == 1),
@@ -144,7 +167,7 @@ class Batch:
         n = context.shape[0]
         for t, what in ((page_table, "page_table"), (context, "context"), (cu_tokens, "cu_tokens")):
             if t is not None:
-                _is(t, "torch.int32", device, what)
+                _is(t, "int32", device, what)
         _need(len(page_table.shape) == 2 and page_table.shape[0] == n and (page_table.stride()[1] == 1 or page_table.shape[1] < 2),
               "page_table is not [sequences, pages] with contiguous pages")
         _need(len(context.shape) == 1 and (n < 2 or context.stride()[0] == 1), "context is not contiguous")
@@ -173,57 +196,73 @@ class Rotation:
     def __init__(self, cos, sin, sections=None, interleaved=False):
         self.device = _device(cos)
         for t in (cos, sin):
-            _is(t, "torch.float32", self.device, "a table of the rotation")
+            _is(t, "float32", self.device, "a table of the rotation")
             _need(len(t.shape) == 2 and tuple(t.shape) == tuple(cos.shape) and t.stride() == (t.shape[1], 1), "the tables are not [rows, pairs] and contiguous")
         sections = tuple(sections) if sections else (cos.shape[1],)
         _need(len(sections) <= MAX_AXES and sum(sections) == cos.shape[1] and min(sections) >= 0, "sections are not the pairs of the axes")
         self.axes = len(sections)
-        self.sections = (C.c_int32 * MAX_AXES)(*sections)
+        self.sections = sections + (0,) * (MAX_AXES - len(sections))
         self.rows, self.dim, self.interleaved = cos.shape[0], 2 * cos.shape[1], int(interleaved)
         self.cos, self.sin = cos.data_ptr(), sin.data_ptr()
         self._keep = (cos, sin)
 
 
-def _rows(t, tokens, heads, dim, kind, device, what):
+def _rows(t, shape, kind, device, what):
     """Strides of a tensor [tokens, heads, dim]."""
-    shape, at = t.shape, t.stride()
-    if len(shape) != 3 or shape[0] != tokens or shape[2] != dim or (heads and shape[1] != heads) or at[2] != 1:
-        raise ValueError("%s is not [%d, %s, %d] with contiguous dims" % (what, tokens, heads or "heads", dim))
-    if _TYPES.get(str(t.dtype)) != kind:
+    at = t.stride()
+    if t.shape != shape or at[2] != 1:
+        raise ValueError("%s is not [%d, %d, %d] with contiguous dims" % ((what,) + shape))
+    if _kind(t) != kind:
         raise ValueError("%s has another type than the rows" % what)
-    if _device(t) != device:
+    if t.device != device:
         raise ValueError("%s is on another device than the cache" % what)
     return at
 
 
+def _heads(q):
+    shape = q.shape
+    if len(shape) != 3:
+        raise ValueError("q is not [tokens, heads, dim]")
+    return shape[1]
+
+
 def append(cache, batch, k, v, q=None, q_out=None, rotation=None, positions=None, stream=0):
     """Rows k and v [tokens, heads, dim] into the cache, k rotated; q rotated into q_out."""
-    n, dim, device = batch.tokens, cache.dim, cache.device
-    kind = _TYPES.get(str(k.dtype))
-    _need(kind in (BF16, F16), "k is not bfloat16 or float16")
-    _need(batch.device == device and (rotation is None or rotation.device == device), "tensors are on different devices")
-    ak = _rows(k, n, cache.heads, dim, kind, device, "k")
-    av = _rows(v, n, cache.heads, dim, kind, device, "v")
-    a = AppendArgs(k.data_ptr(), v.data_ptr(), 0, 0, 0, 0, 0, ak[0], ak[1], av[0], av[1], 0, 0, 0, 0, 0, kind)
+    n, device, kind = batch.tokens, cache.device, _kind(k)
+    if kind != BF16 and kind != F16:
+        raise ValueError("k is not bfloat16 or float16")
+    if batch.device != device:
+        raise ValueError("the batch is on another device than the cache")
+    shape = (n, cache.heads, cache.dim)
+    ak, av = _rows(k, shape, kind, device, "k"), _rows(v, shape, kind, device, "v")
+    q_at = q_out_at = q_token = q_head = out_token = out_head = q_heads = 0
     if q is not None:
-        _need(q_out is not None, "q without q_out")
-        a.q_heads = q.shape[1]
-        a.q_token_stride, a.q_head_stride = _rows(q, n, 0, dim, kind, device, "q")[:2]
-        a.q_out_token_stride, a.q_out_head_stride = _rows(q_out, n, q.shape[1], dim, kind, device, "q_out")[:2]
-        a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
-    if rotation is not None:
-        _need(rotation.axes == 1 or positions is not None, "several axes need positions")
-        a.cos, a.sin, a.rotary_dim, a.interleaved = rotation.cos, rotation.sin, rotation.dim, rotation.interleaved
-        a.table_rows, a.axes, a.sections = rotation.rows, rotation.axes, rotation.sections
-        if positions is not None:
-            _is(positions, "torch.int32", device, "positions")
-            shape, at = tuple(positions.shape), positions.stride()
-            _need(shape == (rotation.axes, n) or (rotation.axes == 1 and shape == (n,)), "positions are not [axes, tokens]")
-            _need(n < 2 or at[-1] == 1, "positions are not contiguous")
-            a.positions, a.positions_stride = positions.data_ptr(), at[0] if rotation.axes > 1 else n
-    else:
+        if q_out is None:
+            raise ValueError("q without q_out")
+        q_heads = _heads(q)
+        shape = (n, q_heads, cache.dim)
+        q_token, q_head, _ = _rows(q, shape, kind, device, "q")
+        out_token, out_head, _ = _rows(q_out, shape, kind, device, "q_out")
+        q_at, q_out_at = q.data_ptr(), q_out.data_ptr()
+    if rotation is None:
         _need(positions is None, "positions without rotation")
-    _call("amem_kv_append", cache._ref, batch._ref, C.byref(a), stream)
+        a = _packed(_append_args, k.data_ptr(), v.data_ptr(), q_at, q_out_at, 0, 0, 0, ak[0], ak[1], av[0], av[1], q_token, q_head, out_token,
+                         out_head, 0, kind, q_heads, 0, 0, 0, 0, 0, 0, 0, 0)
+    else:
+        r, where, apart = rotation, 0, 0
+        if r.device != device:
+            raise ValueError("the rotation is on another device than the cache")
+        if positions is not None:
+            _is(positions, "int32", device, "positions")
+            shape, at = tuple(positions.shape), positions.stride()
+            _need(shape == (r.axes, n) or (r.axes == 1 and shape == (n,)), "positions are not [axes, tokens]")
+            _need(n < 2 or at[-1] == 1, "positions are not contiguous")
+            where, apart = positions.data_ptr(), at[0] if r.axes > 1 else n
+        elif r.axes > 1:
+            raise ValueError("several axes need positions")
+        a = _packed(_append_args, k.data_ptr(), v.data_ptr(), q_at, q_out_at, r.cos, r.sin, where, ak[0], ak[1], av[0], av[1], q_token, q_head,
+                         out_token, out_head, apart, kind, q_heads, r.dim, r.interleaved, r.rows, r.axes, *r.sections)
+    _call("amem_kv_append", cache._ref, batch._ref, a, stream)
 
 
 def attention_workspace(cache, batch, q_heads):
@@ -236,20 +275,23 @@ def attention_workspace(cache, batch, q_heads):
 def attention(cache, batch, q, out, lse=None, scale=None, causal=True, window=0, workspace=None, stream=0):
     """out [tokens, heads, dim] = attention of q over the cache; lse float32 [tokens, heads]; scale: dim ** -0.5 if None;
     workspace: a contiguous tensor of at least attention_workspace() bytes."""
-    n, dim, device = batch.tokens, cache.dim, cache.device
-    kind, heads = _TYPES.get(str(q.dtype)), q.shape[1]
-    _need(kind in (BF16, F16), "q is not bfloat16 or float16")
-    _need(batch.device == device, "the batch is on another device than the cache")
-    aq = _rows(q, n, 0, dim, kind, device, "q")
-    ao = _rows(out, n, heads, dim, kind, device, "out")
+    n, dim, device, kind, heads = batch.tokens, cache.dim, cache.device, _kind(q), _heads(q)
+    if kind != BF16 and kind != F16:
+        raise ValueError("q is not bfloat16 or float16")
+    if batch.device != device:
+        raise ValueError("the batch is on another device than the cache")
+    shape = (n, heads, dim)
+    aq, ao = _rows(q, shape, kind, device, "q"), _rows(out, shape, kind, device, "out")
     lse_at = at = size = 0
     if lse is not None:
-        _is(lse, "torch.float32", device, "lse")
-        _need(tuple(lse.shape) == (n, heads) and lse.is_contiguous(), "lse is not [tokens, heads] and contiguous")
+        _is(lse, "float32", device, "lse")
+        if lse.shape != (n, heads) or not lse.is_contiguous():
+            raise ValueError("lse is not [tokens, heads] and contiguous")
         lse_at = lse.data_ptr()
     if workspace is not None:
-        _need(_device(workspace) == device and workspace.is_contiguous(), "workspace is on another device, or strided")
+        if workspace.device != device or not workspace.is_contiguous():
+            raise ValueError("workspace is on another device, or strided")
         at, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    a = AttentionArgs(q.data_ptr(), out.data_ptr(), lse_at, at, size, aq[0], aq[1], ao[0], ao[1],
-                      dim ** -0.5 if scale is None else scale, kind, heads, int(causal), window, 0)
-    _call("amem_kv_attention", cache._ref, batch._ref, C.byref(a), stream)
+    a = _packed(_attention_args, q.data_ptr(), out.data_ptr(), lse_at, at, size, aq[0], aq[1], ao[0], ao[1],
+                        dim ** -0.5 if scale is None else scale, kind, heads, 1 if causal else 0, window, 0)
+    _call("amem_kv_attention", cache._ref, batch._ref, a, stream)

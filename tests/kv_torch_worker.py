@@ -152,6 +152,9 @@ assert refused(kv.attention, w.cache, w.batch, w.q, half)
 assert refused(kv.attention, w.cache, w.batch, w.q, w.out[:, :4])
 assert refused(kv.attention, w.cache, w.batch, w.q, w.out, lse=w.lse.double())
 assert refused(kv.attention, w.cache, w.batch, w.q.transpose(1, 2), w.out)
+assert refused(kv.attention, w.cache, w.batch, w.q, w.out, window=1 << 40)
+assert refused(kv.attention, w.cache, w.batch, w.q, w.out, window=1.5)
+assert refused(kv.attention, w.cache, w.batch, w.q, w.out, scale=1e300)
 assert refused(kv.Cache, w.k, w.v)
 assert refused(kv.Cache, w.k, w.v, w.ks[:1], w.vs[:1])
 assert refused(kv.Cache, w.k.transpose(2, 3), w.v.transpose(2, 3), w.ks, w.vs)

@@ -168,3 +168,14 @@ def test_indexes_stay_inside(tmp_path):
     r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, r.stdout + r.stderr
     assert "ok" in r.stdout
+
+
+def test_packed_arguments_are_the_structures():
+    """kv.py hands records over as bytes: the same ones as the structures."""
+    numbers = list(range(1, 27))
+    a = kv.AppendArgs.from_buffer_copy(kv._append_args(*numbers))
+    got = [getattr(a, f[0]) for f in a._fields_[:-1]] + list(a.sections)
+    assert got == numbers and C.sizeof(a) == len(kv._append_args(*numbers))
+    numbers = list(range(1, 16))
+    a = kv.AttentionArgs.from_buffer_copy(kv._attention_args(*numbers))
+    assert [getattr(a, f[0]) for f in a._fields_] == numbers and C.sizeof(a) == len(kv._attention_args(*numbers))
