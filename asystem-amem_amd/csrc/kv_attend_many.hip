@@ -2,10 +2,10 @@
 //
 //   s_p = scale q.k_p,  m = max s_p,  l = sum exp(s_p - m),  out = sum exp(s_p - m) v_p / l,  lse = m + log l
 //
-// Bound by the matrix unit. A workgroup takes 128 rows that share a key/value head (32 for each of its four waves) through
-// the positions they see, 64 at a time: its threads load a tile of keys and values while the one before is worked on, and
-// put it into LDS as 16-bit numbers, where every wave reads all of it. Two tiles are held there, so that one barrier a
-// tile is enough. Products are (keys x dims)(dims x rows) and (dims x keys)(keys x rows): a lane holds scores and sums
+// Bound by the matrix unit. A workgroup takes 256 rows that share a key/value head (32 for each of its eight waves; or 128 and
+// four) through the positions they see, 64 at a time: its threads load a tile of keys and values while the one before
+// is worked on, and put it into LDS as 16-bit numbers, where every wave reads all of it. Two tiles are held there, so
+// that one barrier a tile is enough. Products are (keys x dims)(dims x rows) and (dims x keys)(keys x rows): a lane holds scores and sums
 // of one row, the weights go from the first product's result to the second's operand without leaving their lane, and
 // values are read from LDS as columns.
 #include <algorithm>
@@ -15,11 +15,7 @@
 namespace amem {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * kWave;
-constexpr int kShift = 7;      // log2 of a unit's rows
-constexpr int kTile = 64;      // positions
-constexpr int kTarget = 512;   // workgroups that fit at once; contexts are cut until there are as many
+constexpr int kTile = 64;  // positions
 
 // Eight e4m3 codes times a power of two as 16-bit numbers.
 template <bool HALF>
@@ -39,13 +35,15 @@ __device__ __forceinline__ u32x4 widen_scaled(u32x2 x, float scale) {
 }
 
 // D dims, 16 bits of fp16 (HALF) or bf16, a cache of e4m3 (EIGHT), pages of at least 16 slots (WIDE).
-template <int D, bool HALF, bool EIGHT, bool WIDE>
-__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend_many(KvCache c, KvBatch b, KvAttend a, Parts parts) {
+template <int D, bool HALF, bool EIGHT, bool WIDE, int kWaves>
+__global__ __launch_bounds__(kWaves * kWave, (D == 256 ? 1 : 2)) void attend_many(KvCache c, KvBatch b, KvAttend a, Parts parts) {
+  constexpr int kThreads = kWaves * kWave;
+  constexpr int kShift = kWaves == 8 ? 8 : 7;     // log2 of a unit's rows
   constexpr int kElement = EIGHT ? 1 : 2;
   constexpr int kRowLanes = D * kElement / 16;    // threads that load a position's key, or value
   constexpr int kRowsAPass = kThreads / kRowLanes;
   constexpr int kPasses = kTile / kRowsAPass;
-  static_assert(kPasses >= 1, "a pass is at most a tile");
+  static_assert(kRowsAPass <= kTile, "a pass is at most a tile");
   // pads: the rows that are read together are on different banks
   constexpr int kKeyPitch = D * 2 + 16, kValuePitch = D * 2 + 64, kBuffer = kTile * (kKeyPitch + kValuePitch);
   constexpr bool kHalfP = EIGHT || HALF;  // weights are fp16 where the values' type allows it
@@ -124,14 +122,14 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend_many(KvCach
   auto load = [&](int base) {
     missing = 0;
     if constexpr (WIDE) {
+      // every lane its group's, which costs a tenth of four on the scalar unit
+      const int where = kv_checked(c, page[0]);
+      missing = (uint32_t)__ballot(where < 0) & 15;
+      const int64_t mine = (int64_t)(where < 0 ? 0 : where) * c.page_stride + (base + (lane & 3) * 16 & slot_mask) * (int64_t)(int)c.slot_stride;
       int64_t at[4];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        int where = kv_checked(c, __builtin_amdgcn_readlane(page[0], g));
-        if (where < 0) missing |= 1u << g;
-        where = where < 0 ? 0 : where;
-        at[g] = (int64_t)where * c.page_stride + (int64_t)(base + g * 16 & slot_mask) * c.slot_stride;
-      }
+      for (int g = 0; g < 4; ++g)
+        at[g] = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), g) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, g));
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
         constexpr int kGroupsAPass = (kRowsAPass + 15) / 16;
@@ -374,51 +372,76 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend_many(KvCach
     a.lse[(int64_t)(q.row + token) * a.q_heads + head] = q.bad ? __builtin_nanf("") : l == 0 ? -kInf : ((m - kLift) + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// Contexts are cut only where units are fewer than fit at once, and never below 512 positions: a part costs its rows' sums
-// written and read once more.
-void plan(const KvCache& c, const KvBatch& b, int group, int window, Parts* parts) {
-  parts->units = units_of(b, group, kShift);
+// Contexts are cut only where units are fewer than fit at once (one workgroup of eight waves a compute unit, or two of four),
+// and never below 512 positions: a part costs its rows' sums written and read once more.
+constexpr int fit(int waves) { return waves == 8 ? 256 : 512; }
+
+// Eight waves of 32 rows share the loads of a tile, four need them twice as often: a chunk of 4096 over 16384 positions in
+// e4m3 takes 1.035 ms with eight and 1.090 with four. Four where there would be less than two workgroups of eight for each
+// compute unit (2048 x 2048 positions, 32 heads over 8: 69 us, and 78 with eight), for 256 dims, whose registers
+// allow one wave a SIMD, and for 64 of e4m3, where four load a tile at once.
+int waves_of(const KvCache& c, const KvBatch& b, int group, int head_dim) {
+  if (head_dim == 256 || (head_dim == 64 && c.block_shift)) return 4;
+  return (int64_t)units_of(b, group, 8) * c.kv_heads >= 2 * fit(8) ? 8 : 4;
+}
+
+void plan(const KvCache& c, const KvBatch& b, int group, int waves, int window, Parts* parts) {
+  const int shift = waves == 8 ? 8 : 7;
+  parts->units = units_of(b, group, shift);
   int64_t span = b.max_context;
-  const int64_t seen = (int64_t)window + (1 << kShift) / group + 1 + 64;
+  const int64_t seen = (int64_t)window + (1 << shift) / group + 1 + 64;
   if (window && seen < span) span = seen;
   const int64_t all = (int64_t)parts->units * c.kv_heads * span;
-  const int64_t stretch = std::max<int64_t>(((all + kTarget - 1) / kTarget + 511) / 512 * 512, 512);
+  const int64_t stretch = std::max<int64_t>(((all + fit(waves) - 1) / fit(waves) + 511) / 512 * 512, 512);
   parts->stretch = (int)stretch;
   parts->splits = span > stretch ? (int)((span + stretch - 1) / stretch) : 1;
 }
 
-template <int D>
-hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, bool half, bool eight, const Parts& parts, hipStream_t stream) {
+template <int D, int W>
+hipError_t launch_waves(const KvCache& c, const KvBatch& b, const KvAttend& a, bool half, bool eight, const Parts& parts, hipStream_t stream) {
   const uint32_t grid = (uint32_t)parts.units * c.kv_heads * parts.splits;
   const bool wide = c.page_shift >= 4;
-  if (half && eight) attend_many<D, true, true, true><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-  else if (eight) attend_many<D, false, true, true><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-  else if (half && wide) attend_many<D, true, false, true><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-  else if (half) attend_many<D, true, false, false><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-  else if (wide) attend_many<D, false, false, true><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-  else attend_many<D, false, false, false><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  constexpr int kThreads = W * kWave;
+  if (eight) {
+    if constexpr (D > 64 || W == 4) {
+      if (half) attend_many<D, true, true, true, W><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+      else attend_many<D, false, true, true, W><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+    }
+  } else if (half && wide) attend_many<D, true, false, true, W><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  else if (half) attend_many<D, true, false, false, W><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  else if (wide) attend_many<D, false, false, true, W><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  else attend_many<D, false, false, false, W><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || parts.splits == 1) return e;
-  return launch_join(c, b, a, parts, kShift, half || eight ? 8.0f : 0.0f, D, half, stream);
+  return launch_join(c, b, a, parts, W == 8 ? 8 : 7, half || eight ? 8.0f : 0.0f, D, half, stream);
+}
+
+template <int D>
+hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, bool half, bool eight, const Parts& parts, int waves, hipStream_t stream) {
+  if constexpr (D < 256)
+    if (waves == 8) return launch_waves<D, 8>(c, b, a, half, eight, parts, stream);
+  return launch_waves<D, 4>(c, b, a, half, eight, parts, stream);
 }
 
 }  // namespace
 
 uint64_t kv_attend_many_workspace(const KvCache& c, const KvBatch& b, int q_heads, int head_dim) {
   // for any window: plan() has at most that many splits
-  const int64_t units = (int64_t)units_of(b, q_heads / c.kv_heads, kShift) * c.kv_heads;
+  const int group = q_heads / c.kv_heads, waves = waves_of(c, b, group, head_dim), shift = waves == 8 ? 8 : 7;
+  const int64_t units = (int64_t)units_of(b, group, shift) * c.kv_heads;
   if (!units) return 0;
-  const int64_t splits = std::min<int64_t>((b.max_context + 511) / 512, (kTarget + units - 1) / units);
-  return splits < 2 ? 0 : (uint64_t)((units * splits) << kShift) * (head_dim + 2) * 4;
+  const int64_t splits = std::min<int64_t>((b.max_context + 511) / 512, (fit(waves) + units - 1) / units);
+  return splits < 2 ? 0 : (uint64_t)((units * splits) << shift) * (head_dim + 2) * 4;
 }
 
 hipError_t launch_kv_attend_many(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream) {
+  const int group = a.q_heads / c.kv_heads, waves = waves_of(c, b, group, head_dim);
   Parts parts;
-  plan(c, b, a.q_heads / c.kv_heads, a.window, &parts);
+  plan(c, b, group, waves, a.window, &parts);
   parts.sums = (float*)a.workspace;
-  parts.stats = parts.sums + (((int64_t)parts.units * c.kv_heads * parts.splits) << kShift) * head_dim;
-  if (head_dim == 64) return launch<64>(c, b, a, half, eight, parts, stream);
-  if (head_dim == 128) return launch<128>(c, b, a, half, eight, parts, stream);
-  return launch<256>(c, b, a, half, eight, parts, stream);
+  parts.stats = parts.sums + (((int64_t)parts.units * c.kv_heads * parts.splits) << (waves == 8 ? 8 : 7)) * head_dim;
+  if (head_dim == 64) return launch<64>(c, b, a, half, eight, parts, waves, stream);
+  if (head_dim == 128) return launch<128>(c, b, a, half, eight, parts, waves, stream);
+  return launch<256>(c, b, a, half, eight, parts, waves, stream);
 }
 
 }  // namespace amem

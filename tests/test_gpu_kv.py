@@ -398,6 +398,25 @@ def test_attention_strides(arena, eight):
     check_attend(case, case.rows(6))
 
 
+@pytest.mark.parametrize("kind,eight,dim", [("bf16", False, 128), ("f16", False, 64), ("bf16", True, 128), ("f16", True, 128), ("f16", True, 64)])
+def test_attention_many_sequences(arena, kind, eight, dim):
+    """Enough prompts to fill the chip with the largest workgroups; a long one among them, and ones with bad values and hidden NaN."""
+    lengths = [(40, 40 + i % 50) for i in range(70)]
+    lengths[3], lengths[9], lengths[50] = (300, 700), (0, 0), (65, 64)
+    case = Case(arena, lengths, dim=dim, q_heads=8, kv_heads=8, kind=kind, eight=eight, page=16, block=16, seed=25)
+    nan = 0x7F if eight else 0x7FC0 if kind == "bf16" else 0x7E00
+    poison(case, 3, 500, k=nan)
+    poison(case, 3, 650, v=nan)
+    poison(case, 3, 699, v=nan)
+    case.table[20, 1] = -1
+    case.upload()
+    got, lse = check_attend(case, case.rows(8), sequences=[0, 3, 9, 19, 50, 69])
+    rows = O.decode(got, kind)[case.cu[20]:case.cu[21]]
+    n, c = lengths[20]
+    first = max(0, 16 - (c - n))
+    assert np.isnan(rows[first:]).all() and np.isfinite(rows[:first]).all()
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 8.0])
 def test_attention_scales(arena, scale):
     """From weights that are all equal to a single one."""
