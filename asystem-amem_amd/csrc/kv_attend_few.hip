@@ -428,18 +428,17 @@ int blocks_of(int group, int max_tokens, int head_dim) {
   return rows <= 16 ? 1 : rows <= 32 || head_dim > 64 ? 2 : 4;
 }
 
-// Stretches are as long as leaves about kTarget workgroups, and at least kLeast positions.
-void plan(const KvCache& c, const KvBatch& b, int group, int blocks, int window, Parts* few) {
+// Stretches of the same length, as long as leaves about kTarget workgroups, and at least kLeast positions.
+void plan(const KvCache& c, const KvBatch& b, int group, int blocks, const KvAttend& a, Parts* few) {
   const int shift = blocks == 1 ? 4 : blocks == 2 ? 5 : 6;
   int64_t span = b.max_context;
-  const int64_t seen = (int64_t)window + (16 * blocks) / group + 1 + 64;
-  if (window && seen < span) span = seen;
+  const int64_t seen = (int64_t)a.window + (16 * blocks) / group + 1 + 64;
+  if (a.causal && a.window && seen < span) span = seen;  // else a window has no far end
   few->units = units_of(b, group, shift);
   const int64_t all = (int64_t)few->units * c.kv_heads * span;
-  const int64_t step = kWaves * 64;
-  const int64_t stretch = std::max<int64_t>(((all + kTarget - 1) / kTarget + step - 1) / step * step, kLeast);
-  few->stretch = (int)stretch;
+  const int64_t step = kWaves * 64, stretch = std::max<int64_t>((all + kTarget - 1) / kTarget, kLeast);
   few->splits = span > stretch ? (int)((span + stretch - 1) / stretch) : 1;
+  few->stretch = (int)(((span + few->splits - 1) / few->splits + step - 1) / step * step);
 }
 
 template <int D, bool HALF, bool EIGHT, int NB>
@@ -485,7 +484,7 @@ uint64_t kv_attend_few_workspace(const KvCache& c, const KvBatch& b, int q_heads
 hipError_t launch_kv_attend_few(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream) {
   const int group = a.q_heads / c.kv_heads, blocks = blocks_of(group, a.max_tokens, head_dim);
   Parts few;
-  plan(c, b, group, blocks, a.window, &few);
+  plan(c, b, group, blocks, a, &few);
   few.sums = (float*)a.workspace;
   few.stats = few.sums + (int64_t)few.units * c.kv_heads * few.splits * (16 * blocks) * head_dim;
   if (head_dim == 64) return launch_dims<64>(c, b, a, half, eight, few, blocks, stream);

@@ -2,13 +2,14 @@
 //
 //   s_p = scale q.k_p,  m = max s_p,  l = sum exp(s_p - m),  out = sum exp(s_p - m) v_p / l,  lse = m + log l
 //
-// Bound by the matrix unit. A workgroup takes 256 rows that share a key/value head (32 for each of its eight waves; or 128 and
-// four) through the positions they see, 64 at a time: its threads load a tile of keys and values while the one before
-// is worked on, and put it into LDS as 16-bit numbers, where every wave reads all of it. Two tiles are held there, so
-// that one barrier a tile is enough. Products are (keys x dims)(dims x rows) and (dims x keys)(keys x rows): a lane holds scores and sums
+// Bound by the matrix unit. A workgroup takes 256 rows that share a key/value head (32 for each of its eight waves; or 128: four
+// waves, or eight with 16 rows each) through the positions they see, 64 at a time: its threads load a tile of keys
+// and values while the one before is worked on, and put it into LDS as 16-bit numbers, where every wave reads all of it.
+// Two tiles are held there, so that one barrier a tile is enough. Products are (keys x dims)(dims x rows) and (dims x keys)(keys x rows): a lane holds scores and sums
 // of one row, the weights go from the first product's result to the second's operand without leaving their lane, and
 // values are read from LDS as columns.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_parts.h"
 
@@ -35,25 +36,29 @@ __device__ __forceinline__ u32x4 widen_scaled(u32x2 x, float scale) {
 }
 
 // D dims, 16 bits of fp16 (HALF) or bf16, a cache of e4m3 (EIGHT), pages of at least 16 slots (WIDE).
-template <int D, bool HALF, bool EIGHT, bool WIDE, int kWaves>
-__global__ __launch_bounds__(kWaves * kWave, (D == 256 ? 1 : 2)) void attend_many(KvCache c, KvBatch b, KvAttend a, Parts parts) {
-  constexpr int kThreads = kWaves * kWave;
-  constexpr int kShift = kWaves == 8 ? 8 : 7;     // log2 of a unit's rows
+// W waves with R rows each, 32 or 16.
+template <int D, bool HALF, bool EIGHT, bool WIDE, int W, int R>
+__global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b, KvAttend a, Parts parts) {
+  constexpr int kThreads = W * kWave;
+  constexpr int kShift = W * R == 256 ? 8 : 7;    // log2 of a unit's rows
   constexpr int kElement = EIGHT ? 1 : 2;
   constexpr int kRowLanes = D * kElement / 16;    // threads that load a position's key, or value
   constexpr int kRowsAPass = kThreads / kRowLanes;
   constexpr int kPasses = kTile / kRowsAPass;
   static_assert(kRowsAPass <= kTile, "a pass is at most a tile");
   // pads: the rows that are read together are on different banks
-  constexpr int kKeyPitch = D * 2 + 16, kValuePitch = D * 2 + 64, kBuffer = kTile * (kKeyPitch + kValuePitch);
+  constexpr int kKeyPitch = D * 2 + 16, kValuePitch = D * 2 + 2 * R, kBuffer = kTile * (kKeyPitch + kValuePitch);
   constexpr bool kHalfP = EIGHT || HALF;  // weights are fp16 where the values' type allows it
   // fp16 weights are held 2^8 times larger, which keeps small ones out of the subnormal numbers
   constexpr float kLift = kHalfP ? 8.0f : 0.0f;
   // Scales of keys go into the keys where 16 bits hold every product (bf16), else into the scores.
   constexpr bool kFold = EIGHT && !HALF;
-  constexpr int kDims = D / 32;
+  // What a lane holds of its row: scores of kScores positions of a tile, and sums of kSums dims in kBlocks results of the matrix unit.
+  constexpr int kScores = R == 32 ? 32 : 16, kBlocks = D / R, kSums = R == 32 ? 16 : 4;
+  using Result = std::conditional_t<R == 32, f32x16, f32x4>;
+  constexpr int kSteps = R == 32 ? 16 : 32;       // depth of a matrix instruction
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kBuffer];
-  __shared__ uint64_t lds_odd[2][kPasses * kWaves];
+  __shared__ uint64_t lds_odd[2][kPasses * W];
 
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   // heads first, so that the units of a head, which read the same keys, run on one die where heads are a multiple of eight;
@@ -66,14 +71,16 @@ __global__ __launch_bounds__(kWaves * kWave, (D == 256 ? 1 : 2)) void attend_man
   const int begin = u.from + split * parts.stretch;
   if (split && (begin >= u.to || q.bad)) return;
   const int end = begin + parts.stretch < u.to ? begin + parts.stretch : u.to;
-  const int col = lane & 31, half = lane >> 5;
+  const int col = lane & (R - 1), part = lane / R;
+  auto position_of = [&](int j) { return R == 32 ? j / 4 * 8 + part * 4 + j % 4 : j / 4 * 16 + part * 4 + j % 4; };
+  auto dim_of = [&](int i, int e) { return R == 32 ? i * 32 + e / 4 * 8 + part * 4 + e % 4 : i * 16 + part * 4 + e; };
 
   // this wave's rows, and the positions that some, and all, of them see
-  const int wave_first = u.first + wave * 32;
-  const bool active = wave * 32 < u.rows;
-  const int wave_last = std::min(wave_first + 31, u.first + u.rows - 1);
+  const int wave_first = u.first + wave * R;
+  const bool active = wave * R < u.rows;
+  const int wave_last = std::min(wave_first + R - 1, u.first + u.rows - 1);
   int wave_lo = 0, wave_to = 0, all_from = 0, all_to = 0, row_from = 0, row_to = 0, token = 0, head = 0;
-  u32x4 qr[D / 16];
+  u32x4 qr[D / kSteps];
   if (active) {
     row_range(a, q, wave_first / group, wave_lo, all_to);
     row_range(a, q, wave_last / group, all_from, wave_to);
@@ -83,18 +90,18 @@ __global__ __launch_bounds__(kWaves * kWave, (D == 256 ? 1 : 2)) void attend_man
     row_range(a, q, token, row_from, row_to);
     const uint16_t* p = a.q + (q.row + token) * a.q_token + head * a.q_head;
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) qr[t] = *(const u32x4*)(p + t * 16 + half * 8) ^ (a.scale < 0 ? 0x80008000u : 0u);
+    for (int t = 0; t < D / kSteps; ++t) qr[t] = *(const u32x4*)(p + t * kSteps + part * 8) ^ (a.scale < 0 ? 0x80008000u : 0u);
   }
   // weights are exp2(score * factor - top), so the factor has to be above zero for the largest score to give the largest
   // product: its sign is in the queries, and a scale of zero becomes one that is as good as zero
   const float factor = fmaxf(fabsf(a.scale) * kLog2e, 0x1p-100f);
 
   float m = -kInf, l = 0;
-  f32x16 sum[kDims];
+  Result sum[kBlocks];
 #pragma unroll
-  for (int i = 0; i < kDims; ++i)
+  for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) sum[i][j] = 0;
+    for (int j = 0; j < kSums; ++j) sum[i][j] = 0;
   float unit_scale = 0;  // the sums are in multiples of it (8 bits)
 
   // ---- loading: a thread's rows of a tile
@@ -186,7 +193,7 @@ __global__ __launch_bounds__(kWaves * kWave, (D == 256 ? 1 : 2)) void attend_man
         // only some rows see are taken out of the product and added one by one
         if (base + r < u.lo || base + r >= u.to) v = u32x4{0, 0, 0, 0};
         const uint64_t lanes = __ballot(not_finite<HALF, EIGHT>(v));
-        if (lane == 0) lds_odd[buffer][i * kWaves + wave] = lanes;
+        if (lane == 0) lds_odd[buffer][i * W + wave] = lanes;
         if (lanes >> (lane / kRowLanes * kRowLanes) & ((1ull << kRowLanes) - 1)) v = u32x4{0, 0, 0, 0};
       }
       if constexpr (EIGHT) {
@@ -219,7 +226,7 @@ __global__ __launch_bounds__(kWaves * kWave, (D == 256 ? 1 : 2)) void attend_man
     __syncthreads();
     const bool work = active && base < wave_to && base + kTile > wave_lo;
     const uint8_t* const tile = lds + buffer * kBuffer;
-    f32x16 score[2];
+    float score[kScores];
     float f[4];
     if constexpr (EIGHT && !kFold) {
 #pragma unroll
@@ -227,15 +234,21 @@ __global__ __launch_bounds__(kWaves * kWave, (D == 256 ? 1 : 2)) void attend_man
     }
     const float tile_scale = stored_scale;
     if (work) {
+      Result s[kTile / R];
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
+      for (int g = 0; g < kTile / R; ++g)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) score[g][j] = 0;
+        for (int j = 0; j < kSums; ++j) s[g][j] = 0;
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t)
+      for (int t = 0; t < D / kSteps; ++t)
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
-          score[g] = mfma32<HALF>(*(const u32x4*)(tile + (g * 32 + col) * kKeyPitch + t * 32 + half * 16), qr[t], score[g]);
+        for (int g = 0; g < kTile / R; ++g) {
+          const u32x4 k = *(const u32x4*)(tile + (g * R + col) * kKeyPitch + t * kSteps * 2 + part * 16);
+          if constexpr (R == 32) s[g] = mfma32<HALF>(k, qr[t], s[g]);
+          else s[g] = mfma16<HALF>(k, qr[t], s[g]);
+        }
+#pragma unroll
+      for (int j = 0; j < kScores; ++j) score[j] = s[j / kSums][j % kSums];
     }
     if (base + kTile < end) {
       store(base + kTile, buffer ^ 1);
@@ -246,94 +259,88 @@ __global__ __launch_bounds__(kWaves * kWave, (D == 256 ? 1 : 2)) void attend_man
 
     if constexpr (EIGHT && !kFold) {
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) score[g][j] *= f[2 * g + j / 8];
+      for (int j = 0; j < kScores; ++j) score[j] *= f[R == 32 ? j / 8 : j / 4];
     }
     const bool edge = base < all_from || base + kTile > all_to;
     if (edge) {
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int p = base + g * 32 + j / 4 * 8 + half * 4 + j % 4;
-          if (p < row_from || p >= row_to) score[g][j] = -kInf;
-        }
+      for (int j = 0; j < kScores; ++j) {
+        const int p = base + position_of(j);
+        if (p < row_from || p >= row_to) score[j] = -kInf;
+      }
     }
-    float top = score[0][0];
+    float top = score[0];
 #pragma unroll
-    for (int g = 0; g < 2; ++g)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) top = __builtin_elementwise_maximum(top, score[g][j]);  // NaN stays
+    for (int j = 0; j < kScores; ++j) top = __builtin_elementwise_maximum(top, score[j]);  // NaN stays
+    if constexpr (R == 16) top = __builtin_elementwise_maximum(top, __shfl_xor(top, 16, kWave));
     top = __builtin_elementwise_maximum(top, __shfl_xor(top, 32, kWave));
     const float now = __builtin_elementwise_maximum(m, top * factor);
     if (__any(now != m)) {
       const float shrink = now == m ? 1.0f : __builtin_amdgcn_exp2f(m - now);
       l *= shrink;
 #pragma unroll
-      for (int i = 0; i < kDims; ++i)
+      for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) sum[i][j] *= shrink;
+        for (int j = 0; j < kSums; ++j) sum[i][j] *= shrink;
       m = now;
     }
     if (EIGHT && !(tile_scale <= unit_scale)) {
       const float x = unit_scale / tile_scale;
 #pragma unroll
-      for (int i = 0; i < kDims; ++i)
+      for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) sum[i][j] *= x;
+        for (int j = 0; j < kSums; ++j) sum[i][j] *= x;
       unit_scale = tile_scale;
     }
     const float sub = (m == -kInf ? 0.0f : m) - kLift;
-    u32x4 w[4];
+    // weights as operands: the eight of a step are the positions of eight scores in a row
+    u32x4 w[kTile / kSteps];
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        score[g][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[g][j], factor, -sub));
-        l += score[g][j];
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[2 * g + j / 4][j % 4] = pack<kHalfP>(score[g][2 * j], score[g][2 * j + 1]);
+    for (int j = 0; j < kScores; ++j) {
+      score[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j], factor, -sub));
+      l += score[j];
     }
-    // lane m of 16 gives the address of position m / 4 of four, dims 4 (m % 4) on, of the block of 16 dims that these lanes take
-    const uint8_t* const columns = tile + kTile * kKeyPitch + (4 * half + (lane & 15) / 4) * kValuePitch + ((lane >> 4 & 1) * 16 + (lane & 3) * 4) * 2;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int j = 0; j < kScores / 2; ++j) w[j / 4][j % 4] = pack<kHalfP>(score[2 * j], score[2 * j + 1]);
+    // lane m of 16 gives the address of position m / 4 of four, dims 4 (m % 4) on, of the 16 dims that these lanes take
+    const uint8_t* const columns = tile + kTile * kKeyPitch + (4 * part + (lane & 15) / 4) * kValuePitch + ((R == 32 ? (lane >> 4 & 1) * 16 : 0) + (lane & 3) * 4) * 2;
 #pragma unroll
-      for (int i = 0; i < kDims; ++i) {
-        const uint8_t* p = columns + t * 16 * kValuePitch + i * 64;
-        const u32x2 lo = read_columns16(p), hi = read_columns16(p + 8 * kValuePitch);
-        sum[i] = mfma32<kHalfP>(u32x4{lo[0], lo[1], hi[0], hi[1]}, w[t], sum[i]);
+    for (int t = 0; t < kTile / kSteps; ++t)
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) {
+        const uint8_t* p = columns + t * kSteps * kValuePitch + i * R * 2;
+        const u32x2 lo = read_columns16(p), hi = read_columns16(p + kSteps / 2 * kValuePitch);
+        const u32x4 v = u32x4{lo[0], lo[1], hi[0], hi[1]};
+        if constexpr (R == 32) sum[i] = mfma32<kHalfP>(v, w[t], sum[i]);
+        else sum[i] = mfma16<kHalfP>(v, w[t], sum[i]);
       }
     if (edge) {
 #pragma unroll 1
-      for (int n = 0; n < kPasses * kWaves; ++n) {
-        const uint64_t lanes = lds_odd[buffer][n];
+      for (int o = 0; o < kPasses * W; ++o) {
+        const uint64_t lanes = lds_odd[buffer][o];
         if (!lanes) continue;
 #pragma unroll 1
-        for (int j = 0; j < kWave / kRowLanes; ++j) {
-          if (!(lanes >> (j * kRowLanes) & ((1ull << kRowLanes) - 1))) continue;
-          const int k = n / kWaves * kRowsAPass + n % kWaves * (kWave / kRowLanes) + j, p = base + k;
+        for (int n = 0; n < kWave / kRowLanes; ++n) {
+          if (!(lanes >> (n * kRowLanes) & ((1ull << kRowLanes) - 1))) continue;
+          const int k = o / W * kRowsAPass + o % W * (kWave / kRowLanes) + n, p = base + k;
           const int where = kv_page(c, b, u.s, p);  // seen by some row, so below u.to
           if (where < 0) continue;                  // its key is NaN already
           const uint8_t* v = c.v + kv_offset(c, where, kvh, p);
+          // the weight of k, from the lane that has it
+          const int index = R == 32 ? k / 8 * 4 + k % 4 : k / 16 * 4 + k % 4;
           float x = 0;
 #pragma unroll
-          for (int g = 0; g < 2; ++g)
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (k >> 5 == g && (k & 31) / 8 * 4 + k % 4 == e) x = score[g][e];
-          x = __shfl(x, (k >> 2 & 1) * 32 + col, kWave);
+          for (int j = 0; j < kScores; ++j)
+            if (j == index) x = score[j];
+          x = __shfl(x, (R == 32 ? k / 4 % 2 : k / 4 % 4) * R + col, kWave);
           if (p < row_from || p >= row_to) continue;
           if constexpr (EIGHT) x *= c.v_scale[kv_scale_offset(c, where, kvh, p)] * (unit_scale > 0 ? 1.0f / unit_scale : 0.0f);
 #pragma unroll
-          for (int i = 0; i < kDims; ++i)
+          for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int d = i * 32 + e / 4 * 8 + half * 4 + e % 4;
-              if constexpr (EIGHT) sum[i][e] += x * __builtin_amdgcn_cvt_f32_fp8((int)v[d], 0);
-              else sum[i][e] += x * to_float<HALF>(((const uint16_t*)v)[d]);
+            for (int e = 0; e < kSums; ++e) {
+              if constexpr (EIGHT) sum[i][e] += x * __builtin_amdgcn_cvt_f32_fp8((int)v[dim_of(i, e)], 0);
+              else sum[i][e] += x * to_float<HALF>(((const uint16_t*)v)[dim_of(i, e)]);
             }
         }
       }
@@ -341,19 +348,19 @@ __global__ __launch_bounds__(kWaves * kWave, (D == 256 ? 1 : 2)) void attend_man
   }
   if (!active) return;
 
+  if constexpr (R == 16) l += __shfl_xor(l, 16, kWave);
   l += __shfl_xor(l, 32, kWave);
   const float back = EIGHT && unit_scale > 0 ? unit_scale : 1.0f;
-  const int r = wave * 32 + col;
+  const int r = wave * R + col;
   if (r >= u.rows) return;
   if (parts.splits > 1) {
     const int64_t row = (part_of(c, parts, unit, kvh, split) << kShift) + r;
 #pragma unroll
-    for (int i = 0; i < kDims; ++i)
+    for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *(f32x4*)(parts.sums + row * D + i * 32 + j * 8 + half * 4) =
-            f32x4{sum[i][4 * j], sum[i][4 * j + 1], sum[i][4 * j + 2], sum[i][4 * j + 3]} * back;
-    if (half == 0) {
+      for (int e = 0; e < kSums; e += 4)
+        *(f32x4*)(parts.sums + row * D + dim_of(i, e)) = f32x4{sum[i][e], sum[i][e + 1], sum[i][e + 2], sum[i][e + 3]} * back;
+    if (part == 0) {
       parts.stats[row * 2] = m;
       parts.stats[row * 2 + 1] = l;
     }
@@ -362,86 +369,96 @@ __global__ __launch_bounds__(kWaves * kWave, (D == 256 ? 1 : 2)) void attend_man
   const float inverse = q.bad ? __builtin_nanf("") : l == 0 ? 0.0f : back / l;
   uint16_t* const out = a.out + (q.row + token) * a.out_token + head * a.out_head;
 #pragma unroll
-  for (int i = 0; i < kDims; ++i)
+  for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f32x4 x = f32x4{sum[i][4 * j], sum[i][4 * j + 1], sum[i][4 * j + 2], sum[i][4 * j + 3]} * inverse;
-      *(u32x2*)(out + i * 32 + j * 8 + half * 4) = u32x2{pack<HALF>(x[0], x[1]), pack<HALF>(x[2], x[3])};
+    for (int e = 0; e < kSums; e += 4) {
+      const f32x4 x = f32x4{sum[i][e], sum[i][e + 1], sum[i][e + 2], sum[i][e + 3]} * inverse;
+      *(u32x2*)(out + dim_of(i, e)) = u32x2{pack<HALF>(x[0], x[1]), pack<HALF>(x[2], x[3])};
     }
-  if (a.lse && half == 0)
+  if (a.lse && part == 0)
     a.lse[(int64_t)(q.row + token) * a.q_heads + head] = q.bad ? __builtin_nanf("") : l == 0 ? -kInf : ((m - kLift) + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// Contexts are cut only where units are fewer than fit at once (one workgroup of eight waves a compute unit, or two of four),
-// and never below 512 positions: a part costs its rows' sums written and read once more.
-constexpr int fit(int waves) { return waves == 8 ? 256 : 512; }
-
-// Eight waves of 32 rows share the loads of a tile, four need them twice as often: a chunk of 4096 over 16384 positions in
-// e4m3 takes 1.035 ms with eight and 1.090 with four. Four where there would be less than two workgroups of eight for each
-// compute unit (2048 x 2048 positions, 32 heads over 8: 69 us, and 78 with eight), for 256 dims, whose registers
-// allow one wave a SIMD, and for 64 of e4m3, where four load a tile at once.
-int waves_of(const KvCache& c, const KvBatch& b, int group, int head_dim) {
-  if (head_dim == 256 || (head_dim == 64 && c.block_shift)) return 4;
-  return (int64_t)units_of(b, group, 8) * c.kv_heads >= 2 * fit(8) ? 8 : 4;
+// Rows of a unit, and how a workgroup is made of waves. A tile's loads are shared by all of them: a chunk of 4096 over 16384
+// positions in e4m3 takes 1.035 ms with eight waves of 32 rows and 1.090 with four. Four where there would be less than two
+// workgroups of eight for each compute unit (2048 x 2048 positions, 32 heads over 8: 69 us, and 78 with eight), and for 64
+// dims of e4m3, where four load a tile at once. 256 dims leave a wave of 32 rows a SIMD for itself; eight of 16 rows, two a
+// SIMD, read LDS twice as often and are faster all the same: VMEASURE.
+struct Shape {
+  int shift, fit;  // log2 of the rows; workgroups that fit at once
+  bool eight;      // eight waves
+};
+Shape shape_of(const KvCache& c, const KvBatch& b, int group, int head_dim) {
+  if (head_dim == 256) return {7, 256, true};
+  if (head_dim == 64 && c.block_shift) return {7, 512, false};
+  if ((int64_t)units_of(b, group, 8) * c.kv_heads >= 512) return {8, 256, true};
+  return {7, 512, false};
 }
 
-void plan(const KvCache& c, const KvBatch& b, int group, int waves, int window, Parts* parts) {
-  const int shift = waves == 8 ? 8 : 7;
-  parts->units = units_of(b, group, shift);
+constexpr int kLeast = 512;  // positions of a workgroup, at least: a part costs its rows' sums written and read once more
+
+// Contexts are cut only where units are fewer than fit at once, into stretches of the same length.
+void plan(const KvCache& c, const KvBatch& b, int group, const Shape& shape, const KvAttend& a, Parts* parts) {
+  parts->units = units_of(b, group, shape.shift);
   int64_t span = b.max_context;
-  const int64_t seen = (int64_t)window + (1 << shift) / group + 1 + 64;
-  if (window && seen < span) span = seen;
+  const int64_t seen = (int64_t)a.window + (1 << shape.shift) / group + 1 + 64;
+  if (a.causal && a.window && seen < span) span = seen;  // else a window has no far end
   const int64_t all = (int64_t)parts->units * c.kv_heads * span;
-  const int64_t stretch = std::max<int64_t>(((all + fit(waves) - 1) / fit(waves) + 511) / 512 * 512, 512);
-  parts->stretch = (int)stretch;
+  const int64_t stretch = std::max<int64_t>((all + shape.fit - 1) / shape.fit, kLeast);
   parts->splits = span > stretch ? (int)((span + stretch - 1) / stretch) : 1;
+  parts->stretch = (int)(((span + parts->splits - 1) / parts->splits + kTile - 1) / kTile * kTile);
 }
 
-template <int D, int W>
+template <int D, int W, int R>
 hipError_t launch_waves(const KvCache& c, const KvBatch& b, const KvAttend& a, bool half, bool eight, const Parts& parts, hipStream_t stream) {
   const uint32_t grid = (uint32_t)parts.units * c.kv_heads * parts.splits;
   const bool wide = c.page_shift >= 4;
   constexpr int kThreads = W * kWave;
   if (eight) {
     if constexpr (D > 64 || W == 4) {
-      if (half) attend_many<D, true, true, true, W><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-      else attend_many<D, false, true, true, W><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+      if (half) attend_many<D, true, true, true, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+      else attend_many<D, false, true, true, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
     }
-  } else if (half && wide) attend_many<D, true, false, true, W><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-  else if (half) attend_many<D, true, false, false, W><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-  else if (wide) attend_many<D, false, false, true, W><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-  else attend_many<D, false, false, false, W><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  } else if (half && wide) attend_many<D, true, false, true, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  else if (half) attend_many<D, true, false, false, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  else if (wide) attend_many<D, false, false, true, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  else attend_many<D, false, false, false, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || parts.splits == 1) return e;
-  return launch_join(c, b, a, parts, W == 8 ? 8 : 7, half || eight ? 8.0f : 0.0f, D, half, stream);
+  return launch_join(c, b, a, parts, W * R == 256 ? 8 : 7, half || eight ? 8.0f : 0.0f, D, half, stream);
 }
 
 template <int D>
-hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, bool half, bool eight, const Parts& parts, int waves, hipStream_t stream) {
-  if constexpr (D < 256)
-    if (waves == 8) return launch_waves<D, 8>(c, b, a, half, eight, parts, stream);
-  return launch_waves<D, 4>(c, b, a, half, eight, parts, stream);
+hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, bool half, bool eight, const Parts& parts, const Shape& shape, hipStream_t stream) {
+  if constexpr (D == 256) {
+    return launch_waves<D, 8, 16>(c, b, a, half, eight, parts, stream);
+  } else {
+    if (shape.eight) return launch_waves<D, 8, 32>(c, b, a, half, eight, parts, stream);
+    return launch_waves<D, 4, 32>(c, b, a, half, eight, parts, stream);
+  }
 }
 
 }  // namespace
 
 uint64_t kv_attend_many_workspace(const KvCache& c, const KvBatch& b, int q_heads, int head_dim) {
   // for any window: plan() has at most that many splits
-  const int group = q_heads / c.kv_heads, waves = waves_of(c, b, group, head_dim), shift = waves == 8 ? 8 : 7;
-  const int64_t units = (int64_t)units_of(b, group, shift) * c.kv_heads;
+  const int group = q_heads / c.kv_heads;
+  const Shape shape = shape_of(c, b, group, head_dim);
+  const int64_t units = (int64_t)units_of(b, group, shape.shift) * c.kv_heads;
   if (!units) return 0;
-  const int64_t splits = std::min<int64_t>((b.max_context + 511) / 512, (fit(waves) + units - 1) / units);
-  return splits < 2 ? 0 : (uint64_t)((units * splits) << shift) * (head_dim + 2) * 4;
+  const int64_t splits = std::min<int64_t>((b.max_context + kLeast - 1) / kLeast, (shape.fit + units - 1) / units);
+  return splits < 2 ? 0 : (uint64_t)((units * splits) << shape.shift) * (head_dim + 2) * 4;
 }
 
 hipError_t launch_kv_attend_many(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream) {
-  const int group = a.q_heads / c.kv_heads, waves = waves_of(c, b, group, head_dim);
+  const int group = a.q_heads / c.kv_heads;
+  const Shape shape = shape_of(c, b, group, head_dim);
   Parts parts;
-  plan(c, b, group, waves, a.window, &parts);
+  plan(c, b, group, shape, a, &parts);
   parts.sums = (float*)a.workspace;
-  parts.stats = parts.sums + (((int64_t)parts.units * c.kv_heads * parts.splits) << (waves == 8 ? 8 : 7)) * head_dim;
-  if (head_dim == 64) return launch<64>(c, b, a, half, eight, parts, waves, stream);
-  if (head_dim == 128) return launch<128>(c, b, a, half, eight, parts, waves, stream);
-  return launch<256>(c, b, a, half, eight, parts, waves, stream);
+  parts.stats = parts.sums + (((int64_t)parts.units * c.kv_heads * parts.splits) << shape.shift) * head_dim;
+  if (head_dim == 64) return launch<64>(c, b, a, half, eight, parts, shape, stream);
+  if (head_dim == 128) return launch<128>(c, b, a, half, eight, parts, shape, stream);
+  return launch<256>(c, b, a, half, eight, parts, shape, stream);
 }
 
 }  // namespace amem

@@ -389,6 +389,16 @@ def test_attention_masks(arena, causal, window, kind, eight):
 
 
 @pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("causal,window", [(False, 0), (False, 20), (True, 20), (True, 700)])
+def test_attention_masks_of_long_contexts(arena, causal, window, eight):
+    """Contexts that are cut into stretches: a window bounds what a row sees only where the mask is causal."""
+    for lengths in ([(1, 1500), (4, 900)], [(80, 1500)]):
+        case = Case(arena, lengths, dim=64, q_heads=4, kv_heads=2, eight=eight, page=32, block=32, seed=26).upload()
+        check_attend(case, case.rows(4), causal, window)
+        arena.reset()
+
+
+@pytest.mark.parametrize("eight", [False, True])
 def test_attention_strides(arena, eight):
     for lengths in ([(1, 100), (1, 20)], [(50, 90), (2, 40)]):
         case = Case(arena, lengths, dim=128, q_heads=6, kv_heads=3, eight=eight, page=32, block=32, slot_major=True, seed=16, behind=3).upload()
