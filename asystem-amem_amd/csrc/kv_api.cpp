@@ -71,9 +71,10 @@ int check_cache(const char* what, const amem_kv_cache* c, bool addresses, KvCach
 
 int check_batch(const char* what, const amem_kv_batch* b, const KvCache& c, bool addresses, KvBatch* out) {
   NEED(b, "batch is NULL");
-  NEED(b->sequences >= 0 && b->sequences <= 1 << 20 && b->tokens >= 0 && b->tokens <= 1 << 24,
+  // launches stay below 2^32 threads
+  NEED(b->sequences >= 0 && b->sequences <= 1 << 20 && b->tokens >= 0 && b->tokens <= 1 << 22,
        "sequences or tokens out of range");
-  NEED((int64_t)(b->tokens / 16 + 2 * b->sequences) * c.kv_heads <= 1 << 28, "tokens or sequences times kv_heads out of range");
+  NEED((int64_t)(b->tokens / 16 + 2 * b->sequences) * c.kv_heads <= 1 << 22, "tokens or sequences times kv_heads out of range");
   NEED(b->max_tokens >= 0 && b->max_tokens <= b->tokens, "max_tokens is not between 0 and tokens");
   NEED(b->table_pages >= 0 && b->table_stride >= b->table_pages, "table_pages or table_stride");
   NEED(b->max_context >= 0 && b->max_context < 1 << 30 &&
@@ -125,6 +126,7 @@ int on_device(const char* what, int device, hipStream_t stream, Launch launch) {
   }
   if (device != current)
     if (hipError_t e = CHECK_HIP(hipSetDevice(device)); e != hipSuccess) return (int)e;
+  (void)hipGetLastError();  // what an earlier call of the caller's left behind is no error of this one
   const hipError_t e = CHECK_HIP(launch());
   if (device != current) (void)CHECK_HIP(hipSetDevice(current));
   return (int)e;
@@ -195,7 +197,7 @@ int amem_kv_attention_workspace(const amem_kv_cache* cache, const amem_kv_batch*
   if (int e = check_cache(what, cache, false, &c)) return e;
   if (int e = check_batch(what, batch, c, false, &b)) return e;
   NEED(q_heads >= 1 && q_heads <= 1024 && q_heads % c.kv_heads == 0, "q_heads is not a multiple of kv_heads");
-  NEED((int64_t)b.tokens * q_heads < 1 << 30, "tokens * q_heads is 2^30 or more");
+  NEED((int64_t)b.tokens * q_heads <= 1 << 27, "tokens * q_heads is above 2^27");
   NEED(bytes, "bytes is NULL");
   *bytes = kv_attend_workspace(c, b, q_heads, batch->max_tokens, cache->head_dim);
   return 0;
@@ -216,7 +218,7 @@ int amem_kv_attention(const amem_kv_cache* cache, const amem_kv_batch* batch, co
     if (int e = check_rows(what, "address or strides of q", a->q, a->q_token_stride, a->q_head_stride, b.tokens, a->q_heads)) return e;
     if (int e = check_rows(what, "address or strides of out", a->out, a->out_token_stride, a->out_head_stride, b.tokens, a->q_heads)) return e;
   }
-  NEED((int64_t)b.tokens * a->q_heads < 1 << 30, "tokens * q_heads is 2^30 or more");
+  NEED((int64_t)b.tokens * a->q_heads <= 1 << 27, "tokens * q_heads is above 2^27");
   NEED(a->lse % 4 == 0, "address of lse");
   NEED(a->window >= 0, "window is negative");
   NEED(a->scale - a->scale == 0, "scale is not finite");

@@ -84,7 +84,7 @@ AMEM_HD int64_t kv_scale_offset(const KvCache& c, int page, int head, int p) {
 // Work is handed out in units of items (tile = 1 << shift of them, `per_row` items a row) without the host knowing the
 // lengths: unit u belongs to the last sequence s with kv_unit_base(s) <= u. `spare` units more for each sequence
 // cover what its first and last, partial tiles need (1 for tiles that start at its first item, 2 for tiles of its cache
-// positions), so a call has at most kv_units() of them and some are empty. The host holds tokens * per_row below 2^30.
+// positions), so a call has at most kv_units() of them and some are empty. The host holds tokens * per_row to 2^27.
 AMEM_HD int kv_unit_base(const KvBatch& b, int s, int shift, int spare, int per_row = 1) {
   return (kv_cu(b, s) * per_row >> shift) + s * spare;
 }

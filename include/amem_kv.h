@@ -12,7 +12,7 @@
  *
  * Conventions. Device addresses are uint64_t. Every call only enqueues work on `stream` (a
  * hipStream_t of the cache's device, NULL for its default stream) and may be captured; nothing is
- * allocated, copied to the host or kept. Everything that addresses name has to lie on the cache's
+ * allocated, copied to the host or kept, so that tensors have to live until the stream is done with them. Everything that addresses name has to lie on the cache's
  * device, which need not be the current one. Results are the same, bit for bit, from call to call. Returns
  * 0, hipErrorInvalidValue (1) for arguments that are refused (one ERROR line says which) and while
  * paused, or another HIP error. Two calls that may run at the same time need different workspaces,
@@ -37,7 +37,7 @@ enum amem_kv_type { AMEM_KV_BF16 = 0, AMEM_KV_F16 = 1, AMEM_KV_E4M3 = 2 };
 #define AMEM_KV_MAX_AXES 4
 
 /* Keys and values: element [page][head][slot][dim], dims contiguous, the other strides as given (in
- * elements, multiples of 16 bytes; the same for both). 8 bits: values are code * scale, codes e4m3
+ * elements, multiples of 16 bytes; the same for both; the slots of a page less than 2^31 bytes apart). 8 bits: values are code * scale, codes e4m3
  * (largest 448, no infinities), one float32 scale, a power of two from 2^-64 to 2^119, for each
  * [page][head][block of `block_slots` slots], blocks contiguous. */
 typedef struct amem_kv_cache {
@@ -54,7 +54,8 @@ typedef struct amem_kv_cache {
   int32_t reserved;              /* 0 */
 } amem_kv_cache;
 
-/* Sequences of a call. Sequence s has rows [cu_tokens[s], cu_tokens[s+1]) of the token tensors (its
+/* Sequences of a call, at most 2^20 and 2^22 tokens; tokens * q_heads is at most 2^27, and
+ * (tokens / 16 + 2 * sequences) * kv_heads 2^22. Sequence s has rows [cu_tokens[s], cu_tokens[s+1]) of the token tensors (its
  * new tokens, possibly none) and context[s] tokens in the cache, those included: its row j is at
  * position context[s] - n + j, in slot position % page_slots of page page_table[s][position / page_slots].
  * Rows behind the last sequence's are left alone. A sequence whose context is negative, above
@@ -111,7 +112,8 @@ int amem_kv_append(const amem_kv_cache* cache, const amem_kv_batch* batch, const
  * key/value head head / (q_heads / kv_heads). Row at position i of a sequence with context L sees p < L, p <= i
  * if causal, and p > i - window if window > 0. lse, where given, is the natural logarithm of the sum of
  * exp(scale q.k_p). A row that sees nothing, or nothing but scores of -infinity, gives zeros and lse
- * -infinity. What is hidden from a row does not reach it, infinities and NaN included.
+ * -infinity. What is hidden from a row does not reach it, infinities and NaN included. Weights are rounded to 16 bits
+ * (bf16 where the cache is bf16, else fp16) before they meet the values; sums have 32. `out` may be q itself.
  * The queries' rows have to be in the cache already: append first, then attend, on one stream. */
 typedef struct amem_kv_attention_args {
   uint64_t q, out;               /* [token][head][dim], like k in append */
@@ -127,8 +129,8 @@ typedef struct amem_kv_attention_args {
 } amem_kv_attention_args;
 int amem_kv_attention(const amem_kv_cache* cache, const amem_kv_batch* batch, const amem_kv_attention_args* args, void* stream);
 
-/* Bytes of workspace that amem_kv_attention needs for these sizes (sizes and counts are read, no
- * address is), 0 if none. What it holds between calls does not matter. Returns 0, or hipErrorInvalidValue. */
+/* Bytes of workspace that amem_kv_attention needs for these sizes and any mask, 0 if none (no address is read, only
+ * whether cu_tokens is 0). What it holds between calls does not matter. Returns 0, or hipErrorInvalidValue. */
 int amem_kv_attention_workspace(const amem_kv_cache* cache, const amem_kv_batch* batch, int q_heads, uint64_t* bytes);
 
 #pragma GCC visibility pop

@@ -102,6 +102,27 @@ with torch.cuda.stream(side):
 side.synchronize()
 assert same(want, w.state())
 
+step("the result in the queries' place, no tokens at all, an error of the caller's that is not this call's")
+for tokens, context in ((1, 3000), (3, 100), (40, 90)):
+    w = World(3, context, True, tokens=tokens)
+    w.run()
+    torch.cuda.synchronize()
+    s = torch.cuda.current_stream().cuda_stream
+    kv.attention(w.cache, w.batch, w.turned, w.turned, workspace=w.workspace, stream=s)
+    torch.cuda.synchronize()
+    assert torch.equal(w.turned, w.out)
+none = kv.Batch(w.table, w.context, tokens=0, cu_tokens=torch.zeros(4, dtype=torch.int32, device=DEV), max_context=90)
+before = w.state()
+kv.append(w.cache, none, w.new_k[:0], w.new_v[:0], w.q[:0], w.q[:0], rotation=w.rotation, stream=s)
+kv.attention(w.cache, none, w.q[:0], w.out[:0], workspace=w.workspace, stream=s)
+big = torch.randn(8192, 8192, device=DEV)
+big @ big
+e = torch.cuda.Event()
+e.record()
+e.query()                         # most likely not ready
+kv.attention(w.cache, w.batch, w.q, w.out, workspace=w.workspace, stream=s)
+torch.cuda.synchronize()
+
 step("captured and replayed, with eager work in between, two graphs on one workspace")
 for eight in (False, True):
     a, b = World(6, 1500, eight), World(3, 4000, eight, tokens=2)

@@ -323,7 +323,8 @@ def check_attend(case, q, causal=True, window=0, scale=None, sequences=None, q_l
             k, v = case.gathered(s, h // group)
             out, l, size, top = O.attend(O.decode(q[rows, h], case.kind), k, v, scale_, seen)
             score = case.dim * 2.0 ** -23 * top + 2.0 ** -18
-            slack = (weight + score)[:, None] * size + 2.0 ** -30 * np.abs(np.nan_to_num(v, posinf=0, neginf=0)).max(initial=0)
+            with np.errstate(invalid="ignore"):
+                slack = (weight + score)[:, None] * size + 2.0 ** -30 * np.abs(np.nan_to_num(v, posinf=0, neginf=0)).max(initial=0)
             near(got[rows, h], out, case.kind, slack)
             same = (lse[rows, h] == l) | (np.isnan(lse[rows, h]) & np.isnan(l))
             with np.errstate(invalid="ignore"):

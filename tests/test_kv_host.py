@@ -130,6 +130,17 @@ def test_uniform_rows_have_to_add_up(lib):
     assert calls(lib, cache, batch, app, att) == (INVALID, INVALID)
 
 
+@pytest.mark.parametrize("tokens,sequences,kv_heads,q_heads", [(1 << 22, 5, 4, 64), (1 << 21, 5, 64, 64), (100, 1 << 20, 4, 4), (1 << 20, 5, 128, 128)])
+def test_sizes_beyond_a_launch_are_refused(lib, tokens, sequences, kv_heads, q_heads):
+    cache, batch, app, att = valid(True)
+    batch.tokens, batch.max_tokens, batch.sequences = tokens, tokens, sequences
+    cache.kv_heads, att.q_heads = kv_heads, q_heads
+    kv.load()
+    assert lib.amem_kv_attention(C.byref(cache), C.byref(batch), C.byref(att), None) == INVALID
+    n = C.c_uint64()
+    assert lib.amem_kv_attention_workspace(C.byref(cache), C.byref(batch), q_heads, C.byref(n)) == INVALID
+
+
 def test_null_structs(lib):
     cache, batch, app, att = valid()
     kv.load()
