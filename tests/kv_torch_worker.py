@@ -102,6 +102,23 @@ with torch.cuda.stream(side):
 side.synchronize()
 assert same(want, w.state())
 
+step("two calls at once, on two streams with a workspace each")
+a, b = World(2, 20000, True), World(3, 700, False, tokens=30)
+wants = []
+for w in (a, b):
+    w.run()
+    wants.append(w.state())
+streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+for w in (a, b):
+    w.out.zero_()
+    w.lse.zero_()
+torch.cuda.synchronize()
+for _ in range(20):
+    for w, side in zip((a, b), streams):
+        with torch.cuda.stream(side):
+            w.run()
+assert same(wants[0], a.state()) and same(wants[1], b.state())
+
 step("the result in the queries' place, no tokens at all, an error of the caller's that is not this call's")
 for tokens, context in ((1, 3000), (3, 100), (40, 90)):
     w = World(3, context, True, tokens=tokens)

@@ -527,6 +527,51 @@ def test_attention_same_bits_again_and_any_workspace(arena):
 Case_MiB = 1 << 20
 
 
+@pytest.mark.parametrize("eight", [False, True])
+def test_max_tokens_is_a_guide(arena, eight):
+    """Ragged rows with max_tokens too small, and too large: another kernel takes them, with the same definition."""
+    for most, lengths in ((1, [(50, 90), (1, 30), (7, 7)]), (20, [(1, 30), (2, 90), (17, 40)]), (0, [(3, 9)])):
+        case = Case(arena, lengths, dim=128, q_heads=8, kv_heads=2, eight=eight, page=16, seed=27)
+        case.max_tokens = most
+        case.upload()
+        check_attend(case, case.rows(8))
+        arena.reset()
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_offsets_beyond_32_bits(gpu, arena, eight):
+    """A cache whose pages are 2.25 GiB apart."""
+    far = Arena(gpu, 10 << 30)
+    try:
+        for lengths in ([(1, 70), (2, 100)], [(90, 120), (1, 40)]):
+            case = Case(arena, lengths, dim=128, q_heads=4, kv_heads=2, eight=eight, page=64, block=32, seed=28, spare_pages=0).upload()
+            gap = 9 << 28
+            assert 4 << 30 < (int(case.pages) - 1) * gap < 9 << 30
+            element = 1 if eight else 2
+            case.cache.k, case.cache.v, case.cache.page_stride = far.va, far.va + (1 << 28), gap // element
+
+            def each(what):
+                for i in range(case.pages):
+                    what(i, far.va + i * gap, far.va + i * gap + (1 << 28))
+            each(lambda i, k, v: (far.write(k, case.k[i]), far.write(v, case.v[i])))
+
+            def download():
+                k, v = np.empty_like(case.k), np.empty_like(case.v)
+
+                def one(i, kp, vp):
+                    k[i], v[i] = far.read(kp, k[i].shape, k.dtype), far.read(vp, v[i].shape, v.dtype)
+                each(one)
+                scales = tuple(arena.read(x, case.k_scale.shape, np.float32) for x in (case.d_ks, case.d_vs)) if eight else (None, None)
+                return (k, v) + scales
+            case.download = download
+            check_append(case, case.rows(2), case.rows(2), case.rows(4), rotary=128)
+            case.k, case.v = download()[:2]
+            check_attend(case, case.rows(4))
+            arena.reset()
+    finally:
+        far.free()
+
+
 def test_append_then_attend_as_used(arena):
     """A conversation of two sequences: prompts, tokens one by one, drafted tokens of which some are taken back; the cache in 8
     bits. The attention is held to the cache as the definition of append leaves it."""
