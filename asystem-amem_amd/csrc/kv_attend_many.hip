@@ -51,6 +51,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
   constexpr bool kHalfP = EIGHT || HALF;  // weights are fp16 where the values' type allows it
   // fp16 weights are held 2^8 times larger, which keeps small ones out of the subnormal numbers
   constexpr float kLift = kHalfP ? 8.0f : 0.0f;
+  constexpr float kSlack = 7.0f;  // fp16 holds 2^(kLift + kSlack)
   // Scales of keys go into the keys where 16 bits hold every product (bf16), else into the scores.
   constexpr bool kFold = EIGHT && !HALF;
   // What a lane holds of its row: scores of kScores positions of a tile, and sums of kSums dims in kBlocks results of the matrix unit.
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
   for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
     for (int j = 0; j < kSums; ++j) sum[i][j] = 0;
-  float unit_scale = 0;  // the sums are in multiples of it (8 bits)
+  uint32_t unit_scale = 0;  // the sums are in multiples of it (8 bits); bits
 
   // ---- loading: a thread's rows of a tile
   const int my_row = tid / kRowLanes, my_col = tid % kRowLanes * 16;
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
   // of group g; else each of the thread's rows has its own.
   int page[WIDE ? 1 : kPasses];
   uint32_t missing = 0;  // groups, or rows, of the tile in the registers whose page is out of range
-  float ks = 0, vs = 0;  // of the tile in the registers, lane g has group g's
+  uint32_t ks = 0, vs = 0;  // scales of the tile in the registers, lane g has group g's; as bits, whose order is that of the numbers
   // Nothing is done with a page here: that would wait for all loads under way. Behind the last position it is that one's.
   auto look_up = [&](int base) {
     if constexpr (WIDE) {
@@ -160,27 +161,27 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
     }
     if constexpr (EIGHT) {
       const int64_t at = kv_scale_offset(c, kv_checked(c, page[0]) < 0 ? 0 : page[0], kvh, base + (lane & 3) * 16);
-      ks = c.k_scale[at];
-      vs = c.v_scale[at];
+      ks = ((const uint32_t*)c.k_scale)[at];
+      vs = ((const uint32_t*)c.v_scale)[at];
     }
   };
   auto partial = [&](int base) { return base < u.all_from || base + kTile > u.all_to; };
   // The registers' tile into LDS. Keys of a page that is out of range become NaN, which every row that sees them gets.
-  float key_scale[4] = {1, 1, 1, 1}, stored_scale = 0;  // of the tile stored last
+  // Values are stored in multiples of the largest scale so far, as powers of two: a difference of exponents.
+  float key_scale[4];         // of the tile stored last
+  uint32_t stored_scale = 0;  // bits
+  constexpr uint32_t kExponent = 0x7f800000, kOne = 0x3f800000;
   auto store = [&](int base, int buffer) {
     uint8_t* const at = lds + buffer * kBuffer;
-    float value_scale[4];
+    uint32_t seen_vs = 0;
     if constexpr (EIGHT) {
+      const int p = base + (lane & 3) * 16;
+      seen_vs = p < u.to && p + 15 >= u.lo ? vs : 0;  // a hidden group's scale may be anything
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const bool seen = base + g * 16 < u.to && base + g * 16 + 15 >= u.lo;  // a hidden group's scale may be anything
-        key_scale[g] = seen ? lane_value(ks, g) : 0;
-        value_scale[g] = seen ? lane_value(vs, g) : 0;
-        stored_scale = __builtin_elementwise_maximum(stored_scale, value_scale[g]);
+        if constexpr (!kFold) key_scale[g] = lane_value(__builtin_bit_cast(float, ks), g);
+        stored_scale = std::max(stored_scale, (uint32_t)__builtin_amdgcn_readlane((int)seen_vs, g));
       }
-      const float f = stored_scale > 0 ? 1.0f / stored_scale : 0.0f;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) value_scale[g] *= f;
     }
     const bool edge = partial(base);
 #pragma unroll
@@ -197,9 +198,9 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
         if (lanes >> (lane / kRowLanes * kRowLanes) & ((1ull << kRowLanes) - 1)) v = u32x4{0, 0, 0, 0};
       }
       if constexpr (EIGHT) {
-        const int g = r >> 4;
-        const float fk = kFold ? (g & 2 ? (g & 1 ? key_scale[3] : key_scale[2]) : (g & 1 ? key_scale[1] : key_scale[0])) : 1.0f;
-        const float fv = g & 2 ? (g & 1 ? value_scale[3] : value_scale[2]) : (g & 1 ? value_scale[1] : value_scale[0]);
+        const float fk = kFold ? __builtin_bit_cast(float, __shfl((int)ks, r >> 4, kWave)) : 1.0f;
+        const int apart = __shfl((int)seen_vs, r >> 4, kWave) - (int)(stored_scale & kExponent) + (int)kOne;
+        const float fv = __builtin_bit_cast(float, apart > 0 ? apart : 0);
         uint8_t* ka = at + r * kKeyPitch + my_col * 2;
         uint8_t* va = at + kTile * kKeyPitch + r * kValuePitch + my_col * 2;
         *(u32x4*)ka = widen_scaled<HALF>(u32x2{k[0], k[1]}, fk);
@@ -232,7 +233,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
 #pragma unroll
       for (int g = 0; g < 4; ++g) f[g] = key_scale[g];
     }
-    const float tile_scale = stored_scale;
+    const uint32_t tile_scale = stored_scale;
     if (work) {
       Result s[kTile / R];
 #pragma unroll
@@ -274,8 +275,11 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
     for (int j = 0; j < kScores; ++j) top = __builtin_elementwise_maximum(top, score[j]);  // NaN stays
     if constexpr (R == 16) top = __builtin_elementwise_maximum(top, __shfl_xor(top, 16, kWave));
     top = __builtin_elementwise_maximum(top, __shfl_xor(top, 32, kWave));
-    const float now = __builtin_elementwise_maximum(m, top * factor);
-    if (__any(now != m)) {
+    // m follows the largest score only when it is left behind by 2^kSlack: weights above one do no harm, and the sums are rarely
+    // multiplied (for a new largest score in any of a wave's rows it would be most tiles)
+    top *= factor;
+    if (__any(!(top <= m + kSlack))) {
+      const float now = __builtin_elementwise_maximum(m, top);
       const float shrink = now == m ? 1.0f : __builtin_amdgcn_exp2f(m - now);
       l *= shrink;
 #pragma unroll
@@ -284,8 +288,8 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
         for (int j = 0; j < kSums; ++j) sum[i][j] *= shrink;
       m = now;
     }
-    if (EIGHT && !(tile_scale <= unit_scale)) {
-      const float x = unit_scale / tile_scale;
+    if (EIGHT && tile_scale != unit_scale) {  // it only grows
+      const float x = __builtin_bit_cast(float, unit_scale & kExponent) / __builtin_bit_cast(float, tile_scale & kExponent);
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
@@ -334,7 +338,8 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
             if (j == index) x = score[j];
           x = __shfl(x, (R == 32 ? k / 4 % 2 : k / 4 % 4) * R + col, kWave);
           if (p < row_from || p >= row_to) continue;
-          if constexpr (EIGHT) x *= c.v_scale[kv_scale_offset(c, where, kvh, p)] * (unit_scale > 0 ? 1.0f / unit_scale : 0.0f);
+          if constexpr (EIGHT)
+            x *= c.v_scale[kv_scale_offset(c, where, kvh, p)] * (unit_scale ? 1.0f / __builtin_bit_cast(float, unit_scale & kExponent) : 0.0f);
 #pragma unroll
           for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
@@ -350,7 +355,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
 
   if constexpr (R == 16) l += __shfl_xor(l, 16, kWave);
   l += __shfl_xor(l, 32, kWave);
-  const float back = EIGHT && unit_scale > 0 ? unit_scale : 1.0f;
+  const float back = EIGHT ? __builtin_bit_cast(float, unit_scale & kExponent) : 1.0f;
   const int r = wave * R + col;
   if (r >= u.rows) return;
   if (parts.splits > 1) {
