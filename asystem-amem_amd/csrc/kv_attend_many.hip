@@ -35,9 +35,9 @@ __device__ __forceinline__ u32x4 widen_scaled(u32x2 x, float scale) {
   return y;
 }
 
-// D dims, 16 bits of fp16 (HALF) or bf16, a cache of e4m3 (EIGHT), pages of at least 16 slots (WIDE).
+// D dims, 16 bits of fp16 (HALF) or bf16, a cache of e4m3 (EIGHT).
 // W waves with R rows each, 32 or 16.
-template <int D, bool HALF, bool EIGHT, bool WIDE, int W, int R>
+template <int D, bool HALF, bool EIGHT, int W, int R>
 __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b, KvAttend a, Parts parts) {
   constexpr int kThreads = W * kWave;
   constexpr int kShift = W * R == 256 ? 8 : 7;    // log2 of a unit's rows
@@ -111,56 +111,29 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
   const uint8_t* const keys = c.k + (int64_t)kvh * c.head_stride;
   const uint8_t* const values = c.v + (int64_t)kvh * c.head_stride;
   u32x4 kreg[kPasses], vreg[kPasses];
-  // Pages of the tile to be loaded next, as the page table has them. WIDE: 16 positions lie in one page, and lane g has that
-  // of group g; else each of the thread's rows has its own.
-  int page[WIDE ? 1 : kPasses];
-  uint32_t missing = 0;  // groups, or rows, of the tile in the registers whose page is out of range
-  uint32_t ks = 0, vs = 0;  // scales of the tile in the registers, lane g has group g's; as bits, whose order is that of the numbers
+  // Pages of the tile to be loaded next, as the page table has them, of the thread's rows and (8 bits) in lane g of group g of 16.
+  int page[kPasses], group_page = 0;
+  uint32_t missing = 0;         // rows of the tile in the registers whose page is out of range
+  uint32_t ks = 0, vs = 0;      // scales of the tile in the registers, lane g has group g's; as bits, whose order is that of the numbers
   // Nothing is done with a page here: that would wait for all loads under way. Behind the last position it is that one's.
   auto look_up = [&](int base) {
-    if constexpr (WIDE) {
-      page[0] = kv_table(c, b, u.s, std::min(base + (lane & 3) * 16, u.to - 1));
-    } else {
 #pragma unroll
-      for (int i = 0; i < kPasses; ++i) page[i] = kv_table(c, b, u.s, std::min(base + i * kRowsAPass + my_row, u.to - 1));
-    }
+    for (int i = 0; i < kPasses; ++i) page[i] = kv_table(c, b, u.s, std::min(base + i * kRowsAPass + my_row, u.to - 1));
+    if constexpr (EIGHT) group_page = kv_table(c, b, u.s, std::min(base + (lane & 3) * 16, u.to - 1));
   };
-  // this thread's offset in a group: 32 bits, since a page's rows span less than 2^31 bytes
-  const uint32_t my_off = (uint32_t)((my_row & 15) * (int)c.slot_stride + my_col);
   auto load = [&](int base) {
     missing = 0;
-    if constexpr (WIDE) {
-      // every lane its group's, which costs a tenth of four on the scalar unit
-      const int where = kv_checked(c, page[0]);
-      missing = (uint32_t)__ballot(where < 0) & 15;
-      const int64_t mine = (int64_t)(where < 0 ? 0 : where) * c.page_stride + (base + (lane & 3) * 16 & slot_mask) * (int64_t)(int)c.slot_stride;
-      int64_t at[4];
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        at[g] = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), g) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, g));
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        constexpr int kGroupsAPass = (kRowsAPass + 15) / 16;
-        const int g0 = i * kRowsAPass / 16, r0 = i * kRowsAPass % 16;
-        int64_t from = at[g0];
-#pragma unroll
-        for (int g = 1; g < kGroupsAPass; ++g) from = my_row >> 4 >= g ? at[g0 + g] : from;
-        from += r0 * c.slot_stride;
-        kreg[i] = *(const u32x4*)(keys + from + my_off);
-        vreg[i] = *(const u32x4*)(values + from + my_off);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        const int p = base + i * kRowsAPass + my_row, where = kv_checked(c, page[i]);
-        if (where < 0) missing |= 1u << i;
-        const int64_t at = (int64_t)(where < 0 ? 0 : where) * c.page_stride + (int64_t)(p & slot_mask) * c.slot_stride + my_col;
-        kreg[i] = *(const u32x4*)(keys + at);
-        vreg[i] = *(const u32x4*)(values + at);
-      }
+    for (int i = 0; i < kPasses; ++i) {
+      const int p = base + i * kRowsAPass + my_row, where = kv_checked(c, page[i]);
+      if (where < 0) missing |= 1u << i;
+      // a page's rows span less than 2^31 bytes
+      const int64_t at = (int64_t)(where < 0 ? 0 : where) * c.page_stride + (uint32_t)((p & slot_mask) * (int)c.slot_stride + my_col);
+      kreg[i] = *(const u32x4*)(keys + at);
+      vreg[i] = *(const u32x4*)(values + at);
     }
     if constexpr (EIGHT) {
-      const int64_t at = kv_scale_offset(c, kv_checked(c, page[0]) < 0 ? 0 : page[0], kvh, base + (lane & 3) * 16);
+      const int64_t at = kv_scale_offset(c, kv_checked(c, group_page) < 0 ? 0 : group_page, kvh, base + (lane & 3) * 16);
       ks = ((const uint32_t*)c.k_scale)[at];
       vs = ((const uint32_t*)c.v_scale)[at];
     }
@@ -188,7 +161,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
     for (int i = 0; i < kPasses; ++i) {
       const int r = i * kRowsAPass + my_row;
       u32x4 k = kreg[i], v = vreg[i];
-      if (missing && missing >> (WIDE ? r >> 4 : i) & 1) k = u32x4{~0u, ~0u, ~0u, ~0u};
+      if (missing && missing >> i & 1) k = u32x4{~0u, ~0u, ~0u, ~0u};
       if (edge) {
         // a weight of zero does not hide infinities and NaN: values that no row sees become zeros here, and those that
         // only some rows see are taken out of the product and added one by one
@@ -417,17 +390,17 @@ void plan(const KvCache& c, const KvBatch& b, int group, const Shape& shape, con
 template <int D, int W, int R>
 hipError_t launch_waves(const KvCache& c, const KvBatch& b, const KvAttend& a, bool half, bool eight, const Parts& parts, hipStream_t stream) {
   const uint32_t grid = (uint32_t)parts.units * c.kv_heads * parts.splits;
-  const bool wide = c.page_shift >= 4;
   constexpr int kThreads = W * kWave;
   if (eight) {
     if constexpr (D > 64 || W == 4) {
-      if (half) attend_many<D, true, true, true, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-      else attend_many<D, false, true, true, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+      if (half) attend_many<D, true, true, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+      else attend_many<D, false, true, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
     }
-  } else if (half && wide) attend_many<D, true, false, true, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-  else if (half) attend_many<D, true, false, false, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-  else if (wide) attend_many<D, false, false, true, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-  else attend_many<D, false, false, false, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  } else if (half) {
+    attend_many<D, true, false, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  } else {
+    attend_many<D, false, false, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+  }
   if (hipError_t e = hipGetLastError(); e != hipSuccess || parts.splits == 1) return e;
   return launch_join(c, b, a, parts, W * R == 256 ? 8 : 7, half || eight ? 8.0f : 0.0f, D, half, stream);
 }
