@@ -103,7 +103,7 @@ __device__ __forceinline__ void turn(const KvAppend& a, const float (&c)[8], con
 }
 
 // The sequence of a row, -1 if it has none.
-__device__ __forceinline__ int sequence_of_row(const KvBatch& b, int row) { return b.cu_tokens ? find_sequence(b, row, 0, 0) : row / b.uniform; }
+__device__ __forceinline__ int sequence_of_row(const KvBatch& b, int row) { return b.cu_tokens ? find_sequence(b, row, 1, 0) : row / b.uniform; }
 
 // One wave for a share of the heads of a row: query heads and, where the cache has 16 bits (KV), its key and value heads.
 // A lane keeps to the same dims, so its cosines and sines are read once, and takes four heads at a time.
@@ -212,8 +212,8 @@ __device__ __forceinline__ void append_blocks(const KvCache& c, const KvBatch& b
   const int shift = c.block_shift, size = 1 << shift;
   if (unit < units) {
     if (b.cu_tokens) {
-      s = find_sequence(b, unit, shift, 2);
-      unit -= s >= 0 ? kv_unit_base(b, s, shift, 2) : 0;
+      s = find_sequence(b, unit, size, 2);
+      unit -= s >= 0 ? kv_unit_base(b, s, size, 2) : 0;
     } else {
       const int each = ((b.uniform - 1) >> shift) + 2;
       s = unit / each;
@@ -348,7 +348,7 @@ hipError_t launch_kv_append(const KvCache& c, const KvBatch& b, const KvAppend& 
     else append16<false><<<row_groups, kThreads, 0, stream>>>(c, b, a, items, shares);
     return hipGetLastError();
   }
-  const int units = b.cu_tokens ? kv_units(b, c.block_shift, 2) : b.sequences * (((b.uniform - 1) >> c.block_shift) + 2);
+  const int units = b.cu_tokens ? kv_units(b, 1 << c.block_shift, 2) : b.sequences * (((b.uniform - 1) >> c.block_shift) + 2);
   // items that a block gets at most: up to 64 for single tokens, to 2048 for whole blocks, which take one, two or four waves
   const int block_items = items * (b.cu_tokens ? 1 << c.block_shift : std::min(b.uniform, 1 << c.block_shift));
   auto run = [&](auto kernel, int waves) {

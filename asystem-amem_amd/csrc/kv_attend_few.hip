@@ -48,10 +48,9 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   // heads first: their rows of a page are neighbours
   const int group = a.q_heads / c.kv_heads, kvh = blockIdx.x % c.kv_heads, unit = blockIdx.x / c.kv_heads % few.units, split = blockIdx.x / c.kv_heads / few.units;
-  constexpr int shift = NB == 1 ? 4 : NB == 2 ? 5 : 6;
   KvSeq q;
   Unit u;
-  if (!find_unit(b, a, group, shift, unit, q, u)) return;
+  if (!find_unit(b, a, group, 16 * NB, unit, q, u)) return;
   const int begin = u.from + split * few.stretch;
   if (split && (begin >= u.to || q.bad)) return;
   const int end = begin + few.stretch < u.to ? begin + few.stretch : u.to;
@@ -425,16 +424,15 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
 // values are read once.
 int blocks_of(int group, int max_tokens, int head_dim) {
   const int64_t rows = (int64_t)group * max_tokens;
-  return rows <= 16 ? 1 : rows <= 32 || head_dim > 64 ? 2 : 4;
+  return rows <= 16 ? 1 : rows <= 32 || head_dim > 64 ? 2 : rows <= 48 ? 3 : 4;
 }
 
 // Stretches of the same length, as long as leaves about kTarget workgroups, and at least kLeast positions.
 void plan(const KvCache& c, const KvBatch& b, int group, int blocks, const KvAttend& a, Parts* few) {
-  const int shift = blocks == 1 ? 4 : blocks == 2 ? 5 : 6;
   int64_t span = b.max_context;
   const int64_t seen = (int64_t)a.window + (16 * blocks) / group + 1 + 64;
   if (a.causal && a.window && seen < span) span = seen;  // else a window has no far end
-  few->units = units_of(b, group, shift);
+  few->units = units_of(b, group, 16 * blocks);
   const int64_t all = (int64_t)few->units * c.kv_heads * span;
   const int64_t step = kWaves * 64, stretch = std::max<int64_t>((all + kTarget - 1) / kTarget, kLeast);
   few->splits = span > stretch ? (int)((span + stretch - 1) / stretch) : 1;
@@ -443,7 +441,6 @@ void plan(const KvCache& c, const KvBatch& b, int group, int blocks, const KvAtt
 
 template <int D, bool HALF, bool EIGHT, int NB>
 hipError_t launch_few(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& few, hipStream_t stream) {
-  const int group = a.q_heads / c.kv_heads, shift = NB == 1 ? 4 : NB == 2 ? 5 : 6;
   const uint32_t grid = (uint32_t)few.units * c.kv_heads * few.splits;
   if constexpr (!EIGHT) {
     if (c.page_shift < 4) attend_few<D, HALF, EIGHT, NB, false><<<grid, kWaves * kWave, 0, stream>>>(c, b, a, few);
@@ -452,14 +449,14 @@ hipError_t launch_few(const KvCache& c, const KvBatch& b, const KvAttend& a, con
     attend_few<D, HALF, EIGHT, NB, true><<<grid, kWaves * kWave, 0, stream>>>(c, b, a, few);
   }
   if (hipError_t e = hipGetLastError(); e != hipSuccess || few.splits == 1) return e;
-  return launch_join(c, b, a, few, shift, EIGHT || HALF ? 8.0f : 0.0f, D, HALF, stream);
+  return launch_join(c, b, a, few, 16 * NB, EIGHT || HALF ? 8.0f : 0.0f, D, HALF, stream);
 }
 
 template <int D, bool HALF, bool EIGHT>
 hipError_t launch_blocks(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& few, int blocks, hipStream_t stream) {
   if (blocks == 1) return launch_few<D, HALF, EIGHT, 1>(c, b, a, few, stream);
   if (blocks == 2) return launch_few<D, HALF, EIGHT, 2>(c, b, a, few, stream);
-  if constexpr (D == 64) return launch_few<D, HALF, EIGHT, 4>(c, b, a, few, stream);
+  if constexpr (D == 64) return blocks == 3 ? launch_few<D, HALF, EIGHT, 3>(c, b, a, few, stream) : launch_few<D, HALF, EIGHT, 4>(c, b, a, few, stream);
   else return launch_few<D, HALF, EIGHT, 2>(c, b, a, few, stream);
 }
 
@@ -474,8 +471,7 @@ hipError_t launch_dims(const KvCache& c, const KvBatch& b, const KvAttend& a, bo
 uint64_t kv_attend_few_workspace(const KvCache& c, const KvBatch& b, int q_heads, int max_tokens, int head_dim) {
   // for any window: plan() has at most that many splits
   const int group = q_heads / c.kv_heads, blocks = blocks_of(group, max_tokens, head_dim);
-  const int shift = blocks == 1 ? 4 : blocks == 2 ? 5 : 6;
-  const int64_t units = (int64_t)units_of(b, group, shift) * c.kv_heads;
+  const int64_t units = (int64_t)units_of(b, group, 16 * blocks) * c.kv_heads;
   if (!units) return 0;
   const int64_t splits = std::min<int64_t>((b.max_context + kLeast - 1) / kLeast, (kTarget + units - 1) / units);
   return splits < 2 ? 0 : (uint64_t)(units * splits * (16 * blocks)) * (head_dim + 2) * 4;

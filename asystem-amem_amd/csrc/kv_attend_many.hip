@@ -40,7 +40,6 @@ __device__ __forceinline__ u32x4 widen_scaled(u32x2 x, float scale) {
 template <int D, bool HALF, bool EIGHT, int W, int R>
 __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b, KvAttend a, Parts parts) {
   constexpr int kThreads = W * kWave;
-  constexpr int kShift = W * R == 256 ? 8 : 7;    // log2 of a unit's rows
   constexpr int kElement = EIGHT ? 1 : 2;
   constexpr int kRowLanes = D * kElement / 16;    // threads that load a position's key, or value
   constexpr int kRowsAPass = kThreads / kRowLanes;
@@ -68,7 +67,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
   const int unit = parts.units - 1 - blockIdx.x / c.kv_heads % parts.units, split = blockIdx.x / c.kv_heads / parts.units;
   KvSeq q;
   Unit u;
-  if (!find_unit(b, a, group, kShift, unit, q, u)) return;
+  if (!find_unit(b, a, group, W * R, unit, q, u)) return;
   const int begin = u.from + split * parts.stretch;
   if (split && (begin >= u.to || q.bad)) return;
   const int end = begin + parts.stretch < u.to ? begin + parts.stretch : u.to;
@@ -341,7 +340,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
   const int r = wave * R + col;
   if (r >= u.rows) return;
   if (parts.splits > 1) {
-    const int64_t row = (part_of(c, parts, unit, kvh, split) << kShift) + r;
+    const int64_t row = part_of(c, parts, unit, kvh, split) * (W * R) + r;
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
@@ -372,23 +371,23 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
 // dims of e4m3, where four load a tile at once. 256 dims leave a wave of 32 rows a SIMD for itself; eight of 16 rows, two a
 // SIMD, read LDS twice as often and are faster all the same: VMEASURE.
 struct Shape {
-  int shift, fit;  // log2 of the rows; workgroups that fit at once
+  int rows, fit;   // of a unit; workgroups that fit at once
   bool eight;      // eight waves
 };
 Shape shape_of(const KvCache& c, const KvBatch& b, int group, int head_dim) {
-  if (head_dim == 256) return {7, 256, true};
-  if (head_dim == 64 && c.block_shift) return {7, 512, false};
-  if ((int64_t)units_of(b, group, 8) * c.kv_heads >= 512) return {8, 256, true};
-  return {7, 512, false};
+  if (head_dim == 256) return {128, 256, true};
+  if (head_dim == 64 && c.block_shift) return {128, 512, false};
+  if ((int64_t)units_of(b, group, 256) * c.kv_heads >= 512) return {256, 256, true};
+  return {128, 512, false};
 }
 
 constexpr int kLeast = 512;  // positions of a workgroup, at least: a part costs its rows' sums written and read once more
 
 // Contexts are cut only where units are fewer than fit at once, into stretches of the same length.
 void plan(const KvCache& c, const KvBatch& b, int group, const Shape& shape, const KvAttend& a, Parts* parts) {
-  parts->units = units_of(b, group, shape.shift);
+  parts->units = units_of(b, group, shape.rows);
   int64_t span = b.max_context;
-  const int64_t seen = (int64_t)a.window + (1 << shape.shift) / group + 1 + 64;
+  const int64_t seen = (int64_t)a.window + shape.rows / group + 1 + 64;
   if (a.causal && a.window && seen < span) span = seen;  // else a window has no far end
   const int64_t all = (int64_t)parts->units * c.kv_heads * span;
   const int64_t stretch = std::max<int64_t>((all + shape.fit - 1) / shape.fit, kLeast);
@@ -411,7 +410,7 @@ hipError_t launch_waves(const KvCache& c, const KvBatch& b, const KvAttend& a, b
     attend_many<D, false, false, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
   }
   if (hipError_t e = hipGetLastError(); e != hipSuccess || parts.splits == 1) return e;
-  return launch_join(c, b, a, parts, W * R == 256 ? 8 : 7, half || eight ? 8.0f : 0.0f, D, half, stream);
+  return launch_join(c, b, a, parts, W * R, half || eight ? 8.0f : 0.0f, D, half, stream);
 }
 
 template <int D>
@@ -430,10 +429,10 @@ uint64_t kv_attend_many_workspace(const KvCache& c, const KvBatch& b, int q_head
   // for any window: plan() has at most that many splits
   const int group = q_heads / c.kv_heads;
   const Shape shape = shape_of(c, b, group, head_dim);
-  const int64_t units = (int64_t)units_of(b, group, shape.shift) * c.kv_heads;
+  const int64_t units = (int64_t)units_of(b, group, shape.rows) * c.kv_heads;
   if (!units) return 0;
   const int64_t splits = std::min<int64_t>((b.max_context + kLeast - 1) / kLeast, (shape.fit + units - 1) / units);
-  return splits < 2 ? 0 : (uint64_t)((units * splits) << shape.shift) * (head_dim + 2) * 4;
+  return splits < 2 ? 0 : (uint64_t)(units * splits * shape.rows) * (head_dim + 2) * 4;
 }
 
 hipError_t launch_kv_attend_many(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream) {
@@ -442,7 +441,7 @@ hipError_t launch_kv_attend_many(const KvCache& c, const KvBatch& b, const KvAtt
   Parts parts;
   plan(c, b, group, shape, a, &parts);
   parts.sums = (float*)a.workspace;
-  parts.stats = parts.sums + (((int64_t)parts.units * c.kv_heads * parts.splits) << shape.shift) * head_dim;
+  parts.stats = parts.sums + (int64_t)parts.units * c.kv_heads * parts.splits * shape.rows * head_dim;
   if (head_dim == 64) return launch<64>(c, b, a, half, eight, parts, shape, stream);
   if (head_dim == 128) return launch<128>(c, b, a, half, eight, parts, shape, stream);
   return launch<256>(c, b, a, half, eight, parts, shape, stream);

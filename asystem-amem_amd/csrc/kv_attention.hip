@@ -10,7 +10,7 @@ constexpr int kJoinWaves = 4;
 // Joins the stretches of a row and query head: W waves take the stretches in turn (one wave where they are few, since then
 // rows are many).
 template <int D, bool HALF, int W>
-__global__ __launch_bounds__(kJoinWaves * kWave) void join_stretches(KvCache c, KvBatch b, KvAttend a, Parts parts, int shift, float lift) {
+__global__ __launch_bounds__(kJoinWaves * kWave) void join_stretches(KvCache c, KvBatch b, KvAttend a, Parts parts, int tile, float lift) {
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int index = blockIdx.x * (kJoinWaves / W) + wave / W, turn = wave % W;
   const int row = index / a.q_heads, head = index % a.q_heads, group = a.q_heads / c.kv_heads, kvh = head / group;
@@ -18,7 +18,7 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void join_stretches(KvCache c, 
   float m = -kInf, l = 0, x[N] = {};
   KvSeq q;
   Unit u;
-  const int s = row >= b.tokens ? -1 : b.cu_tokens ? find_sequence(b, row, 0, 0) : row / b.uniform;
+  const int s = row >= b.tokens ? -1 : b.cu_tokens ? find_sequence(b, row, 1, 0) : row / b.uniform;
   bool mine = s >= 0;
   if (mine) {
     q = kv_seq(b, s);
@@ -26,12 +26,12 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void join_stretches(KvCache c, 
   }
   if (mine) {
     const int r = (row - q.row) * group + head % group;
-    const int unit = (b.cu_tokens ? kv_unit_base(b, s, shift, 1, group) : s * (((b.uniform * group - 1) >> shift) + 1)) + (r >> shift);
-    unit_at(b, a, group, shift, s, r >> shift, q, u);
+    const int unit = (b.cu_tokens ? kv_unit_base(b, s, tile, 1, group) : s * ((b.uniform * group - 1) / tile + 1)) + r / tile;
+    unit_at(b, a, group, tile, s, r / tile, q, u);
     int count = (u.to - u.from + parts.stretch - 1) / parts.stretch;
     count = q.bad || count < 1 ? 1 : count > parts.splits ? parts.splits : count;
     for (int i = turn; i < count; i += W) {
-      const int64_t at = (part_of(c, parts, unit, kvh, i) << shift) + (r & ((1 << shift) - 1));
+      const int64_t at = part_of(c, parts, unit, kvh, i) * tile + r % tile;
       const float mi = parts.stats[at * 2], li = parts.stats[at * 2 + 1];
       const float now = __builtin_elementwise_maximum(m, mi);
       const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now), g = mi == now ? 1.0f : __builtin_amdgcn_exp2f(mi - now);
@@ -66,10 +66,10 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void join_stretches(KvCache c, 
 }
 
 template <int D, bool HALF>
-hipError_t join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int shift, float lift, hipStream_t stream) {
+hipError_t join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int tile, float lift, hipStream_t stream) {
   const int rows = b.tokens * a.q_heads;
-  if (parts.splits > 8) join_stretches<D, HALF, kJoinWaves><<<rows, kJoinWaves * kWave, 0, stream>>>(c, b, a, parts, shift, lift);
-  else join_stretches<D, HALF, 1><<<(rows + kJoinWaves - 1) / kJoinWaves, kJoinWaves * kWave, 0, stream>>>(c, b, a, parts, shift, lift);
+  if (parts.splits > 8) join_stretches<D, HALF, kJoinWaves><<<rows, kJoinWaves * kWave, 0, stream>>>(c, b, a, parts, tile, lift);
+  else join_stretches<D, HALF, 1><<<(rows + kJoinWaves - 1) / kJoinWaves, kJoinWaves * kWave, 0, stream>>>(c, b, a, parts, tile, lift);
   return hipGetLastError();
 }
 
@@ -82,10 +82,10 @@ bool few_rows(int q_heads, int kv_heads, int max_tokens, int head_dim) {
 
 }  // namespace
 
-hipError_t launch_join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int shift, float lift, int head_dim, bool half, hipStream_t stream) {
-  if (head_dim == 64) return half ? join<64, true>(c, b, a, parts, shift, lift, stream) : join<64, false>(c, b, a, parts, shift, lift, stream);
-  if (head_dim == 128) return half ? join<128, true>(c, b, a, parts, shift, lift, stream) : join<128, false>(c, b, a, parts, shift, lift, stream);
-  return half ? join<256, true>(c, b, a, parts, shift, lift, stream) : join<256, false>(c, b, a, parts, shift, lift, stream);
+hipError_t launch_join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int tile, float lift, int head_dim, bool half, hipStream_t stream) {
+  if (head_dim == 64) return half ? join<64, true>(c, b, a, parts, tile, lift, stream) : join<64, false>(c, b, a, parts, tile, lift, stream);
+  if (head_dim == 128) return half ? join<128, true>(c, b, a, parts, tile, lift, stream) : join<128, false>(c, b, a, parts, tile, lift, stream);
+  return half ? join<256, true>(c, b, a, parts, tile, lift, stream) : join<256, false>(c, b, a, parts, tile, lift, stream);
 }
 
 uint64_t kv_attend_workspace(const KvCache& c, const KvBatch& b, int q_heads, int max_tokens, int head_dim) {

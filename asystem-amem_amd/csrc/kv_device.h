@@ -108,12 +108,12 @@ __device__ __forceinline__ u32x2 read_columns8(const uint8_t* p) {
 
 // The sequence that unit `u` belongs to, or -1: the number of sequences whose first unit is at most u, less one.
 // The wave looks at 64 of them at a time, so a batch of up to 64 costs one round of loads and not a chain of them.
-__device__ __forceinline__ int find_sequence(const KvBatch& b, int u, int shift, int spare, int per_row = 1) {
+__device__ __forceinline__ int find_sequence(const KvBatch& b, int u, int tile, int spare, int per_row = 1) {
   const int lane = threadIdx.x & (kWave - 1);
   int count = 0;
   for (int s0 = 0; s0 < b.sequences; s0 += kWave) {
     const int s = s0 + lane;
-    const bool below = s < b.sequences && kv_unit_base(b, s, shift, spare, per_row) <= u;
+    const bool below = s < b.sequences && kv_unit_base(b, s, tile, spare, per_row) <= u;
     const int n = __popcll(__ballot(below));
     count += n;
     if (n < kWave) break;

@@ -81,15 +81,15 @@ AMEM_HD int64_t kv_scale_offset(const KvCache& c, int page, int head, int p) {
          ((p & ((1 << c.page_shift) - 1)) >> c.block_shift);
 }
 
-// Work is handed out in units of items (tile = 1 << shift of them, `per_row` items a row) without the host knowing the
-// lengths: unit u belongs to the last sequence s with kv_unit_base(s) <= u. `spare` units more for each sequence
-// cover what its first and last, partial tiles need (1 for tiles that start at its first item, 2 for tiles of its cache
-// positions), so a call has at most kv_units() of them and some are empty. The host holds tokens * per_row to 2^27.
-AMEM_HD int kv_unit_base(const KvBatch& b, int s, int shift, int spare, int per_row = 1) {
-  return (kv_cu(b, s) * per_row >> shift) + s * spare;
+// Work is handed out in units of `tile` items (`per_row` items a row) without the host knowing the lengths: unit u
+// belongs to the last sequence s with kv_unit_base(s) <= u. `spare` units more for each sequence cover what its first and
+// last, partial tiles need (1 for tiles that start at its first item, 2 for tiles of its cache positions), so a call has at
+// most kv_units() of them and some are empty. The host holds tokens * per_row to 2^27.
+AMEM_HD int kv_unit_base(const KvBatch& b, int s, int tile, int spare, int per_row = 1) {
+  return (int)((uint32_t)(kv_cu(b, s) * per_row) / (uint32_t)tile) + s * spare;
 }
-AMEM_HD int kv_units(const KvBatch& b, int shift, int spare, int per_row = 1) {
-  return (b.tokens * per_row >> shift) + b.sequences * spare;
+AMEM_HD int kv_units(const KvBatch& b, int tile, int spare, int per_row = 1) {
+  return b.tokens * per_row / tile + b.sequences * spare;
 }
 
 }  // namespace amem

@@ -31,32 +31,32 @@ __device__ __forceinline__ void row_range(const KvAttend& a, const KvSeq& q, int
   from = a.window && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
 }
 
-// The unit of sequence s that starts at row `tile` << shift; false if there are no rows.
-__device__ __forceinline__ bool unit_at(const KvBatch& b, const KvAttend& a, int group, int shift, int s, int tile, const KvSeq& q, Unit& u) {
+// Unit `index` of sequence s, `tile` rows long; false if there are no rows.
+__device__ __forceinline__ bool unit_at(const KvBatch& b, const KvAttend& a, int group, int tile, int s, int index, const KvSeq& q, Unit& u) {
   u.s = s;
-  u.first = tile << shift;
+  u.first = index * tile;
   u.rows = q.n * group - u.first;
   if (u.rows <= 0) return false;
-  if (u.rows > 1 << shift) u.rows = 1 << shift;
+  if (u.rows > tile) u.rows = tile;
   row_range(a, q, u.first / group, u.lo, u.all_to);
   row_range(a, q, (u.first + u.rows - 1) / group, u.all_from, u.to);
   u.from = u.lo & ~63;
   return true;
 }
 
-__device__ __forceinline__ bool find_unit(const KvBatch& b, const KvAttend& a, int group, int shift, int index, KvSeq& q, Unit& u) {
+__device__ __forceinline__ bool find_unit(const KvBatch& b, const KvAttend& a, int group, int tile, int index, KvSeq& q, Unit& u) {
   int s;
   if (b.cu_tokens) {
-    s = find_sequence(b, index, shift, 1, group);
+    s = find_sequence(b, index, tile, 1, group);
     if (s < 0) return false;
-    index -= kv_unit_base(b, s, shift, 1, group);
+    index -= kv_unit_base(b, s, tile, 1, group);
   } else {
-    const int each = ((b.uniform * group - 1) >> shift) + 1;
+    const int each = (b.uniform * group - 1) / tile + 1;
     s = index / each;
     index -= s * each;
   }
   q = kv_seq(b, s);
-  return unit_at(b, a, group, shift, s, index, q, u);
+  return unit_at(b, a, group, tile, s, index, q, u);
 }
 
 // Where a stretch's part of a unit is kept.
@@ -64,14 +64,14 @@ __device__ __forceinline__ int64_t part_of(const KvCache& c, const Parts& parts,
   return ((int64_t)unit * c.kv_heads + kvh) * parts.splits + split;
 }
 
-inline int units_of(const KvBatch& b, int group, int shift) {
-  return b.cu_tokens ? kv_units(b, shift, 1, group) : b.sequences * (((b.uniform * group - 1) >> shift) + 1);
+inline int units_of(const KvBatch& b, int group, int tile) {
+  return b.cu_tokens ? kv_units(b, tile, 1, group) : b.sequences * ((b.uniform * group - 1) / tile + 1);
 }
 
 }  // namespace
 
-// Joins the stretches of every row: kv_attention.hip. `shift`: log2 of a unit's rows; `lift`: what the kernel added to m.
-hipError_t launch_join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int shift, float lift, int head_dim, bool half, hipStream_t stream);
+// Joins the stretches of every row: kv_attention.hip. `tile`: a unit's rows; `lift`: what the kernel added to m.
+hipError_t launch_join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int tile, float lift, int head_dim, bool half, hipStream_t stream);
 
 }  // namespace amem
 #endif

@@ -19,9 +19,9 @@ using namespace amem;
     }                                                        \
   } while (0)
 
-static int find(const KvBatch& b, int u, int shift, int spare) {  // what a wave of the kernels counts
+static int find(const KvBatch& b, int u, int tile, int spare) {  // what a wave of the kernels counts
   int n = 0;
-  while (n < b.sequences && kv_unit_base(b, n, shift, spare) <= u) ++n;
+  while (n < b.sequences && kv_unit_base(b, n, tile, spare) <= u) ++n;
   return n - 1;
 }
 
@@ -78,14 +78,14 @@ int main() {
         CHECK(at >= 0 && at + c.slot_stride <= cache_bytes);
       }
     }
-    for (int shift = 0; shift < 7; shift += 3) {  // tiles of rows
+    for (int tile : {1, 8, 48, 64}) {  // tiles of rows
       std::vector<int> rows(b.tokens, 0);
-      for (int u = 0; u < kv_units(b, shift, 1); ++u) {
-        const int s = find(b, u, shift, 1);
+      for (int u = 0; u < kv_units(b, tile, 1); ++u) {
+        const int s = find(b, u, tile, 1);
         if (s < 0) continue;
         const KvSeq q = kv_seq(b, s);
-        const int64_t first = (int64_t)(u - kv_unit_base(b, s, shift, 1)) << shift;
-        for (int64_t j = first; j < first + (1 << shift) && j < q.n; ++j) {
+        const int64_t first = (int64_t)(u - kv_unit_base(b, s, tile, 1)) * tile;
+        for (int64_t j = first; j < first + tile && j < q.n; ++j) {
           CHECK(q.row + j >= 0 && q.row + j < b.tokens);
           ++rows[q.row + j];
         }
@@ -95,12 +95,12 @@ int main() {
     }
     // blocks of cache positions
     std::vector<int> rows(b.tokens, 0);
-    for (int u = 0; u < kv_units(b, 4, 2); ++u) {
-      const int s = find(b, u, 4, 2);
+    for (int u = 0; u < kv_units(b, 16, 2); ++u) {
+      const int s = find(b, u, 16, 2);
       if (s < 0) continue;
       const KvSeq q = kv_seq(b, s);
       const int first = q.context - q.n > 0 ? q.context - q.n : 0;
-      const int64_t start = ((int64_t)(first >> 4) + u - kv_unit_base(b, s, 4, 2)) << 4;
+      const int64_t start = ((int64_t)(first >> 4) + u - kv_unit_base(b, s, 16, 2)) << 4;
       if (q.bad || !q.n || start >= q.context) continue;
       for (int64_t p = start > first ? start : first; p < start + 16 && p < q.context; ++p) {
         const int64_t row = q.row + q.n - q.context + p;
