@@ -1,5 +1,7 @@
 // Attention over a paged key/value cache: which kernel takes a call, and the join of the parts of rows whose positions were
 // dealt out to several workgroups.
+#include <algorithm>
+
 #include "kv_parts.h"
 
 namespace amem {
@@ -30,15 +32,29 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void join_stretches(KvCache c, 
     unit_at(b, a, group, tile, s, r / tile, q, u);
     int count = (u.to - u.from + parts.stretch - 1) / parts.stretch;
     count = q.bad || count < 1 ? 1 : count > parts.splits ? parts.splits : count;
-    for (int i = turn; i < count; i += W) {
-      const int64_t at = part_of(c, parts, unit, kvh, i) * tile + r % tile;
-      const float mi = parts.stats[at * 2], li = parts.stats[at * 2 + 1];
-      const float now = __builtin_elementwise_maximum(m, mi);
-      const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now), g = mi == now ? 1.0f : __builtin_amdgcn_exp2f(mi - now);
-      m = now;
-      l = l * f + li * g;
+    // Eight parts are loaded at once, the first eight without waiting for the lengths, which say how many there are.
+    constexpr int kBatch = 8;
+    for (int i0 = turn; i0 < (W > 1 ? count : kBatch); i0 += W * kBatch) {
+      float mi[kBatch], li[kBatch], xi[kBatch][N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[j] = x[j] * f + parts.sums[at * D + lane * N + j] * g;
+      for (int n = 0; n < kBatch; ++n) {
+        const int64_t at = part_of(c, parts, unit, kvh, std::min(i0 + n * W, parts.splits - 1)) * tile + r % tile;
+        mi[n] = parts.stats[at * 2];
+        li[n] = parts.stats[at * 2 + 1];
+#pragma unroll
+        for (int j = 0; j < N; ++j) xi[n][j] = parts.sums[at * D + lane * N + j];
+      }
+#pragma unroll
+      for (int n = 0; n < kBatch; ++n) {
+        const bool there = i0 + n * W < count;  // else it may hold anything
+        mi[n] = there ? mi[n] : -kInf;
+        const float now = __builtin_elementwise_maximum(m, mi[n]);
+        const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now), g = mi[n] == now ? 1.0f : __builtin_amdgcn_exp2f(mi[n] - now);
+        m = now;
+        l = l * f + (there ? li[n] * g : 0);
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = x[j] * f + (there ? xi[n][j] * g : 0);
+      }
     }
   }
   if constexpr (W > 1) {

@@ -92,19 +92,16 @@ def load():
     return lib
 
 
-def _packed(pack, *values):
-    try:
-        return pack(*values)
-    except (struct.error, OverflowError) as e:
-        raise ValueError("an argument is no number of its type: %s" % e) from None
-
-
 def _call(name, *args):
     if not _entry:
         load()
     code = _entry[name](*args)
     if code:
         raise KvError(name, code)
+
+
+def _unfit(e):
+    return ValueError("an argument is no number of its type: %s" % e)
 
 
 def _need(ok, why):
@@ -200,23 +197,18 @@ class Rotation:
             _need(len(t.shape) == 2 and tuple(t.shape) == tuple(cos.shape) and t.stride() == (t.shape[1], 1), "the tables are not [rows, pairs] and contiguous")
         sections = tuple(sections) if sections else (cos.shape[1],)
         _need(len(sections) <= MAX_AXES and sum(sections) == cos.shape[1] and min(sections) >= 0, "sections are not the pairs of the axes")
-        self.axes = len(sections)
-        self.sections = sections + (0,) * (MAX_AXES - len(sections))
-        self.rows, self.dim, self.interleaved = cos.shape[0], 2 * cos.shape[1], int(interleaved)
-        self.cos, self.sin = cos.data_ptr(), sin.data_ptr()
+        # as append() hands them over: addresses, rotary_dim, interleaved, rows, axes, sections
+        self.packed = (cos.data_ptr(), sin.data_ptr(), 2 * cos.shape[1], int(interleaved), cos.shape[0], len(sections),
+                       sections + (0,) * (MAX_AXES - len(sections)))
         self._keep = (cos, sin)
 
 
-def _rows(t, shape, kind, device, what):
-    """Strides of a tensor [tokens, heads, dim]."""
-    at = t.stride()
-    if t.shape != shape or at[2] != 1:
-        raise ValueError("%s is not [%d, %d, %d] with contiguous dims" % ((what,) + shape))
-    if _kind(t) != kind:
-        raise ValueError("%s has another type than the rows" % what)
-    if t.device != device:
-        raise ValueError("%s is on another device than the cache" % what)
-    return at
+def _refuse_rows(shape, dtype, device, **tensors):
+    """Says what is wrong with one of the tensors, which are to be `shape` with contiguous dims."""
+    for what, t in tensors.items():
+        _need(t.shape == shape and t.stride()[2] == 1, "%s is not [%d, %d, %d] with contiguous dims" % ((what,) + shape))
+        _need(t.dtype == dtype, "%s has another type than the other rows" % what)
+        _need(t.device == device, "%s is on another device than the cache" % what)
 
 
 def _heads(q):
@@ -228,40 +220,50 @@ def _heads(q):
 
 def append(cache, batch, k, v, q=None, q_out=None, rotation=None, positions=None, stream=0):
     """Rows k and v [tokens, heads, dim] into the cache, k rotated; q rotated into q_out."""
-    n, device, kind = batch.tokens, cache.device, _kind(k)
+    n, device, dtype = batch.tokens, cache.device, k.dtype
+    kind = _kinds.get(dtype)
+    if kind is None:
+        kind = _kind(k)
     if kind != BF16 and kind != F16:
         raise ValueError("k is not bfloat16 or float16")
     if batch.device != device:
         raise ValueError("the batch is on another device than the cache")
-    shape = (n, cache.heads, cache.dim)
-    ak, av = _rows(k, shape, kind, device, "k"), _rows(v, shape, kind, device, "v")
-    q_at = q_out_at = q_token = q_head = out_token = out_head = q_heads = 0
+    shape, k_at, v_at = (n, cache.heads, cache.dim), k.stride(), v.stride()
+    if (k.shape != shape or v.shape != shape or k_at[2] != 1 or v_at[2] != 1 or v.dtype != dtype or k.device != device
+            or v.device != device):
+        _refuse_rows(shape, dtype, device, k=k, v=v)
+    q_ptr = out_ptr = q_heads = 0
+    q_at = out_at = (0, 0)
     if q is not None:
         if q_out is None:
             raise ValueError("q without q_out")
         q_heads = _heads(q)
-        shape = (n, q_heads, cache.dim)
-        q_token, q_head, _ = _rows(q, shape, kind, device, "q")
-        out_token, out_head, _ = _rows(q_out, shape, kind, device, "q_out")
-        q_at, q_out_at = q.data_ptr(), q_out.data_ptr()
-    if rotation is None:
-        _need(positions is None, "positions without rotation")
-        a = _packed(_append_args, k.data_ptr(), v.data_ptr(), q_at, q_out_at, 0, 0, 0, ak[0], ak[1], av[0], av[1], q_token, q_head, out_token,
-                         out_head, 0, kind, q_heads, 0, 0, 0, 0, 0, 0, 0, 0)
-    else:
-        r, where, apart = rotation, 0, 0
-        if r.device != device:
+        shape, q_at, out_at = (n, q_heads, cache.dim), q.stride(), q_out.stride()
+        if (q.shape != shape or q_out.shape != shape or q_at[2] != 1 or out_at[2] != 1 or q.dtype != dtype or q_out.dtype != dtype
+                or q.device != device or q_out.device != device):
+            _refuse_rows(shape, dtype, device, q=q, q_out=q_out)
+        q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
+    cos = sin = where = apart = dim = interleaved = rows = axes = 0
+    sections = (0, 0, 0, 0)
+    if rotation is not None:
+        if rotation.device != device:
             raise ValueError("the rotation is on another device than the cache")
+        cos, sin, dim, interleaved, rows, axes, sections = rotation.packed
         if positions is not None:
             _is(positions, "int32", device, "positions")
             shape, at = tuple(positions.shape), positions.stride()
-            _need(shape == (r.axes, n) or (r.axes == 1 and shape == (n,)), "positions are not [axes, tokens]")
+            _need(shape == (axes, n) or (axes == 1 and shape == (n,)), "positions are not [axes, tokens]")
             _need(n < 2 or at[-1] == 1, "positions are not contiguous")
-            where, apart = positions.data_ptr(), at[0] if r.axes > 1 else n
-        elif r.axes > 1:
+            where, apart = positions.data_ptr(), at[0] if axes > 1 else n
+        elif axes > 1:
             raise ValueError("several axes need positions")
-        a = _packed(_append_args, k.data_ptr(), v.data_ptr(), q_at, q_out_at, r.cos, r.sin, where, ak[0], ak[1], av[0], av[1], q_token, q_head,
-                         out_token, out_head, apart, kind, q_heads, r.dim, r.interleaved, r.rows, r.axes, *r.sections)
+    elif positions is not None:
+        raise ValueError("positions without rotation")
+    try:
+        a = _append_args(k.data_ptr(), v.data_ptr(), q_ptr, out_ptr, cos, sin, where, k_at[0], k_at[1], v_at[0], v_at[1], q_at[0], q_at[1],
+                         out_at[0], out_at[1], apart, kind, q_heads, dim, interleaved, rows, axes, *sections)
+    except (struct.error, OverflowError) as e:
+        raise _unfit(e) from None
     _call("amem_kv_append", cache._ref, batch._ref, a, stream)
 
 
@@ -275,23 +277,31 @@ def attention_workspace(cache, batch, q_heads):
 def attention(cache, batch, q, out, lse=None, scale=None, causal=True, window=0, workspace=None, stream=0):
     """out [tokens, heads, dim] = attention of q over the cache; lse float32 [tokens, heads]; scale: dim ** -0.5 if None;
     workspace: a contiguous tensor of at least attention_workspace() bytes."""
-    n, dim, device, kind, heads = batch.tokens, cache.dim, cache.device, _kind(q), _heads(q)
+    n, dim, device, dtype, heads = batch.tokens, cache.dim, cache.device, q.dtype, _heads(q)
+    kind = _kinds.get(dtype)
+    if kind is None:
+        kind = _kind(q)
     if kind != BF16 and kind != F16:
         raise ValueError("q is not bfloat16 or float16")
     if batch.device != device:
         raise ValueError("the batch is on another device than the cache")
-    shape = (n, heads, dim)
-    aq, ao = _rows(q, shape, kind, device, "q"), _rows(out, shape, kind, device, "out")
-    lse_at = at = size = 0
+    shape, q_at, out_at = (n, heads, dim), q.stride(), out.stride()
+    if (q.shape != shape or out.shape != shape or q_at[2] != 1 or out_at[2] != 1 or out.dtype != dtype or q.device != device
+            or out.device != device):
+        _refuse_rows(shape, dtype, device, q=q, out=out)
+    lse_ptr = at = size = 0
     if lse is not None:
         _is(lse, "float32", device, "lse")
         if lse.shape != (n, heads) or not lse.is_contiguous():
             raise ValueError("lse is not [tokens, heads] and contiguous")
-        lse_at = lse.data_ptr()
+        lse_ptr = lse.data_ptr()
     if workspace is not None:
         if workspace.device != device or not workspace.is_contiguous():
             raise ValueError("workspace is on another device, or strided")
         at, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    a = _packed(_attention_args, q.data_ptr(), out.data_ptr(), lse_at, at, size, aq[0], aq[1], ao[0], ao[1],
-                        dim ** -0.5 if scale is None else scale, kind, heads, 1 if causal else 0, window, 0)
+    try:
+        a = _attention_args(q.data_ptr(), out.data_ptr(), lse_ptr, at, size, q_at[0], q_at[1], out_at[0], out_at[1],
+                            dim ** -0.5 if scale is None else scale, kind, heads, 1 if causal else 0, window, 0)
+    except (struct.error, OverflowError) as e:
+        raise _unfit(e) from None
     _call("amem_kv_attention", cache._ref, batch._ref, a, stream)
