@@ -47,7 +47,9 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
 
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   // heads first: their rows of a page are neighbours
-  const int group = a.q_heads / c.kv_heads, kvh = blockIdx.x % c.kv_heads, unit = blockIdx.x / c.kv_heads % few.units, split = blockIdx.x / c.kv_heads / few.units;
+  const int group = a.q_heads / c.kv_heads;
+  int kvh, unit, split;
+  pair_of(c, few, blockIdx.x, unit, kvh, split);
   KvSeq q;
   Unit u;
   if (!find_unit(b, a, group, 16 * NB, unit, q, u)) return;
@@ -371,7 +373,7 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
       lds_l[wave][n * 16 + lane] = l[n];
     }
   }
-  const int64_t part = part_of(c, few, unit, kvh, split);
+  const int64_t part = part_of(c, few, unit, kvh) + split;
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     __syncthreads();
@@ -436,12 +438,13 @@ void plan(const KvCache& c, const KvBatch& b, int group, int blocks, const KvAtt
   const int64_t all = (int64_t)few->units * c.kv_heads * span;
   const int64_t step = kWaves * 64, stretch = std::max<int64_t>((all + kTarget - 1) / kTarget, kLeast);
   few->splits = span > stretch ? (int)((span + stretch - 1) / stretch) : 1;
+  few->whole = few->splits > 1 ? 0 : few->units * c.kv_heads;
   few->stretch = (int)(((span + few->splits - 1) / few->splits + step - 1) / step * step);
 }
 
 template <int D, bool HALF, bool EIGHT, int NB>
 hipError_t launch_few(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& few, hipStream_t stream) {
-  const uint32_t grid = (uint32_t)few.units * c.kv_heads * few.splits;
+  const uint32_t grid = workgroups(c, few);
   if constexpr (!EIGHT) {
     if (c.page_shift < 4) attend_few<D, HALF, EIGHT, NB, false><<<grid, kWaves * kWave, 0, stream>>>(c, b, a, few);
     else attend_few<D, HALF, EIGHT, NB, true><<<grid, kWaves * kWave, 0, stream>>>(c, b, a, few);

@@ -63,14 +63,16 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   // heads first, so that the units of a head, which read the same keys, run on one die where heads are a multiple of eight;
   // the last units, which see most, before the others
-  const int group = a.q_heads / c.kv_heads, kvh = blockIdx.x % c.kv_heads;
-  const int unit = parts.units - 1 - blockIdx.x / c.kv_heads % parts.units, split = blockIdx.x / c.kv_heads / parts.units;
+  const int group = a.q_heads / c.kv_heads;
+  int kvh, unit, split;
+  pair_of(c, parts, blockIdx.x, unit, kvh, split);
   KvSeq q;
   Unit u;
   if (!find_unit(b, a, group, W * R, unit, q, u)) return;
   const int begin = u.from + split * parts.stretch;
   if (split && (begin >= u.to || q.bad)) return;
-  const int end = begin + parts.stretch < u.to ? begin + parts.stretch : u.to;
+  const int64_t cut = part_of(c, parts, unit, kvh);  // below zero: the unit's positions are not cut
+  const int end = cut >= 0 && begin + parts.stretch < u.to ? begin + parts.stretch : u.to;
   const int col = lane & (R - 1), part = lane / R;
   auto position_of = [&](int j) { return R == 32 ? j / 4 * 8 + part * 4 + j % 4 : j / 4 * 16 + part * 4 + j % 4; };
   auto dim_of = [&](int i, int e) { return R == 32 ? i * 32 + e / 4 * 8 + part * 4 + e % 4 : i * 16 + part * 4 + e; };
@@ -339,8 +341,8 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
   const float back = EIGHT ? __builtin_bit_cast(float, unit_scale & kExponent) : 1.0f;
   const int r = wave * R + col;
   if (r >= u.rows) return;
-  if (parts.splits > 1) {
-    const int64_t row = part_of(c, parts, unit, kvh, split) * (W * R) + r;
+  if (cut >= 0) {
+    const int64_t row = (cut + split) * (W * R) + r;
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
@@ -365,45 +367,65 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
     a.lse[(int64_t)(q.row + token) * a.q_heads + head] = q.bad ? __builtin_nanf("") : l == 0 ? -kInf : ((m - kLift) + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// Rows of a unit, and how a workgroup is made of waves. A tile's loads are shared by all of them: a chunk of 4096 over 16384
-// positions in e4m3 takes 1.035 ms with eight waves of 32 rows and 1.090 with four. Four where there would be less than two
-// workgroups of eight for each compute unit (2048 x 2048 positions, 32 heads over 8: 69 us, and 78 with eight), and for 64
-// dims of e4m3, where four load a tile at once. 256 dims leave a wave of 32 rows a SIMD for itself; eight of 16 rows, two a
-// SIMD, read LDS twice as often and are faster all the same: VMEASURE.
+// Rows of a unit, and how a workgroup is made of waves. A tile's loads are shared by all of them: a chunk of 4096 rows over 16384
+// positions (32 heads over 8, 128 dims, e4m3) takes 920 us with eight waves of 32 rows and 970 with four. Four where there would be
+// less than two workgroups of eight for each compute unit (2048 x 2048 positions: 69 us, and 78 with eight), and for 64
+// dims, where three workgroups of them fit (9000 x 9000 positions: 428 us, and 446 with eight). 256 dims leave a wave of 32 rows a
+// SIMD for itself; eight of 16 rows, two a SIMD, read LDS twice as often and are faster all the same: 2 x 3001 rows, a window of
+// 1024, 8 heads over one take 121 us, and 173 with four of 32.
 struct Shape {
   int rows, fit;   // of a unit; workgroups that fit at once
   bool eight;      // eight waves
 };
 Shape shape_of(const KvCache& c, const KvBatch& b, int group, int head_dim) {
   if (head_dim == 256) return {128, 256, true};
-  if (head_dim == 64 && c.block_shift) return {128, 512, false};
+  if (head_dim == 64) return {128, 768, false};
   if ((int64_t)units_of(b, group, 256) * c.kv_heads >= 512) return {256, 256, true};
   return {128, 512, false};
 }
 
-constexpr int kLeast = 512;  // positions of a workgroup, at least: a part costs its rows' sums written and read once more
+constexpr int kLeast = 512;  // positions of a stretch, about, at least
+// What parts cost, in positions: one more launch, and for 128 rows of a part their sums, written and read once more.
+constexpr int kJoin = 150, kPart = 1;
 
-// Contexts are cut only where units are fewer than fit at once, into stretches of the same length.
+// As many stretches as a context is cut into, at most.
+int most_splits(int64_t span) { return (int)((span + kLeast / 2) / kLeast); }
+
+// A round is as many workgroups as fit at once. What is cut is the last round, or the only one, where it is not full and units
+// see about as many positions each (else the last ones of a causal prompt, which are short, fill it): into as many stretches
+// of the same length as fill one round, or two, if that ends sooner. Uncut, and cut (us): 32 heads over 8, 128 dims, 16 bits, 1200
+// rows of 8192 positions 254 and 226; 4500 of 16384 1262 and 1062; 256 dims, 8 bits, 1100 rows of 16000 positions 1290 and 775.
 void plan(const KvCache& c, const KvBatch& b, int group, const Shape& shape, const KvAttend& a, Parts* parts) {
   parts->units = units_of(b, group, shape.rows);
   int64_t span = b.max_context;
   const int64_t seen = (int64_t)a.window + shape.rows / group + 1 + 64;
   if (a.causal && a.window && seen < span) span = seen;  // else a window has no far end
-  const int64_t all = (int64_t)parts->units * c.kv_heads * span;
-  const int64_t stretch = std::max<int64_t>((all + shape.fit - 1) / shape.fit, kLeast);
-  parts->splits = span > stretch ? (int)((span + stretch - 1) / stretch) : 1;
+  const int pairs = parts->units * c.kv_heads;
+  const bool even = !a.causal || a.window || 2 * (int64_t)a.max_tokens <= b.max_context;
+  const int last = pairs <= shape.fit ? pairs : even ? pairs % shape.fit : 0;
+  parts->splits = 1;
+  // what a number of workgroups takes, in thirds of the time of one that has its compute unit for itself: two take 4/3, three 5/3
+  auto thirds = [&](int count) { return count / shape.fit * (2 + shape.fit / 256) + (count % shape.fit ? 2 + (count % shape.fit + 255) / 256 : 0); };
+  int64_t least = thirds(last) * span;
+  for (int slots : {256, shape.fit, 2 * shape.fit}) {
+    const int splits = last ? std::min(slots / last, most_splits(span)) : 0;
+    if (splits < 2) continue;
+    const int64_t cost = thirds(last * splits) * (span / splits) + 3 * (kJoin + (int64_t)last * splits * (shape.rows / 128) * kPart);
+    if (cost >= least) continue;
+    least = cost;
+    parts->splits = splits;
+  }
+  parts->whole = parts->splits > 1 ? pairs - last : pairs;
   parts->stretch = (int)(((span + parts->splits - 1) / parts->splits + kTile - 1) / kTile * kTile);
 }
 
 template <int D, int W, int R>
 hipError_t launch_waves(const KvCache& c, const KvBatch& b, const KvAttend& a, bool half, bool eight, const Parts& parts, hipStream_t stream) {
-  const uint32_t grid = (uint32_t)parts.units * c.kv_heads * parts.splits;
+  const uint32_t grid = workgroups(c, parts);
   constexpr int kThreads = W * kWave;
   if (eight) {
-    if constexpr (D > 64 || W == 4) {
-      if (half) attend_many<D, true, true, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-      else attend_many<D, false, true, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
-    }
+    if (half) attend_many<D, true, true, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
+    else attend_many<D, false, true, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
   } else if (half) {
     attend_many<D, true, false, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
   } else {
@@ -417,6 +439,8 @@ template <int D>
 hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, bool half, bool eight, const Parts& parts, const Shape& shape, hipStream_t stream) {
   if constexpr (D == 256) {
     return launch_waves<D, 8, 16>(c, b, a, half, eight, parts, stream);
+  } else if constexpr (D == 64) {
+    return launch_waves<D, 4, 32>(c, b, a, half, eight, parts, stream);
   } else {
     if (shape.eight) return launch_waves<D, 8, 32>(c, b, a, half, eight, parts, stream);
     return launch_waves<D, 4, 32>(c, b, a, half, eight, parts, stream);
@@ -426,13 +450,11 @@ hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, bool ha
 }  // namespace
 
 uint64_t kv_attend_many_workspace(const KvCache& c, const KvBatch& b, int q_heads, int head_dim) {
-  // for any window: plan() has at most that many splits
+  // for any mask: plan() cuts at most a round, into at most two
   const int group = q_heads / c.kv_heads;
   const Shape shape = shape_of(c, b, group, head_dim);
-  const int64_t units = (int64_t)units_of(b, group, shape.rows) * c.kv_heads;
-  if (!units) return 0;
-  const int64_t splits = std::min<int64_t>((b.max_context + kLeast - 1) / kLeast, (shape.fit + units - 1) / units);
-  return splits < 2 ? 0 : (uint64_t)(units * splits * shape.rows) * (head_dim + 2) * 4;
+  const int64_t pairs = (int64_t)units_of(b, group, shape.rows) * c.kv_heads, splits = most_splits(b.max_context);
+  return splits < 2 ? 0 : (uint64_t)(std::min(std::min<int64_t>(pairs, shape.fit) * splits, 2 * (int64_t)shape.fit) * shape.rows) * (head_dim + 2) * 4;
 }
 
 hipError_t launch_kv_attend_many(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream) {
@@ -441,7 +463,7 @@ hipError_t launch_kv_attend_many(const KvCache& c, const KvBatch& b, const KvAtt
   Parts parts;
   plan(c, b, group, shape, a, &parts);
   parts.sums = (float*)a.workspace;
-  parts.stats = parts.sums + (int64_t)parts.units * c.kv_heads * parts.splits * shape.rows * head_dim;
+  parts.stats = parts.sums + (int64_t)(parts.units * c.kv_heads - parts.whole) * parts.splits * shape.rows * head_dim;
   if (head_dim == 64) return launch<64>(c, b, a, half, eight, parts, shape, stream);
   if (head_dim == 128) return launch<128>(c, b, a, half, eight, parts, shape, stream);
   return launch<256>(c, b, a, half, eight, parts, shape, stream);

@@ -26,9 +26,15 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void join_stretches(KvCache c, 
     q = kv_seq(b, s);
     mine = row >= q.row && row < q.row + q.n;
   }
+  int r = 0;
+  int64_t first = 0;
   if (mine) {
-    const int r = (row - q.row) * group + head % group;
+    r = (row - q.row) * group + head % group;
     const int unit = (b.cu_tokens ? kv_unit_base(b, s, tile, 1, group) : s * ((b.uniform * group - 1) / tile + 1)) + r / tile;
+    first = part_of(c, parts, unit, kvh);
+    mine = first >= 0;  // else the unit's positions were not cut
+  }
+  if (mine) {
     unit_at(b, a, group, tile, s, r / tile, q, u);
     int count = (u.to - u.from + parts.stretch - 1) / parts.stretch;
     count = q.bad || count < 1 ? 1 : count > parts.splits ? parts.splits : count;
@@ -38,7 +44,7 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void join_stretches(KvCache c, 
       float mi[kBatch], li[kBatch], xi[kBatch][N];
 #pragma unroll
       for (int n = 0; n < kBatch; ++n) {
-        const int64_t at = part_of(c, parts, unit, kvh, std::min(i0 + n * W, parts.splits - 1)) * tile + r % tile;
+        const int64_t at = (first + std::min(i0 + n * W, parts.splits - 1)) * tile + r % tile;
         mi[n] = parts.stats[at * 2];
         li[n] = parts.stats[at * 2 + 1];
 #pragma unroll
@@ -83,7 +89,13 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void join_stretches(KvCache c, 
 
 template <int D, bool HALF>
 hipError_t join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int tile, float lift, hipStream_t stream) {
-  const int rows = b.tokens * a.q_heads;
+  // the units that are cut are the first ones; without cu_tokens it is known which tokens they have
+  int tokens = b.tokens;
+  if (!b.cu_tokens) {
+    const int group = a.q_heads / c.kv_heads, each = (b.uniform * group - 1) / tile + 1, unit = parts.units - 1 - parts.whole / c.kv_heads;
+    tokens = unit / each * b.uniform + (int)std::min<int64_t>(b.uniform, ((int64_t)(unit % each + 1) * tile + group - 1) / group);
+  }
+  const int rows = tokens * a.q_heads;
   if (parts.splits > 8) join_stretches<D, HALF, kJoinWaves><<<rows, kJoinWaves * kWave, 0, stream>>>(c, b, a, parts, tile, lift);
   else join_stretches<D, HALF, 1><<<(rows + kJoinWaves - 1) / kJoinWaves, kJoinWaves * kWave, 0, stream>>>(c, b, a, parts, tile, lift);
   return hipGetLastError();

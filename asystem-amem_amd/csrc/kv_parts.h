@@ -10,9 +10,11 @@ namespace amem {
 struct Parts {
   int stretch;   // positions of a workgroup, a multiple of 64
   int units;
-  int splits;    // most stretches of a unit
-  float* sums;   // [unit][kv head][split][row][dim]
-  float* stats;  // [unit][kv head][split][row]{m, l}, m in units of log 2
+  // Pairs of a unit and a kv head are numbered heads first and the last units first. The first `whole` of them are not cut, each of
+  // the others is, into at most `splits` stretches.
+  int whole, splits;
+  float* sums;   // [pair - whole][split][row][dim]
+  float* stats;  // [pair - whole][split][row]{m, l}, m in units of log 2
 };
 
 namespace {
@@ -59,9 +61,22 @@ __device__ __forceinline__ bool find_unit(const KvBatch& b, const KvAttend& a, i
   return unit_at(b, a, group, tile, s, index, q, u);
 }
 
-// Where a stretch's part of a unit is kept.
-__device__ __forceinline__ int64_t part_of(const KvCache& c, const Parts& parts, int unit, int kvh, int split) {
-  return ((int64_t)unit * c.kv_heads + kvh) * parts.splits + split;
+// The pair and the stretch that workgroup `index` has.
+__device__ __forceinline__ void pair_of(const KvCache& c, const Parts& parts, int index, int& unit, int& kvh, int& split) {
+  const int cut = parts.units * c.kv_heads - parts.whole;
+  split = index < parts.whole ? 0 : (index - parts.whole) / cut;
+  const int pair = index < parts.whole ? index : parts.whole + (index - parts.whole) % cut;
+  unit = parts.units - 1 - pair / c.kv_heads;
+  kvh = pair % c.kv_heads;
+}
+
+// Where the part of a pair's first stretch is kept, those of the others behind it; below zero if the pair is not cut.
+__device__ __forceinline__ int64_t part_of(const KvCache& c, const Parts& parts, int unit, int kvh) {
+  return ((int64_t)(parts.units - 1 - unit) * c.kv_heads + kvh - parts.whole) * parts.splits;
+}
+
+inline uint32_t workgroups(const KvCache& c, const Parts& parts) {
+  return (uint32_t)parts.whole + (uint32_t)(parts.units * c.kv_heads - parts.whole) * parts.splits;
 }
 
 inline int units_of(const KvBatch& b, int group, int tile) {

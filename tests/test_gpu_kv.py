@@ -428,6 +428,24 @@ def test_attention_many_sequences(arena, kind, eight, dim):
     assert np.isnan(rows[first:]).all() and np.isfinite(rows[:first]).all()
 
 
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 1000), (False, 0)])
+@pytest.mark.parametrize("dim,sequences,tokens,eight,uniform", [(256, 33, 40, False, True), (256, 33, 40, True, False), (128, 65, 40, True, True),
+                                                                (128, 40, 130, False, True), (64, 100, 40, True, True)])
+def test_attention_last_round_is_cut(gpu, dim, sequences, tokens, eight, uniform, causal, window):
+    """More workgroups than fit at once, and a few more: those (the first sequences') are cut into stretches, the others are not."""
+    big = Arena(gpu, 512 << 20)
+    try:
+        lengths = [(tokens, tokens + i % 50) for i in range(sequences)]
+        lengths[0], lengths[1], lengths[sequences - 1] = (tokens, 1600), (tokens, 700), (tokens, 1100)
+        if not uniform:
+            lengths[2], lengths[5] = (3, 1500), (0, 9)
+        case = Case(big, lengths, dim=dim, q_heads=8, kv_heads=8, eight=eight, page=32, block=32, uniform=uniform, seed=27).upload()
+        got, lse = check_attend(case, case.rows(8), causal, window, sequences=[0, 1, 2, 3, 5, 6, sequences // 2, sequences - 1])
+        assert np.isfinite(O.decode(got, case.kind)).all() and np.isfinite(lse).all()
+    finally:
+        big.free()
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 8.0])
 def test_attention_scales(arena, scale):
     """From weights that are all equal to a single one."""
