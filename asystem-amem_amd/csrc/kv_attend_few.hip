@@ -19,8 +19,6 @@ namespace amem {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kLeast = 256;   // positions of a workgroup, at least: shorter ones and no join would both be slower, down to a context of 500
-constexpr int kTarget = 512;  // workgroups that a call is cut into, where its contexts are long enough
 
 // Whether a wave has a SIMD, and all of its registers, to itself: where two would spill.
 template <int D, bool EIGHT, int NB>
@@ -54,8 +52,9 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
   Unit u;
   if (!find_unit(b, a, group, 16 * NB, unit, q, u)) return;
   const int begin = u.from + split * few.stretch;
+  const int64_t part = part_of(c, few, unit, kvh) + split;  // below zero: the unit's positions are not cut
   if (split && (begin >= u.to || q.bad)) return;
-  const int end = begin + few.stretch < u.to ? begin + few.stretch : u.to;
+  const int end = part >= 0 && begin + few.stretch < u.to ? begin + few.stretch : u.to;
   const int col = lane & 15, quad = lane >> 4;
 
   // Queries, the operand of a block of rows: dims in the order of the keys' operand. More than one block leaves no registers
@@ -373,7 +372,6 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
       lds_l[wave][n * 16 + lane] = l[n];
     }
   }
-  const int64_t part = part_of(c, few, unit, kvh) + split;
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     __syncthreads();
@@ -402,7 +400,7 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
         ll += lds_l[i][n * 16 + r] * (mi == mm ? 1.0f : __builtin_amdgcn_exp2f(mi - mm));
         x += *(const f32x4*)((const float*)lds + (i * 16 + r) * (D + 4) + d);
       }
-      if (few.splits > 1) {
+      if (part >= 0) {
         const int64_t row = part * (16 * NB) + n * 16 + r;
         *(f32x4*)(few.sums + row * D + d) = x;
         if (d == 0) {
@@ -429,17 +427,21 @@ int blocks_of(int group, int max_tokens, int head_dim) {
   return rows <= 16 ? 1 : rows <= 32 || head_dim > 64 ? 2 : rows <= 48 ? 3 : 4;
 }
 
-// Stretches of the same length, as long as leaves about kTarget workgroups, and at least kLeast positions.
-void plan(const KvCache& c, const KvBatch& b, int group, int blocks, const KvAttend& a, Parts* few) {
+// Workgroups are bound by what a compute unit can load, or all of them by the memory. The figures are fitted to times of 25
+// calls with 1 to 32 stretches (8 to 512 pairs, contexts of 2000 to 131072, equal and not), 4 % above the best on average. Uncut, and
+// cut (us): 128 dims of e4m3, 33 sequences of 1000 to 4000 positions 50 and 44; 65 of 4000 126 and 102; 3 of 30000 270 and 40.
+Cut cut_of(int head_dim, bool eight, int blocks) {
+  const int fit = head_dim == 256 && (!eight || blocks > 1) ? 256 : head_dim == 64 && !eight && blocks == 1 ? 768 : 512;
+  const int bytes = head_dim * (eight ? 2 : 4);  // of a position
+  return {fit, 4, 2, 256, 256, 37, 39, 33, 79, 5500 / bytes, 12000 / bytes, 34 * blocks * (head_dim + 2) / bytes};
+}
+
+void plan(const KvCache& c, const KvBatch& b, int group, int head_dim, bool eight, int blocks, const KvAttend& a, Parts* few) {
   int64_t span = b.max_context;
   const int64_t seen = (int64_t)a.window + (16 * blocks) / group + 1 + 64;
   if (a.causal && a.window && seen < span) span = seen;  // else a window has no far end
   few->units = units_of(b, group, 16 * blocks);
-  const int64_t all = (int64_t)few->units * c.kv_heads * span;
-  const int64_t step = kWaves * 64, stretch = std::max<int64_t>((all + kTarget - 1) / kTarget, kLeast);
-  few->splits = span > stretch ? (int)((span + stretch - 1) / stretch) : 1;
-  few->whole = few->splits > 1 ? 0 : few->units * c.kv_heads;
-  few->stretch = (int)(((span + few->splits - 1) / few->splits + step - 1) / step * step);
+  cut_last_round(cut_of(head_dim, eight, blocks), few->units * c.kv_heads, span, true, few);
 }
 
 template <int D, bool HALF, bool EIGHT, int NB>
@@ -472,20 +474,16 @@ hipError_t launch_dims(const KvCache& c, const KvBatch& b, const KvAttend& a, bo
 }  // namespace
 
 uint64_t kv_attend_few_workspace(const KvCache& c, const KvBatch& b, int q_heads, int max_tokens, int head_dim) {
-  // for any window: plan() has at most that many splits
   const int group = q_heads / c.kv_heads, blocks = blocks_of(group, max_tokens, head_dim);
-  const int64_t units = (int64_t)units_of(b, group, 16 * blocks) * c.kv_heads;
-  if (!units) return 0;
-  const int64_t splits = std::min<int64_t>((b.max_context + kLeast - 1) / kLeast, (kTarget + units - 1) / units);
-  return splits < 2 ? 0 : (uint64_t)(units * splits * (16 * blocks)) * (head_dim + 2) * 4;
+  return parts_bytes(cut_of(head_dim, c.block_shift > 0, blocks), (int64_t)units_of(b, group, 16 * blocks) * c.kv_heads, b.max_context, 16 * blocks, head_dim);
 }
 
 hipError_t launch_kv_attend_few(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream) {
   const int group = a.q_heads / c.kv_heads, blocks = blocks_of(group, a.max_tokens, head_dim);
   Parts few;
-  plan(c, b, group, blocks, a, &few);
+  plan(c, b, group, head_dim, eight, blocks, a, &few);
   few.sums = (float*)a.workspace;
-  few.stats = few.sums + (int64_t)few.units * c.kv_heads * few.splits * (16 * blocks) * head_dim;
+  few.stats = few.sums + (int64_t)(few.units * c.kv_heads - few.whole) * few.splits * (16 * blocks) * head_dim;
   if (head_dim == 64) return launch_dims<64>(c, b, a, half, eight, few, blocks, stream);
   if (head_dim == 128) return launch_dims<128>(c, b, a, half, eight, few, blocks, stream);
   return launch_dims<256>(c, b, a, half, eight, few, blocks, stream);

@@ -384,39 +384,19 @@ Shape shape_of(const KvCache& c, const KvBatch& b, int group, int head_dim) {
   return {128, 512, false};
 }
 
-constexpr int kLeast = 512;  // positions of a stretch, about, at least
-// What parts cost, in positions: one more launch, and for 128 rows of a part their sums, written and read once more.
-constexpr int kJoin = 150, kPart = 1;
+// Two workgroups of a compute unit take 4/3 of the time of one, three 5/3; a part of 128 rows costs about a position's work
+// once all compute units write theirs. Uncut, and cut (us): 32 heads over 8, 128 dims, 16 bits, 1200 rows of 8192 positions 254 and
+// 226; 4500 of 16384 1262 and 1062; 256 dims, 8 bits, 1100 rows of 16000 positions 1290 and 775.
+Cut cut_of(const Shape& shape) { return {shape.fit, 2, 0, 512, kTile, 66, 33, 0, 100, 0, 150, shape.rows * 100 / 128}; }
 
-// As many stretches as a context is cut into, at most.
-int most_splits(int64_t span) { return (int)((span + kLeast / 2) / kLeast); }
-
-// A round is as many workgroups as fit at once. What is cut is the last round, or the only one, where it is not full and units
-// see about as many positions each (else the last ones of a causal prompt, which are short, fill it): into as many stretches
-// of the same length as fill one round, or two, if that ends sooner. Uncut, and cut (us): 32 heads over 8, 128 dims, 16 bits, 1200
-// rows of 8192 positions 254 and 226; 4500 of 16384 1262 and 1062; 256 dims, 8 bits, 1100 rows of 16000 positions 1290 and 775.
 void plan(const KvCache& c, const KvBatch& b, int group, const Shape& shape, const KvAttend& a, Parts* parts) {
   parts->units = units_of(b, group, shape.rows);
   int64_t span = b.max_context;
   const int64_t seen = (int64_t)a.window + shape.rows / group + 1 + 64;
   if (a.causal && a.window && seen < span) span = seen;  // else a window has no far end
-  const int pairs = parts->units * c.kv_heads;
+  // the last rows of a prompt see more than the first ones
   const bool even = !a.causal || a.window || 2 * (int64_t)a.max_tokens <= b.max_context;
-  const int last = pairs <= shape.fit ? pairs : even ? pairs % shape.fit : 0;
-  parts->splits = 1;
-  // what a number of workgroups takes, in thirds of the time of one that has its compute unit for itself: two take 4/3, three 5/3
-  auto thirds = [&](int count) { return count / shape.fit * (2 + shape.fit / 256) + (count % shape.fit ? 2 + (count % shape.fit + 255) / 256 : 0); };
-  int64_t least = thirds(last) * span;
-  for (int slots : {256, shape.fit, 2 * shape.fit}) {
-    const int splits = last ? std::min(slots / last, most_splits(span)) : 0;
-    if (splits < 2) continue;
-    const int64_t cost = thirds(last * splits) * (span / splits) + 3 * (kJoin + (int64_t)last * splits * (shape.rows / 128) * kPart);
-    if (cost >= least) continue;
-    least = cost;
-    parts->splits = splits;
-  }
-  parts->whole = parts->splits > 1 ? pairs - last : pairs;
-  parts->stretch = (int)(((span + parts->splits - 1) / parts->splits + kTile - 1) / kTile * kTile);
+  cut_last_round(cut_of(shape), parts->units * c.kv_heads, span, even, parts);
 }
 
 template <int D, int W, int R>
@@ -450,11 +430,9 @@ hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, bool ha
 }  // namespace
 
 uint64_t kv_attend_many_workspace(const KvCache& c, const KvBatch& b, int q_heads, int head_dim) {
-  // for any mask: plan() cuts at most a round, into at most two
   const int group = q_heads / c.kv_heads;
   const Shape shape = shape_of(c, b, group, head_dim);
-  const int64_t pairs = (int64_t)units_of(b, group, shape.rows) * c.kv_heads, splits = most_splits(b.max_context);
-  return splits < 2 ? 0 : (uint64_t)(std::min(std::min<int64_t>(pairs, shape.fit) * splits, 2 * (int64_t)shape.fit) * shape.rows) * (head_dim + 2) * 4;
+  return parts_bytes(cut_of(shape), (int64_t)units_of(b, group, shape.rows) * c.kv_heads, b.max_context, shape.rows, head_dim);
 }
 
 hipError_t launch_kv_attend_many(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream) {

@@ -446,6 +446,23 @@ def test_attention_last_round_is_cut(gpu, dim, sequences, tokens, eight, uniform
         big.free()
 
 
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 1000), (False, 0)])
+@pytest.mark.parametrize("dim,sequences,tokens,kind,eight,uniform", [(256, 33, 1, "bf16", False, True), (256, 65, 2, "f16", True, False), (128, 65, 1, "bf16", True, True),
+                                                                     (128, 70, 3, "bf16", False, False), (64, 97, 1, "f16", False, True), (128, 33, 1, "bf16", True, True)])
+def test_attention_last_round_of_few_rows_is_cut(gpu, dim, sequences, tokens, kind, eight, uniform, causal, window):
+    big = Arena(gpu, 512 << 20)
+    try:
+        lengths = [(tokens, tokens + 7 * i % 200) for i in range(sequences)]
+        lengths[0], lengths[1], lengths[sequences - 1] = (tokens, 2600), (tokens, 700), (tokens, 2100)
+        if not uniform:
+            lengths[2], lengths[5] = (1, 1500), (0, 9)
+        case = Case(big, lengths, dim=dim, q_heads=16, kv_heads=8, kind=kind, eight=eight, page=32, block=32, uniform=uniform, seed=28).upload()
+        got, lse = check_attend(case, case.rows(16), causal, window, sequences=[0, 1, 2, 3, 5, 6, sequences // 2, sequences - 1])
+        assert np.isfinite(O.decode(got, case.kind)).all() and np.isfinite(lse).all()
+    finally:
+        big.free()
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 8.0])
 def test_attention_scales(arena, scale):
     """From weights that are all equal to a single one."""
