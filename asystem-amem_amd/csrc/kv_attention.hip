@@ -7,97 +7,94 @@
 namespace amem {
 namespace {
 
-constexpr int kJoinWaves = 4;
+constexpr int kJoinThreads = 256;
 
-// Joins the stretches of a row and query head: W waves take the stretches in turn (one wave where they are few, since then
-// rows are many).
-template <int D, bool HALF, int W>
-__global__ __launch_bounds__(kJoinWaves * kWave) void join_stretches(KvCache c, KvBatch b, KvAttend a, Parts parts, int tile, float lift) {
-  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int index = blockIdx.x * (kJoinWaves / W) + wave / W, turn = wave % W;
-  const int row = index / a.q_heads, head = index % a.q_heads, group = a.q_heads / c.kv_heads, kvh = head / group;
-  constexpr int N = D / kWave;
-  float m = -kInf, l = 0, x[N] = {};
+// Joins the stretches of the pairs that were cut. A thread has four dims of a row, or W threads have, which take the stretches in
+// turn; B parts are loaded at once, the first of them before the lengths are known, which say how many there are, where all units have
+// as many rows. `rows`: those that a unit can have.
+template <int D, bool HALF, int W, int B>
+__global__ __launch_bounds__(kJoinThreads) void join_stretches(KvCache c, KvBatch b, KvAttend a, Parts parts, int tile, int rows, float lift) {
+  constexpr int kItems = kJoinThreads / W;
+  const int blocks = (rows * (D / 4) + kItems - 1) / kItems, pair = blockIdx.x / blocks, turn = threadIdx.x / kItems;
+  const int item = blockIdx.x % blocks * kItems + threadIdx.x % kItems, r = item / (D / 4), d = item % (D / 4) * 4;
+  const int64_t first = (int64_t)pair * parts.splits;
+  float m = -kInf, l = 0;
+  f32x4 x = {0, 0, 0, 0}, xi[B];
+  f32x2 si[B];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int n = 0; n < B; ++n) {
+      const int64_t at = (first + std::min(i0 + n * W, parts.splits - 1)) * tile + r;
+      si[n] = *(const f32x2*)(parts.stats + at * 2);
+      xi[n] = *(const f32x4*)(parts.sums + at * D + d);
+    }
+  };
+  if (!b.cu_tokens) load(turn);
+  const int group = a.q_heads / c.kv_heads;
+  int unit, kvh, split;
+  pair_of(c, parts, parts.whole + pair, unit, kvh, split);
   KvSeq q;
   Unit u;
-  const int s = row >= b.tokens ? -1 : b.cu_tokens ? find_sequence(b, row, 1, 0) : row / b.uniform;
-  bool mine = s >= 0;
+  const bool mine = find_unit(b, a, group, tile, unit, q, u) && r < u.rows;
   if (mine) {
-    q = kv_seq(b, s);
-    mine = row >= q.row && row < q.row + q.n;
-  }
-  int r = 0;
-  int64_t first = 0;
-  if (mine) {
-    r = (row - q.row) * group + head % group;
-    const int unit = (b.cu_tokens ? kv_unit_base(b, s, tile, 1, group) : s * ((b.uniform * group - 1) / tile + 1)) + r / tile;
-    first = part_of(c, parts, unit, kvh);
-    mine = first >= 0;  // else the unit's positions were not cut
-  }
-  if (mine) {
-    unit_at(b, a, group, tile, s, r / tile, q, u);
+    if (b.cu_tokens) load(turn);
     int count = (u.to - u.from + parts.stretch - 1) / parts.stretch;
     count = q.bad || count < 1 ? 1 : count > parts.splits ? parts.splits : count;
-    // Eight parts are loaded at once, the first eight without waiting for the lengths, which say how many there are.
-    constexpr int kBatch = 8;
-    for (int i0 = turn; i0 < (W > 1 ? count : kBatch); i0 += W * kBatch) {
-      float mi[kBatch], li[kBatch], xi[kBatch][N];
+    for (int i0 = turn;;) {
 #pragma unroll
-      for (int n = 0; n < kBatch; ++n) {
-        const int64_t at = (first + std::min(i0 + n * W, parts.splits - 1)) * tile + r % tile;
-        mi[n] = parts.stats[at * 2];
-        li[n] = parts.stats[at * 2 + 1];
-#pragma unroll
-        for (int j = 0; j < N; ++j) xi[n][j] = parts.sums[at * D + lane * N + j];
-      }
-#pragma unroll
-      for (int n = 0; n < kBatch; ++n) {
+      for (int n = 0; n < B; ++n) {
         const bool there = i0 + n * W < count;  // else it may hold anything
-        mi[n] = there ? mi[n] : -kInf;
-        const float now = __builtin_elementwise_maximum(m, mi[n]);
-        const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now), g = mi[n] == now ? 1.0f : __builtin_amdgcn_exp2f(mi[n] - now);
+        const float mi = there ? si[n][0] : -kInf, now = __builtin_elementwise_maximum(m, mi);
+        const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now), g = mi == now ? 1.0f : __builtin_amdgcn_exp2f(mi - now);
         m = now;
-        l = l * f + (there ? li[n] * g : 0);
+        l = l * f + (there ? si[n][1] * g : 0);
 #pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = x[j] * f + (there ? xi[n][j] * g : 0);
+        for (int j = 0; j < 4; ++j) x[j] = x[j] * f + (there ? xi[n][j] * g : 0);
       }
+      i0 += W * B;
+      if (i0 >= count) break;
+      load(i0);
     }
   }
   if constexpr (W > 1) {
-    __shared__ float part[W][D], stat[W][2];
-#pragma unroll
-    for (int j = 0; j < N; ++j) part[turn][lane * N + j] = x[j];
-    if (lane == 0) { stat[turn][0] = m; stat[turn][1] = l; }
+    __shared__ f32x4 part[W][kItems];
+    __shared__ f32x2 stat[W][kItems];
+    part[turn][threadIdx.x % kItems] = x;
+    stat[turn][threadIdx.x % kItems] = f32x2{m, l};
     __syncthreads();
     if (turn) return;
 #pragma unroll
     for (int i = 1; i < W; ++i) {
-      const float mi = stat[i][0], now = __builtin_elementwise_maximum(m, mi);
-      const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now), g = mi == now ? 1.0f : __builtin_amdgcn_exp2f(mi - now);
+      const f32x2 s = stat[i][threadIdx.x];
+      const f32x4 y = part[i][threadIdx.x];
+      const float now = __builtin_elementwise_maximum(m, s[0]);
+      const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now), g = s[0] == now ? 1.0f : __builtin_amdgcn_exp2f(s[0] - now);
       m = now;
-      l = l * f + stat[i][1] * g;
+      l = l * f + s[1] * g;
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[j] = x[j] * f + part[i][lane * N + j] * g;
+      for (int j = 0; j < 4; ++j) x[j] = x[j] * f + y[j] * g;
     }
   }
   if (!mine) return;
-  uint16_t* at = a.out + row * a.out_token + head * a.out_head + lane * N;
-#pragma unroll
-  for (int j = 0; j < N; ++j) at[j] = from_float<HALF>(q.bad ? __builtin_nanf("") : l == 0 ? 0.0f : x[j] / l);
-  if (a.lse && lane == 0) a.lse[(int64_t)row * a.q_heads + head] = q.bad ? __builtin_nanf("") : l == 0 ? -kInf : ((m - lift) + __builtin_amdgcn_logf(l)) * kLn2;
+  const int token = (u.first + r) / group, head = kvh * group + (u.first + r) % group;
+  if (q.bad || l == 0) {
+    x = f32x4{0, 0, 0, 0};
+    l = q.bad ? __builtin_nanf("") : 0;
+  }
+  const float inverse = l == 0 ? 0.0f : 1.0f / l;
+  *(u32x2*)(a.out + (q.row + token) * a.out_token + head * a.out_head + d) =
+      u32x2{pack<HALF>(x[0] * inverse, x[1] * inverse), pack<HALF>(x[2] * inverse, x[3] * inverse)};
+  if (a.lse && d == 0) a.lse[(int64_t)(q.row + token) * a.q_heads + head] = l == 0 ? -kInf : ((m - lift) + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 template <int D, bool HALF>
 hipError_t join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int tile, float lift, hipStream_t stream) {
-  // the units that are cut are the first ones; without cu_tokens it is known which tokens they have
-  int tokens = b.tokens;
-  if (!b.cu_tokens) {
-    const int group = a.q_heads / c.kv_heads, each = (b.uniform * group - 1) / tile + 1, unit = parts.units - 1 - parts.whole / c.kv_heads;
-    tokens = unit / each * b.uniform + (int)std::min<int64_t>(b.uniform, ((int64_t)(unit % each + 1) * tile + group - 1) / group);
-  }
-  const int rows = tokens * a.q_heads;
-  if (parts.splits > 8) join_stretches<D, HALF, kJoinWaves><<<rows, kJoinWaves * kWave, 0, stream>>>(c, b, a, parts, tile, lift);
-  else join_stretches<D, HALF, 1><<<(rows + kJoinWaves - 1) / kJoinWaves, kJoinWaves * kWave, 0, stream>>>(c, b, a, parts, tile, lift);
+  const int pairs = parts.units * c.kv_heads - parts.whole;
+  const int rows = b.cu_tokens ? tile : (int)std::min<int64_t>(tile, (int64_t)b.uniform * (a.q_heads / c.kv_heads)), items = rows * (D / 4);
+  auto blocks = [&](int each) { return pairs * ((items + each - 1) / each); };
+  if (parts.splits > 8) join_stretches<D, HALF, 4, 8><<<blocks(kJoinThreads / 4), kJoinThreads, 0, stream>>>(c, b, a, parts, tile, rows, lift);
+  else if (parts.splits > 4) join_stretches<D, HALF, 1, 8><<<blocks(kJoinThreads), kJoinThreads, 0, stream>>>(c, b, a, parts, tile, rows, lift);
+  else join_stretches<D, HALF, 1, 4><<<blocks(kJoinThreads), kJoinThreads, 0, stream>>>(c, b, a, parts, tile, rows, lift);
   return hipGetLastError();
 }
 
