@@ -45,8 +45,9 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
   constexpr int kRowsAPass = kThreads / kRowLanes;
   constexpr int kPasses = kTile / kRowsAPass;
   static_assert(kRowsAPass <= kTile, "a pass is at most a tile");
-  // pads: the rows that are read together are on different banks
-  constexpr int kKeyPitch = D * 2 + 16, kValuePitch = D * 2 + 2 * R, kBuffer = kTile * (kKeyPitch + kValuePitch);
+  // pads: the rows that are read together are on different banks (keys of 256 dims: 674 us with 32 bytes, 773 with 16, 780 with 64, at
+  // 1100 rows of 16000 positions in e4m3; of 128 dims 16 and 32 differ by 1 %)
+  constexpr int kKeyPitch = D * 2 + (R == 32 ? 16 : 32), kValuePitch = D * 2 + 2 * R, kBuffer = kTile * (kKeyPitch + kValuePitch);
   constexpr bool kHalfP = EIGHT || HALF;  // weights are fp16 where the values' type allows it
   // fp16 weights are held 2^8 times larger, which keeps small ones out of the subnormal numbers
   constexpr float kLift = kHalfP ? 8.0f : 0.0f;
@@ -372,7 +373,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
 // less than two workgroups of eight for each compute unit (2048 x 2048 positions: 69 us, and 78 with eight), and for 64
 // dims, where three workgroups of them fit (9000 x 9000 positions: 428 us, and 446 with eight). 256 dims leave a wave of 32 rows a
 // SIMD for itself; eight of 16 rows, two a SIMD, read LDS twice as often and are faster all the same: 2 x 3001 rows, a window of
-// 1024, 8 heads over one take 121 us, and 173 with four of 32.
+// 1024, 8 heads over one took 121 us, and 173 with four of 32.
 struct Shape {
   int rows, fit;   // of a unit; workgroups that fit at once
   bool eight;      // eight waves
@@ -386,7 +387,7 @@ Shape shape_of(const KvCache& c, const KvBatch& b, int group, int head_dim) {
 
 // Two workgroups of a compute unit take 4/3 of the time of one, three 5/3; a part of 128 rows costs about a position's work
 // once all compute units write theirs. Uncut, and cut (us): 32 heads over 8, 128 dims, 16 bits, 1200 rows of 8192 positions 254 and
-// 226; 4500 of 16384 1262 and 1062; 256 dims, 8 bits, 1100 rows of 16000 positions 1290 and 775.
+// 226; 4500 of 16384 1262 and 1062; 256 dims, 8 bits, 1100 rows of 16000 positions 1290 and 674.
 Cut cut_of(const Shape& shape) { return {shape.fit, 2, 0, 512, kTile, 66, 33, 0, 100, 0, 150, shape.rows * 100 / 128}; }
 
 void plan(const KvCache& c, const KvBatch& b, int group, const Shape& shape, const KvAttend& a, Parts* parts) {
