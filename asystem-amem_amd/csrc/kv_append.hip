@@ -5,6 +5,10 @@
 // All of it moves bytes: a row is read once and written once, in one launch for keys, values and queries. An item of work
 // is 16 dims of one head of one row, as two vectors of eight elements that hold both members of eight pairs, so that
 // a lane turns them by itself and reads eight neighbouring cosines and sines, once for all the heads that it takes.
+//
+// Measured, where a large copy moves 4.9 TB/s: up to 2500 rows of six sequences, 32 heads over 4, 64 dims, half of them turned, fp16: 112 MB
+// in 24 us, 4.7 TB/s; 2 x 8192 rows, 64 heads over 8, 128 dims, three axes, e4m3: 395 MB in 94 us, 4.2 TB/s; the single tokens of 128
+// sequences, e4m3: 8 us; one row 4.5 us, about what a launch takes.
 #include <algorithm>
 
 #include "kv_device.h"
@@ -339,7 +343,8 @@ __global__ __launch_bounds__(kThreads) void append8(KvCache c, KvBatch b, KvAppe
 hipError_t launch_kv_append(const KvCache& c, const KvBatch& b, const KvAppend& a, int head_dim, bool half, bool eight, hipStream_t stream) {
   const int items = head_dim / 16, heads = a.q_heads + (eight ? 0 : 2 * c.kv_heads);
   // A wave takes all heads of a row where rows are many, since its angles serve them all; with fewer rows up to as many
-  // waves as have four heads for each lane share them, until there are about 4096.
+  // waves as have four heads for each lane share them, until there are about 4096. One wave a row and that many (us; 64 heads over 8,
+  // 128 dims, 16 bits): one row 7.7 and 5.2, 500 rows 10.4 and 8.0, 4000 rows 36 and 35.
   const int most = (heads * items + 4 * kWave - 1) / (4 * kWave);
   const int shares = std::max(1, std::min(most, 4096 / std::max(1, b.tokens)));
   const int row_groups = heads ? (int)(((int64_t)b.tokens * shares + kWaves - 1) / kWaves) : 0;
@@ -349,7 +354,9 @@ hipError_t launch_kv_append(const KvCache& c, const KvBatch& b, const KvAppend& 
     return hipGetLastError();
   }
   const int units = b.cu_tokens ? kv_units(b, 1 << c.block_shift, 2) : b.sequences * (((b.uniform - 1) >> c.block_shift) + 2);
-  // items that a block gets at most: up to 64 for single tokens, to 2048 for whole blocks, which take one, two or four waves
+  // Items that a block gets at most: up to 64 for single tokens, to 2048 for whole blocks. As many waves as have one or two items a
+  // lane, up to four: with fewer waves and more items a lane 300 rows of 128 dims, 64 in a block, take 12 us instead of 8, 8192 rows 51
+  // instead of 48; single tokens of 128 sequences 8.6 with the shortest kernel and 10.6 with the one for 256 items.
   const int block_items = items * (b.cu_tokens ? 1 << c.block_shift : std::min(b.uniform, 1 << c.block_shift));
   auto run = [&](auto kernel, int waves) {
     const int groups = (int)(((int64_t)units * 2 * c.kv_heads * waves + kWaves - 1) / kWaves);
@@ -357,16 +364,16 @@ hipError_t launch_kv_append(const KvCache& c, const KvBatch& b, const KvAppend& 
   };
   if (half) {
     if (block_items <= 64) run(append8<true, 1, 1>, 1);
-    else if (block_items <= 128) run(append8<true, 1, 2>, 1);
-    else if (block_items <= 256) run(append8<true, 1, 4>, 1);
-    else if (block_items <= 512) run(append8<true, 2, 4>, 2);
+    else if (block_items <= 128) run(append8<true, 2, 1>, 2);
+    else if (block_items <= 256) run(append8<true, 2, 2>, 2);
+    else if (block_items <= 512) run(append8<true, 4, 2>, 4);
     else if (block_items <= 1024) run(append8<true, 4, 4>, 4);
     else run(append8<true, 4, 8>, 4);
   } else {
     if (block_items <= 64) run(append8<false, 1, 1>, 1);
-    else if (block_items <= 128) run(append8<false, 1, 2>, 1);
-    else if (block_items <= 256) run(append8<false, 1, 4>, 1);
-    else if (block_items <= 512) run(append8<false, 2, 4>, 2);
+    else if (block_items <= 128) run(append8<false, 2, 1>, 2);
+    else if (block_items <= 256) run(append8<false, 2, 2>, 2);
+    else if (block_items <= 512) run(append8<false, 4, 2>, 4);
     else if (block_items <= 1024) run(append8<false, 4, 4>, 4);
     else run(append8<false, 4, 8>, 4);
   }
