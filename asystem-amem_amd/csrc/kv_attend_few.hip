@@ -11,6 +11,11 @@
 // holds scores and sums of one row: the softmax needs two exchanges between lanes a tile. Keys and values are loaded as
 // they lie, whole lines by one instruction, past the caches (nothing reads them twice), and pass through LDS, wave
 // by wave, to become operands. A tile's registers are loaded again for the next tile as soon as LDS has them.
+//
+// Measured, where reading alone reaches 6.6 TB/s: 64 single tokens of 2048 to 8192 positions, 32 heads over 8, 128 dims, e4m3: 704 MB in
+// 124 us, 5.7 TB/s; four of 32768 to 131072: 683 MB in 118 us, 5.8; 32 of 1024 to 4096, 16 heads each with its own keys, bf16: 675 MB in
+// 111 us, 6.1; five drafted tokens of 24 sequences, 64 heads over 8, 64 dims, fp16: 190 MB in 44 us, 4.3; one token of 1000 positions:
+// 12 us, of which the join takes 3.5: latency of memory, page number, then keys.
 #include <algorithm>
 
 #include "kv_parts.h"
