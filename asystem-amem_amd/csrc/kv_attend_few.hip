@@ -446,7 +446,7 @@ void plan(const KvCache& c, const KvBatch& b, int group, int head_dim, bool eigh
   const int64_t seen = (int64_t)a.window + (16 * blocks) / group + 1 + 64;
   if (a.causal && a.window && seen < span) span = seen;  // else a window has no far end
   few->units = units_of(b, group, 16 * blocks);
-  cut_last_round(cut_of(head_dim, eight, blocks), few->units * c.kv_heads, span, true, few);
+  cut_pairs(cut_of(head_dim, eight, blocks), c, span, true, few);
 }
 
 template <int D, bool HALF, bool EIGHT, int NB>

@@ -402,7 +402,7 @@ void plan(const KvCache& c, const KvBatch& b, int group, const Shape& shape, con
   if (a.causal && a.window && seen < span) span = seen;  // else a window has no far end
   // the last rows of a prompt see more than the first ones
   const bool even = !a.causal || a.window || 2 * (int64_t)a.max_tokens <= b.max_context;
-  cut_last_round(cut_of(shape), parts->units * c.kv_heads, span, even, parts);
+  cut_pairs(cut_of(shape), c, span, even, parts);
 }
 
 template <int D, int W, int R>

@@ -2,8 +2,7 @@
 #ifndef AMEM_KV_PARTS_H_
 #define AMEM_KV_PARTS_H_
 
-#include <algorithm>
-
+#include "kv_cut.h"
 #include "kv_device.h"
 
 namespace amem {
@@ -77,52 +76,21 @@ __device__ __forceinline__ int64_t part_of(const KvCache& c, const Parts& parts,
   return ((int64_t)(parts.units - 1 - unit) * c.kv_heads + kvh - parts.whole) * parts.splits;
 }
 
-// How pairs are cut. A round is as many workgroups as fit at once; what is cut is the last round, or the only one, where it is not
-// full: into as many stretches of the same length as fill some rounds, if they end sooner. Costs are hundredths of positions.
-struct Cut {
-  int fit;               // workgroups that fit at once, a multiple of the 256 compute units
-  int rounds, over;      // that the last round becomes, at most; up to `over` rounds may be overfull, since some pairs are shorter
-  int least, step;       // positions of a stretch: about the fewest, and what they are a multiple of
-  int base, each, load;  // workgroups take base + each * (those of a compute unit), and at least load * (all of them) / 100
-  int fill;              // positions that pairs have on average, in percent of the longest one's
-  int start, join;       // positions: what a stretch costs beside its own, and the join
-  int part;              // each part's sums, written and read once more
-};
-
-// As many stretches as a context is cut into, at most.
-inline int most_splits(const Cut& cut, int64_t span) { return (int)std::min<int64_t>((span + cut.least / 2) / cut.least, cut.rounds * cut.fit); }
-
 inline int units_of(const KvBatch& b, int group, int tile) {
   return b.cu_tokens ? kv_units(b, tile, 1, group) : b.sequences * ((b.uniform * group - 1) / tile + 1);
 }
 
-// Sets whole, splits and stretch. `even`: pairs see about as many positions each, at most `span`; else the last round is left as
-// it is, since the short ones fill it.
-inline void cut_last_round(const Cut& cut, int pairs, int64_t span, bool even, Parts* parts) {
-  const int last = pairs <= cut.fit ? pairs : even ? pairs % cut.fit : 0, most = most_splits(cut, span);
-  auto time = [&](int count, int loads) { return (int64_t)std::max(cut.base + cut.each * ((count + 255) / 256), cut.load * loads / 100); };
-  parts->splits = 1;
-  int64_t least = time(last, last * cut.fill / 100) * (span + cut.start / 4);
-  for (int i = 0; last && i <= cut.rounds + cut.over; ++i) {
-    // a compute unit's worth, rounds, and rounds that are overfull
-    const int slots = i == 0 ? 256 : i <= cut.rounds ? i * cut.fit : (i - cut.rounds) * cut.fit + last - 1;
-    const int splits = std::min(slots / last, most);
-    if (splits < 2) continue;
-    const int count = last * (100 + (splits - 1) * cut.fill) / 100, rest = count % cut.fit;
-    const int64_t all = count / cut.fit * time(cut.fit, cut.fit) + (rest ? time(rest, rest) : 0);
-    const int64_t cost = all * (span / splits + cut.start) + 100 * (int64_t)cut.join + (int64_t)count * cut.part;
-    if (cost >= least) continue;
-    least = cost;
-    parts->splits = splits;
-  }
-  parts->whole = parts->splits > 1 ? pairs - last : pairs;
-  parts->stretch = (int)(((span + parts->splits - 1) / parts->splits + cut.step - 1) / cut.step * cut.step);
+// Sets whole, splits and stretch.
+inline void cut_pairs(const Cut& cut, const KvCache& c, int64_t span, bool even, Parts* parts) {
+  const CutInto into = cut_last_round(cut, parts->units * c.kv_heads, span, even);
+  parts->whole = into.whole;
+  parts->splits = into.splits;
+  parts->stretch = into.stretch;
 }
 
-// Bytes of the parts of a call, for any mask.
+// Bytes of a call's parts: `rows` of each, their sums, m and l.
 inline uint64_t parts_bytes(const Cut& cut, int64_t pairs, int64_t span, int rows, int head_dim) {
-  const int64_t splits = most_splits(cut, span);
-  return splits < 2 ? 0 : (uint64_t)(std::min<int64_t>(std::min<int64_t>(pairs, cut.fit) * splits, cut.rounds * cut.fit) * rows) * (head_dim + 2) * 4;
+  return (uint64_t)most_parts(cut, pairs, span) * rows * (head_dim + 2) * 4;
 }
 
 inline uint32_t workgroups(const KvCache& c, const Parts& parts) {

@@ -161,13 +161,14 @@ class Batch:
 
     def __init__(self, page_table, context, tokens, cu_tokens=None, max_tokens=None, max_context=None, page_slots=None):
         device = _device(context)
+        _need(len(context.shape) == 1, "context is not [sequences]")
         n = context.shape[0]
         for t, what in ((page_table, "page_table"), (context, "context"), (cu_tokens, "cu_tokens")):
             if t is not None:
                 _is(t, "int32", device, what)
         _need(len(page_table.shape) == 2 and page_table.shape[0] == n and (page_table.stride()[1] == 1 or page_table.shape[1] < 2),
               "page_table is not [sequences, pages] with contiguous pages")
-        _need(len(context.shape) == 1 and (n < 2 or context.stride()[0] == 1), "context is not contiguous")
+        _need(n < 2 or context.stride()[0] == 1, "context is not contiguous")
         if cu_tokens is not None:
             _need(tuple(cu_tokens.shape) == (n + 1,) and cu_tokens.stride()[0] == 1, "cu_tokens is not [sequences + 1]")
             max_tokens = tokens if max_tokens is None else max_tokens
