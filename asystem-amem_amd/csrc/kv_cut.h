@@ -13,11 +13,12 @@ namespace amem {
 struct Cut {
   int fit;               // workgroups that fit at once, a multiple of the 256 compute units
   int rounds, over;      // that the last round becomes, at most; up to `over` rounds may be overfull, since some pairs are shorter
-  int least, step;       // positions of a stretch: about the fewest, and what they are a multiple of
+  int least, step;       // positions of a stretch: about the fewest, and what they are a multiple of; up to 512 of them: of `least`
   int base, each, load;  // workgroups take base + each * (those of a compute unit), and at least load * (all of them) / 100
   int fill;              // positions that pairs have on average, in percent of the longest one's
   int start, join;       // positions: what a stretch costs beside its own, and the join
   int part;              // each part's sums, written and read once more
+  int shorter = 0;       // positions: what is shorter is not cut
 };
 
 // The first `whole` pairs stay whole, each of the others becomes at most `splits` stretches of `stretch` positions.
@@ -26,7 +27,9 @@ struct CutInto {
 };
 
 // As many stretches as a context is cut into, at most.
-inline int most_splits(const Cut& cut, int64_t span) { return (int)std::min<int64_t>((span + cut.least / 2) / cut.least, cut.rounds * cut.fit); }
+inline int most_splits(const Cut& cut, int64_t span) {
+  return span < cut.shorter ? 1 : (int)std::min<int64_t>((span + cut.least / 2) / cut.least, cut.rounds * cut.fit);
+}
 
 // `even`: pairs see about as many positions each, at most `span`; else the last round is left as it is, since the short ones fill it.
 inline CutInto cut_last_round(const Cut& cut, int pairs, int64_t span, bool even) {
@@ -44,7 +47,9 @@ inline CutInto cut_last_round(const Cut& cut, int pairs, int64_t span, bool even
     const int64_t cost = all * (span / splits + cut.start) + 100 * (int64_t)cut.join + (int64_t)count * cut.part;
     if (cost >= least) continue;
     least = cost;
-    into = {pairs - last, splits, (int)(((span + splits - 1) / splits + cut.step - 1) / cut.step * cut.step)};
+    const int64_t length = (span + splits - 1) / splits;
+    const int step = length <= 512 ? std::min(cut.least, cut.step) : cut.step;
+    into = {pairs - last, splits, (int)((length + step - 1) / step * step)};
   }
   return into;
 }
