@@ -311,7 +311,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
         if constexpr (R == 32) sum[i] = mfma32<kHalfP>(v, w[t], sum[i]);
         else sum[i] = mfma16<kHalfP>(v, w[t], sum[i]);
       }
-    if (edge) {
+    if (partial(base)) {  // as store() saw it: rows of this wave may all see the tile, and those of others not
 #pragma unroll 1
       for (int o = 0; o < kPasses * W; ++o) {
         const uint64_t lanes = lds_odd[buffer][o];

@@ -1,0 +1,60 @@
+"""Attention over a paged key/value cache on the GPU where tiles, masks, scales and lengths meet badly; against the restatement in 64
+bits and at the tolerances of test_gpu_kv.py."""
+import numpy as np
+import pytest
+
+from tests import kv_oracle as O
+from tests.kv_case import Arena, Case
+from tests.test_gpu_kv import TYPES, check_attend, poison
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def arena(gpu):
+    a = Arena(gpu)
+    yield a
+    a.free()
+
+
+@pytest.fixture(autouse=True)
+def _fresh_arena(request):
+    if "arena" in request.fixturenames:
+        request.getfixturevalue("arena").reset()
+
+
+def bad_patterns(kind, eight):
+    """NaN and infinity (e4m3 has none: NaN)."""
+    return (0x7F, 0x7F) if eight else (0x7FC0, 0x7F80) if kind == "bf16" else (0x7E00, 0x7C00)
+
+
+@pytest.mark.parametrize("kind,eight", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("window,at", [(0, 500), (0, 430), (200, 300), (200, 650)])
+def test_visible_infinities_and_nan_reach_every_row(arena, dim, kind, eight, window, at):
+    """Values that are not finite in tiles that some waves of a workgroup see whole and others in part, or not at all."""
+    nan, inf = bad_patterns(kind, eight)
+    for bad in (nan, inf):
+        case = Case(arena, [(300, 700)], dim=dim, q_heads=2, kv_heads=2, kind=kind, eight=eight, page=16, block=16, seed=31)
+        poison(case, 0, at, v=bad)
+        case.v[case.table[0, (at + 3) // 16], 1, (at + 3) % 16, 5] = nan     # one value of one head
+        case.upload()
+        got, _ = check_attend(case, case.rows(2), window=window)
+        rows = O.decode(got, kind)
+        seen = case.visible(0, True, window)[:, at]
+        assert 0 < seen.sum() < 300
+        assert not np.isfinite(rows[seen]).any() and np.isfinite(rows[~seen, 0]).all()
+        arena.reset()
+
+
+@pytest.mark.parametrize("kind,eight", TYPES)
+def test_visible_nan_in_the_largest_workgroups(arena, kind, eight):
+    """Enough prompts to fill the chip with eight waves of 32 rows each, a long one among them."""
+    lengths = [(40, 40 + i % 50) for i in range(70)]
+    lengths[3] = (300, 700)
+    case = Case(arena, lengths, dim=128, q_heads=8, kv_heads=8, kind=kind, eight=eight, page=16, block=16, seed=32)
+    nan, inf = bad_patterns(kind, eight)
+    poison(case, 3, 500, v=nan)
+    poison(case, 3, 420, v=inf)
+    case.upload()
+    check_attend(case, case.rows(8), sequences=[0, 3, 69])
