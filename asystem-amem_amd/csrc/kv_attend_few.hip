@@ -54,7 +54,7 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
   int kvh, unit, split;
   pair_of(c, few, blockIdx.x, unit, kvh, split);
   KvSeq q;
-  Unit u;
+  KvUnit u;
   if (!find_unit(b, a, group, 16 * NB, unit, q, u)) return;
   const int begin = u.from + split * few.stretch;
   const int64_t part = part_of(c, few, unit, kvh) + split;  // below zero: the unit's positions are not cut

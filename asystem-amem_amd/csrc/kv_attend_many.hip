@@ -73,7 +73,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
   int kvh, unit, split;
   pair_of(c, parts, blockIdx.x, unit, kvh, split);
   KvSeq q;
-  Unit u;
+  KvUnit u;
   if (!find_unit(b, a, group, W * R, unit, q, u)) return;
   const int begin = u.from + split * parts.stretch;
   if (split && (begin >= u.to || q.bad)) return;

@@ -37,7 +37,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_stretches(KvCache c, KvBatc
   int unit, kvh, split;
   pair_of(c, parts, parts.whole + pair, unit, kvh, split);
   KvSeq q;
-  Unit u;
+  KvUnit u;
   const bool mine = find_unit(b, a, group, tile, unit, q, u) && r < u.rows;
   if (mine) {
     if (b.cu_tokens) load(turn);

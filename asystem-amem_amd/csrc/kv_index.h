@@ -92,5 +92,33 @@ AMEM_HD int kv_units(const KvBatch& b, int tile, int spare, int per_row = 1) {
   return b.tokens * per_row / tile + b.sequences * spare;
 }
 
+// A unit of attention's rows: some rows of one sequence (row r is head r % group of new token r / group), and the positions they see.
+struct KvUnit {
+  int s, first, rows;  // the sequence, the first of its rows, how many
+  int lo, to;          // positions that some row sees: [lo, to)
+  int from;            // lo, down to a multiple of 64
+  int all_from, all_to;  // positions that every row sees
+};
+
+// The positions [from, to) that the rows of a new token see.
+AMEM_HD void kv_row_range(bool causal, int window, const KvSeq& q, int token, int& from, int& to) {
+  const int pos = q.context - q.n + token;
+  to = causal && pos + 1 < q.context ? pos + 1 : q.context;
+  from = window && pos - window + 1 > 0 ? pos - window + 1 : 0;
+}
+
+// Unit `index` of sequence s, `tile` rows long; false if there are no rows, as for an index below zero, which offsets that do not ascend give.
+AMEM_HD bool kv_unit_at(bool causal, int window, int group, int tile, int s, int index, const KvSeq& q, KvUnit& u) {
+  u.s = s;
+  u.first = index * tile;
+  u.rows = q.n * group - u.first;
+  if (index < 0 || u.rows <= 0) return false;
+  if (u.rows > tile) u.rows = tile;
+  kv_row_range(causal, window, q, u.first / group, u.lo, u.all_to);
+  kv_row_range(causal, window, q, (u.first + u.rows - 1) / group, u.all_from, u.to);
+  u.from = u.lo & ~63;
+  return true;
+}
+
 }  // namespace amem
 #endif

@@ -20,34 +20,11 @@ struct Parts {
 
 namespace {
 
-// A unit: some rows of one sequence (row r is head r % group of new token r / group), and the positions they see.
-struct Unit {
-  int s, first, rows;  // the sequence, the first of its rows, how many
-  int lo, to;          // positions that some row sees: [lo, to)
-  int from;            // lo, down to a multiple of 64
-  int all_from, all_to;  // positions that every row sees
-};
-
 __device__ __forceinline__ void row_range(const KvAttend& a, const KvSeq& q, int token, int& from, int& to) {
-  const int pos = q.context - q.n + token;
-  to = a.causal && pos + 1 < q.context ? pos + 1 : q.context;
-  from = a.window && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
+  kv_row_range(a.causal, a.window, q, token, from, to);
 }
 
-// Unit `index` of sequence s, `tile` rows long; false if there are no rows.
-__device__ __forceinline__ bool unit_at(const KvBatch& b, const KvAttend& a, int group, int tile, int s, int index, const KvSeq& q, Unit& u) {
-  u.s = s;
-  u.first = index * tile;
-  u.rows = q.n * group - u.first;
-  if (u.rows <= 0) return false;
-  if (u.rows > tile) u.rows = tile;
-  row_range(a, q, u.first / group, u.lo, u.all_to);
-  row_range(a, q, (u.first + u.rows - 1) / group, u.all_from, u.to);
-  u.from = u.lo & ~63;
-  return true;
-}
-
-__device__ __forceinline__ bool find_unit(const KvBatch& b, const KvAttend& a, int group, int tile, int index, KvSeq& q, Unit& u) {
+__device__ __forceinline__ bool find_unit(const KvBatch& b, const KvAttend& a, int group, int tile, int index, KvSeq& q, KvUnit& u) {
   int s;
   if (b.cu_tokens) {
     s = find_sequence(b, index, tile, 1, group);
@@ -59,7 +36,7 @@ __device__ __forceinline__ bool find_unit(const KvBatch& b, const KvAttend& a, i
     index -= s * each;
   }
   q = kv_seq(b, s);
-  return unit_at(b, a, group, tile, s, index, q, u);
+  return kv_unit_at(a.causal, a.window, group, tile, s, index, q, u);
 }
 
 // The pair and the stretch that workgroup `index` has.

@@ -1,10 +1,13 @@
 """Attention over a paged key/value cache on the GPU where tiles, masks, scales and lengths meet badly; against the restatement in 64
 bits and at the tolerances of test_gpu_kv.py."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
+from asystem_amem_amd import kv
 from tests import kv_oracle as O
-from tests.kv_case import Arena, Case
+from tests.kv_case import KINDS, Arena, Case
 from tests.test_gpu_kv import TYPES, check_attend, poison
 
 pytestmark = pytest.mark.gpu
@@ -58,3 +61,23 @@ def test_visible_nan_in_the_largest_workgroups(arena, kind, eight):
     poison(case, 3, 420, v=inf)
     case.upload()
     check_attend(case, case.rows(8), sequences=[0, 3, 69])
+
+
+@pytest.mark.parametrize("most", [1, 200], ids=["few rows", "many rows"])
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("cu", [(0, 8, 15, 16, 16, 11, 14), (0, 16, 2, 16, 3, 9, 5), (7, 5, 3, 16, -4, 1 << 30, 2)])
+def test_offsets_that_do_not_ascend_stay_inside_the_tensors(arena, cu, eight, most):
+    """What lies around the result and lse keeps its bytes; which rows get what is not defined."""
+    case = Case(arena, [(8, 30), (7, 20), (1, 20), (0, 20), (0, 9), (0, 20)], dim=128, q_heads=8, kv_heads=2, eight=eight, page=16, seed=33)
+    assert case.tokens == 16
+    case.cu, case.max_tokens = np.array(cu, np.int32), min(most, 16)
+    case.upload()
+    q, guard = case.rows(8), 1 << 16
+    n = C.c_uint64()
+    assert case.lib.amem_kv_attention_workspace(C.byref(case.cache), C.byref(case.batch), 8, C.byref(n)) == 0
+    out, lse = arena.blank(q.nbytes + 2 * guard), arena.blank(16 * 8 * 4 + 2 * guard)
+    args = kv.AttentionArgs(arena.put(q), out + guard, lse + guard, arena.blank(n.value), n.value, 1024, 128, 1024, 128, 0.1, KINDS["bf16"], 8, 1, 0, 0)
+    assert case.lib.amem_kv_attention(C.byref(case.cache), C.byref(case.batch), C.byref(args), None) == 0
+    for at, size in ((out, q.nbytes), (lse, 16 * 8 * 4)):
+        x = arena.read(at, (size + 2 * guard,), np.uint8)
+        assert (x[:guard] == 0xA5).all() and (x[guard + size:] == 0xA5).all()
