@@ -104,7 +104,7 @@ struct KvUnit {
 AMEM_HD void kv_row_range(bool causal, int window, const KvSeq& q, int token, int& from, int& to) {
   const int pos = q.context - q.n + token;
   to = causal && pos + 1 < q.context ? pos + 1 : q.context;
-  from = window && pos - window + 1 > 0 ? pos - window + 1 : 0;
+  from = window && pos >= window ? pos - window + 1 : 0;  // any window, and positions below zero, without overflow
 }
 
 // Unit `index` of sequence s, `tile` rows long; false if there are no rows, as for an index below zero, which offsets that do not ascend give.

@@ -62,7 +62,7 @@ typedef struct amem_kv_cache {
  * `max_context` or above table_pages * page_slots is out of range, and so is a page number outside
  * [0, pages) that a position needs: append writes nothing there, attention gives NaN in the
  * rows that would see it. New tokens at negative positions (a context shorter than them) are not
- * appended, and as queries they see nothing. */
+ * appended; as queries they see what the masks leave them, which is nothing where causal. */
 typedef struct amem_kv_batch {
   uint64_t page_table;           /* int32 [sequences][table_stride] */
   uint64_t context;              /* int32 [sequences] */

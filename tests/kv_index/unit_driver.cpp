@@ -54,6 +54,9 @@ static void units(const KvBatch& b, int group, int tile, bool causal, int window
       int from, end;
       kv_row_range(causal, window, q, r / group, from, end);
       CHECK(from >= 0 && end <= q.context);
+      // as 64 bits have it
+      const int64_t pos = (int64_t)q.context - q.n + r / group, far = window ? pos - window + 1 : 0;
+      CHECK(from == (far > 0 ? far : 0) && end == (causal && pos + 1 < q.context ? pos + 1 : q.context));
       lo = from < lo ? from : lo;
       to = end > to ? end : to;
       all_from = from > all_from ? from : all_from;
@@ -99,9 +102,9 @@ int main() {
     }
     b.cu_tokens = cu.data();
     b.context = context.data();
-    const int windows[] = {0, 0, 1, 5, 64, 1000};
+    const int windows[] = {0, 0, 1, 5, 64, 1000, INT_MAX, INT_MAX - 1};
     for (int tile : {16, 48, 128}) {
-      units(b, group, tile, r() % 2, windows[r() % 6], times);
+      units(b, group, tile, r() % 2, windows[r() % 8], times);
       if (!wrong)
         for (int i = 0; i < b.tokens * group; ++i) CHECK(times[i] == (i < used * group));
     }

@@ -81,3 +81,13 @@ def test_offsets_that_do_not_ascend_stay_inside_the_tensors(arena, cu, eight, mo
     for at, size in ((out, q.nbytes), (lse, 16 * 8 * 4)):
         x = arena.read(at, (size + 2 * guard,), np.uint8)
         assert (x[:guard] == 0xA5).all() and (x[guard + size:] == 0xA5).all()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 30])
+def test_the_widest_windows(arena, window, causal):
+    """They hide nothing, from rows at negative positions neither."""
+    for lengths in ([(4, 2), (1, 1300), (3, 1)], [(70, 33), (40, 1300), (300, 280)]):
+        case = Case(arena, lengths, dim=64, q_heads=4, kv_heads=2, page=16, seed=34).upload()
+        check_attend(case, case.rows(4), causal, window)
+        arena.reset()
