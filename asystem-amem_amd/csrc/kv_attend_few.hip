@@ -99,7 +99,10 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i) sum[n][i] = f32x4{0, 0, 0, 0};
   }
-  float unit_scale = 0;  // the sums are in multiples of it; the largest scale of values so far (8 bits)
+  // 8 bits: the sums are in multiples of unit_scale, or (far) of the row's 2^sum_unit
+  float unit_scale = 0, h[NB];
+  int sum_unit[NB];
+  bool far = false;
 
   uint8_t* const mine = lds + wave * kTile * kPitch;
   const uint8_t* const keys = c.k + (int64_t)kvh * c.head_stride;
@@ -150,6 +153,8 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
 
   int base = begin + wave * kTile;
   constexpr int kStep = kWaves * kTile;
+  auto seen = [&](int from) { return from < u.to && from + 15 >= u.lo; };  // a hidden group's scale may be anything
+  float inverse_unit = 0;
   if (base < end) {
     page = look_up(base);
     page_next = look_up(base + kStep);
@@ -157,6 +162,12 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
     load_rows(keys, base, page, true, kreg);
     load_scales(base, page, ks, vs);
     load_rows(values, base, page, true, vreg);
+    if constexpr (EIGHT) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) unit_scale = fmaxf(unit_scale, seen(base + g * 16) ? lane_value(vs, g * 16) : 0);
+      unit_scale *= 1 << kNear;
+      inverse_unit = 1.0f / unit_scale;
+    }
   }
   for (; base < end; base += kStep) {
     const bool more = base + kStep < end;
@@ -249,6 +260,27 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
     load_scales(base + kStep, page, ks_next, vs_next);
     load_rows(values, base + kStep, page, more, vreg);
 
+    float f_scale[kGroups];  // scales of values, in multiples of unit_scale
+    if constexpr (EIGHT) {
+      float least = 1, most = 0;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        f_scale[g] = far ? 1.0f : seen(base + g * 16) ? lane_value(vs, g * 16) * inverse_unit : 1.0f;
+        least = fminf(least, f_scale[g]);
+        most = fmaxf(most, f_scale[g]);
+      }
+      if (!(most <= 1 && least >= 1.0f / (1 << 2 * kNear))) {
+        far = true;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          sum_unit[n] = exponent_of(unit_scale);
+          h[n] = m[n] == -kInf ? kNothing : sum_unit[n] + kLift;  // weights were at most 2^kLift
+        }
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) f_scale[g] = 1.0f;
+      }
+    }
+
     // running maximum; where it grows, what has been summed shrinks
     bool grew = false;
     float shrink[NB];
@@ -264,28 +296,8 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
       const float now = __builtin_elementwise_maximum(m[n], top);
       shrink[n] = now == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - now);
       grew |= now != m[n];
+      if (EIGHT && far) h[n] = fmaxf(h[n] + (m[n] - now), kNothing);
       m[n] = now;
-    }
-    float f_scale[kGroups];
-    if constexpr (EIGHT) {
-      float top = 0;
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        const bool seen = base + g * 16 < u.to && base + g * 16 + 15 >= u.lo;  // a hidden group's scale may be anything
-        f_scale[g] = seen ? lane_value(vs, g * 16) : 0;
-        top = __builtin_elementwise_maximum(top, f_scale[g]);
-      }
-      if (!(top <= unit_scale)) {
-        const float f = unit_scale / top;
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-          for (int i = 0; i < kBlocks; ++i) sum[n][i] *= f;
-        unit_scale = top;
-      }
-      const float f = unit_scale > 0 ? 1.0f / unit_scale : 0.0f;
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) f_scale[g] *= f;
     }
     if (__any(grew)) {
 #pragma unroll
@@ -306,11 +318,40 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
         for (int i = 0; i < 4; ++i) {
           x[i] = __builtin_amdgcn_exp2f(score[n][g][i] - top);
           l[n] += x[i];
-          if constexpr (EIGHT) x[i] *= f_scale[g];
           score[n][g][i] = x[i];
         }
         w[n][g / 2][g % 2 * 2] = pack<kHalfP>(x[0], x[1]);
         w[n][g / 2][g % 2 * 2 + 1] = pack<kHalfP>(x[2], x[3]);
+      }
+    }
+    if (EIGHT && far) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        int of[kGroups];
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          float x = score[n][g][0];
+#pragma unroll
+          for (int i = 1; i < 4; ++i) x = __builtin_elementwise_maximum(x, score[n][g][i]);
+          x = __builtin_elementwise_maximum(x, __shfl_xor(x, 16, kWave));
+          x = __builtin_elementwise_maximum(x, __shfl_xor(x, 32, kWave));
+          of[g] = exponent_of(lane_value(vs, g * 16));
+          if (x != 0) h[n] = fmaxf(h[n], exponent_of(x) + 1 + of[g]);
+        }
+        const int before = sum_unit[n];
+        sum_unit[n] = far_unit(h[n]);
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_ldexpf(score[n][g][i], of[g] - sum_unit[n]);
+          w[n][g / 2][g % 2 * 2] = pack<true>(x[0], x[1]);
+          w[n][g / 2][g % 2 * 2 + 1] = pack<true>(x[2], x[3]);
+        }
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[n][i][e] = __builtin_amdgcn_ldexpf(sum[n][i][e], before - sum_unit[n]);
       }
     }
 #pragma unroll
@@ -320,7 +361,7 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
         const uint8_t* p = mine + read_at + t * 32 * kPitch + i * 16 * kElement;
         u32x4 v;
         if constexpr (EIGHT) {
-          v = widen<true>(read_columns8(p));
+          v = widen<true>(read_columns8(p), f_scale[2 * t], f_scale[2 * t + 1]);
         } else {
           const u32x2 lo = read_columns16(p), hi = read_columns16(p + 16 * kPitch);
           v = u32x4{lo[0], lo[1], hi[0], hi[1]};
@@ -351,6 +392,11 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
               if (g == k / 16 && e == k % 4) x = score[n][g][e];
           x = __shfl(x, (k % 16 / 4) * 16 + col, kWave);
           if (p < row_from[n] || p >= row_to[n]) continue;
+          if constexpr (EIGHT) {
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g)
+              if (g == k / 16) x = far ? __builtin_amdgcn_ldexpf(x, exponent_of(lane_value(vs, g * 16)) - sum_unit[n]) : x * f_scale[g];
+          }
 #pragma unroll
           for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
@@ -383,7 +429,8 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
     float top = lds_m[0][n * 16 + col];
 #pragma unroll
     for (int i = 1; i < kWaves; ++i) top = __builtin_elementwise_maximum(top, lds_m[i][n * 16 + col]);
-    const float f = (m[n] == top ? 1.0f : __builtin_amdgcn_exp2f(m[n] - top)) * (EIGHT && unit_scale > 0 ? unit_scale : 1.0f);
+    float f = m[n] == top ? 1.0f : __builtin_amdgcn_exp2f(m[n] - top);
+    if constexpr (EIGHT) f *= far ? __builtin_amdgcn_ldexpf(1.0f, sum_unit[n] - kPartExponent) : unit_scale / kPartUnit;
     float* at = (float*)lds + (wave * 16 + col) * (D + 4) + quad * 4;
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i) *(f32x4*)(at + i * 16) = sum[n][i] * f;
@@ -415,7 +462,7 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
         continue;
       }
       const int rr = u.first + n * 16 + r, token = rr / group, head = kvh * group + rr % group;
-      const float inverse = q.bad ? __builtin_nanf("") : ll == 0 ? 0.0f : 1.0f / ll;
+      const float inverse = q.bad ? __builtin_nanf("") : ll == 0 ? 0.0f : (EIGHT ? kPartUnit : 1.0f) / ll;
       if (ll == 0) x = f32x4{0, 0, 0, 0};
       *(u32x2*)(a.out + (q.row + token) * a.out_token + head * a.out_head + d) =
           u32x2{pack<HALF>(x[0] * inverse, x[1] * inverse), pack<HALF>(x[2] * inverse, x[3] * inverse)};
@@ -463,7 +510,7 @@ hipError_t launch_few(const KvCache& c, const KvBatch& b, const KvAttend& a, con
     attend_few<D, HALF, EIGHT, NB, true><<<grid, kWaves * kWave, 0, stream>>>(c, b, a, few);
   }
   if (hipError_t e = hipGetLastError(); e != hipSuccess || few.splits == 1) return e;
-  return launch_join(c, b, a, few, 16 * NB, EIGHT || HALF ? 8.0f : 0.0f, D, HALF, stream);
+  return launch_join(c, b, a, few, 16 * NB, EIGHT || HALF ? 8.0f : 0.0f, EIGHT ? kPartUnit : 1.0f, D, HALF, stream);
 }
 
 template <int D, bool HALF, bool EIGHT>

@@ -23,27 +23,10 @@ namespace {
 
 constexpr int kTile = 64;  // positions
 
-// Eight e4m3 codes times a power of two as 16-bit numbers.
-template <bool HALF>
-__device__ __forceinline__ u32x4 widen_scaled(u32x2 x, float scale) {
-  u32x4 y;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if constexpr (HALF) {
-      y[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[i], scale, false));
-      y[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[i], scale, true));
-    } else {
-      y[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], scale, false));
-      y[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], scale, true));
-    }
-  }
-  return y;
-}
-
 // D dims, 16 bits of fp16 (HALF) or bf16, a cache of e4m3 (EIGHT).
 // W waves with R rows each, 32 or 16.
 template <int D, bool HALF, bool EIGHT, int W, int R>
-__global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b, KvAttend a, Parts parts) {
+__global__ __launch_bounds__(W * kWave, (D == 64 ? 3 : 2)) void attend_many(KvCache c, KvBatch b, KvAttend a, Parts parts) {
   constexpr int kThreads = W * kWave;
   constexpr int kElement = EIGHT ? 1 : 2;
   constexpr int kRowLanes = D * kElement / 16;    // threads that load a position's key, or value
@@ -85,7 +68,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
   // the second ones behind them, so that neighbouring threads write to neighbouring banks (963 -> 957 us at a chunk of 4096 over 16384). What
   // dim is at a place of a row:
   auto dim_at = [](int place) { return EIGHT ? place % (D / 2) / 8 * 16 + place / (D / 2) * 8 + place % 8 : place; };
-  auto dim_of = [&](int i, int e) { return dim_at(R == 32 ? i * 32 + e / 4 * 8 + part * 4 + e % 4 : i * 16 + part * 4 + e); };
+  auto dim_of = [&](int i, int e, int part) { return dim_at(R == 32 ? i * 32 + e / 4 * 8 + part * 4 + e % 4 : i * 16 + part * 4 + e); };
 
   // this wave's rows, and the positions that some, and all, of them see
   const int wave_first = u.first + wave * R;
@@ -114,7 +97,9 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
   for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
     for (int j = 0; j < kSums; ++j) sum[i][j] = 0;
-  uint32_t unit_scale = 0;  // the sums are in multiples of it (8 bits); bits
+  uint32_t unit_scale = 0;  // 8 bits: the sums are in multiples of it, as bits; or (far) of the row's 2^sum_unit
+  float h = kNothing;
+  int sum_unit = 0;
 
   // ---- loading: a thread's rows of a tile
   const int my_row = tid / kRowLanes, my_col = tid % kRowLanes * 16;
@@ -151,21 +136,25 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
   };
   auto partial = [&](int base) { return base < u.all_from || base + kTile > u.all_to; };
   // The registers' tile into LDS. Keys of a page that is out of range become NaN, which every row that sees them gets.
-  // Values are stored in multiples of the largest scale so far, as powers of two: a difference of exponents.
-  float key_scale[4];         // of the tile stored last
-  uint32_t stored_scale = 0;  // bits
+  // Values are stored in multiples of unit_scale, as powers of two: a difference of exponents; or as they are (far).
+  float key_scale[4];  // of the tile stored last
+  uint64_t far = 0;    // not zero once a scale was far; a ballot, which stays in scalar registers
   constexpr uint32_t kExponent = 0x7f800000, kOne = 0x3f800000;
+  auto seen = [&](int base) {  // this lane's group: a hidden one's scale may be anything
+    const int p = base + (lane & 3) * 16;
+    return p < u.to && p + 15 >= u.lo;
+  };
   auto store = [&](int base, int buffer) {
     uint8_t* const at = lds + buffer * kBuffer;
-    uint32_t seen_vs = 0;
+    uint32_t value_scale = kOne;
     if constexpr (EIGHT) {
-      const int p = base + (lane & 3) * 16;
-      seen_vs = p < u.to && p + 15 >= u.lo ? vs : 0;  // a hidden group's scale may be anything
+      if constexpr (!kFold) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        if constexpr (!kFold) key_scale[g] = lane_value(__builtin_bit_cast(float, ks), g);
-        stored_scale = std::max(stored_scale, (uint32_t)__builtin_amdgcn_readlane((int)seen_vs, g));
+        for (int g = 0; g < 4; ++g) key_scale[g] = lane_value(__builtin_bit_cast(float, ks), g);
       }
+      const uint32_t scale = seen(base) ? vs : unit_scale;
+      far |= __ballot(unit_scale - scale > (uint32_t)(2 * kNear) << 23);
+      value_scale = far ? kOne : scale - unit_scale + kOne;
     }
     const bool edge = partial(base);
 #pragma unroll
@@ -183,14 +172,13 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
       }
       if constexpr (EIGHT) {
         const float fk = kFold ? __builtin_bit_cast(float, __shfl((int)ks, r >> 4, kWave)) : 1.0f;
-        const int apart = __shfl((int)seen_vs, r >> 4, kWave) - (int)(stored_scale & kExponent) + (int)kOne;
-        const float fv = __builtin_bit_cast(float, apart > 0 ? apart : 0);
+        const float fv = __builtin_bit_cast(float, __shfl((int)value_scale, r >> 4, kWave));
         uint8_t* ka = at + r * kKeyPitch + my_col;
         uint8_t* va = at + kTile * kKeyPitch + r * kValuePitch + my_col;
-        *(u32x4*)ka = widen_scaled<HALF>(u32x2{k[0], k[1]}, fk);
-        *(u32x4*)(ka + D) = widen_scaled<HALF>(u32x2{k[2], k[3]}, fk);
-        *(u32x4*)va = widen_scaled<true>(u32x2{v[0], v[1]}, fv);
-        *(u32x4*)(va + D) = widen_scaled<true>(u32x2{v[2], v[3]}, fv);
+        *(u32x4*)ka = widen<HALF>(u32x2{k[0], k[1]}, fk, fk);
+        *(u32x4*)(ka + D) = widen<HALF>(u32x2{k[2], k[3]}, fk, fk);
+        *(u32x4*)va = widen<true>(u32x2{v[0], v[1]}, fv, fv);
+        *(u32x4*)(va + D) = widen<true>(u32x2{v[2], v[3]}, fv, fv);
       } else {
         *(u32x4*)(at + r * kKeyPitch + my_col) = k;
         *(u32x4*)(at + kTile * kKeyPitch + r * kValuePitch + my_col) = v;
@@ -202,12 +190,20 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
     look_up(begin);
     load(begin);
     look_up(begin + kTile);
+    if constexpr (EIGHT) {
+      const uint32_t scale = seen(begin) ? vs : 0;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) unit_scale = std::max(unit_scale, (uint32_t)__builtin_amdgcn_readlane((int)scale, g) & kExponent);
+      unit_scale += kNear << 23;
+    }
     store(begin, 0);
     load(begin + kTile);
     look_up(begin + 2 * kTile);
   }
-  int buffer = 0;
-  for (int base = begin; base < end; base += kTile, buffer ^= 1) {
+  int base = begin, buffer = 0;
+  // One tile; kFar: its scales, or earlier ones, are far apart.
+  auto take = [&](auto is_far) {
+    constexpr bool kFar = decltype(is_far)::value;
     __syncthreads();
     const bool work = active && base < wave_to && base + kTile > wave_lo;
     const uint8_t* const tile = lds + buffer * kBuffer;
@@ -217,7 +213,6 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
 #pragma unroll
       for (int g = 0; g < 4; ++g) f[g] = key_scale[g];
     }
-    const uint32_t tile_scale = stored_scale;
     if (work) {
       Result s[kTile / R];
 #pragma unroll
@@ -249,7 +244,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
       load(base + 2 * kTile);
       look_up(base + 3 * kTile);
     }
-    if (!work) continue;
+    if (!work) return;
 
     if constexpr (EIGHT && !kFold) {
 #pragma unroll
@@ -279,15 +274,8 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
       for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
         for (int j = 0; j < kSums; ++j) sum[i][j] *= shrink;
+      if constexpr (kFar) h = fmaxf(h + (m - now), kNothing);
       m = now;
-    }
-    if (EIGHT && tile_scale != unit_scale) {  // it only grows
-      const float x = __builtin_bit_cast(float, unit_scale & kExponent) / __builtin_bit_cast(float, tile_scale & kExponent);
-#pragma unroll
-      for (int i = 0; i < kBlocks; ++i)
-#pragma unroll
-        for (int j = 0; j < kSums; ++j) sum[i][j] *= x;
-      unit_scale = tile_scale;
     }
     const float sub = (m == -kInf ? 0.0f : m) - kLift;
     // weights as operands: the eight of a step are the positions of eight scores in a row
@@ -297,8 +285,37 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
       score[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j], factor, -sub));
       l += score[j];
     }
+    if constexpr (!kFar) {
 #pragma unroll
-    for (int j = 0; j < kScores / 2; ++j) w[j / 4][j % 4] = pack<kHalfP>(score[2 * j], score[2 * j + 1]);
+      for (int j = 0; j < kScores / 2; ++j) w[j / 4][j % 4] = pack<kHalfP>(score[2 * j], score[2 * j + 1]);
+    } else {
+      // the scales are read once more, which costs less than keeping them where they are not needed
+      const int p = std::min(base + (lane & 3) * 16, u.to - 1), where = kv_page(c, b, u.s, p);
+      const float scales = c.v_scale[kv_scale_offset(c, where < 0 ? 0 : where, kvh, p)];
+      constexpr int kEach = kScores / 4;  // scores of a lane that share a scale
+      int of[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float x = score[g * kEach];
+#pragma unroll
+        for (int j = 1; j < kEach; ++j) x = __builtin_elementwise_maximum(x, score[g * kEach + j]);
+        if constexpr (R == 16) x = __builtin_elementwise_maximum(x, __shfl_xor(x, 16, kWave));
+        x = __builtin_elementwise_maximum(x, __shfl_xor(x, 32, kWave));
+        of[g] = exponent_of(lane_value(scales, g));
+        if (x != 0) h = fmaxf(h, exponent_of(x) + 1 + of[g]);
+      }
+      const int before = sum_unit;
+      sum_unit = far_unit(h);
+#pragma unroll
+      for (int j = 0; j < kScores / 2; ++j) {
+        const int by = of[2 * j / kEach] - sum_unit;
+        w[j / 4][j % 4] = pack<true>(__builtin_amdgcn_ldexpf(score[2 * j], by), __builtin_amdgcn_ldexpf(score[2 * j + 1], by));
+      }
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+        for (int e = 0; e < kSums; ++e) sum[i][e] = __builtin_amdgcn_ldexpf(sum[i][e], before - sum_unit);
+    }
     // lane m of 16 gives the address of position m / 4 of four, dims 4 (m % 4) on, of the 16 dims that these lanes take
     const uint8_t* const columns = tile + kTile * kKeyPitch + (4 * part + (lane & 15) / 4) * kValuePitch + ((R == 32 ? (lane >> 4 & 1) * 16 : 0) + (lane & 3) * 4) * 2;
 #pragma unroll
@@ -323,6 +340,8 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
           const int where = kv_page(c, b, u.s, p);  // seen by some row, so below u.to
           if (where < 0) continue;                  // its key is NaN already
           const uint8_t* v = c.v + kv_offset(c, where, kvh, p);
+          int own = part;
+          asm volatile("" : "+v"(own));  // keeps the places of all dims from being computed, and held, before the tiles
           // the weight of k, from the lane that has it
           const int index = R == 32 ? k / 8 * 4 + k % 4 : k / 16 * 4 + k % 4;
           float x = 0;
@@ -331,24 +350,39 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
             if (j == index) x = score[j];
           x = __shfl(x, (R == 32 ? k / 4 % 2 : k / 4 % 4) * R + col, kWave);
           if (p < row_from || p >= row_to) continue;
-          if constexpr (EIGHT)
-            x *= c.v_scale[kv_scale_offset(c, where, kvh, p)] * (unit_scale ? 1.0f / __builtin_bit_cast(float, unit_scale & kExponent) : 0.0f);
+          if constexpr (EIGHT) {
+            const float scale = c.v_scale[kv_scale_offset(c, where, kvh, p)];
+            x = kFar ? __builtin_amdgcn_ldexpf(x, exponent_of(scale) - sum_unit)
+                     : x * (scale / __builtin_bit_cast(float, unit_scale));
+          }
 #pragma unroll
           for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
             for (int e = 0; e < kSums; ++e) {
-              if constexpr (EIGHT) sum[i][e] += x * __builtin_amdgcn_cvt_f32_fp8((int)v[dim_of(i, e)], 0);
-              else sum[i][e] += x * to_float<HALF>(((const uint16_t*)v)[dim_of(i, e)]);
+              if constexpr (EIGHT) sum[i][e] += x * __builtin_amdgcn_cvt_f32_fp8((int)v[dim_of(i, e, own)], 0);
+              else sum[i][e] += x * to_float<HALF>(((const uint16_t*)v)[dim_of(i, e, own)]);
             }
         }
       }
+    }
+  };
+  // A loop of its own for what comes after scales far apart: as a branch of this one between exponentials and products it would keep them from
+  // mixing (a chunk of 4096 over 16384, e4m3: 945 us, and 1112).
+  bool sums_far = false;
+  for (; base < end && !(EIGHT && far); base += kTile, buffer ^= 1) take(std::false_type());
+  if constexpr (EIGHT) {
+    if (base < end) {
+      sums_far = true;
+      sum_unit = exponent_of(__builtin_bit_cast(float, unit_scale));
+      h = m == -kInf ? kNothing : sum_unit + (kLift + kSlack);  // weights were at most 2^(kLift + kSlack)
+      for (; base < end; base += kTile, buffer ^= 1) take(std::true_type());
     }
   }
   if (!active) return;
 
   if constexpr (R == 16) l += __shfl_xor(l, 16, kWave);
   l += __shfl_xor(l, 32, kWave);
-  const float back = EIGHT ? __builtin_bit_cast(float, unit_scale & kExponent) : 1.0f;
+  const float back = !EIGHT ? 1.0f : sums_far ? __builtin_amdgcn_ldexpf(1.0f, sum_unit) : __builtin_bit_cast(float, unit_scale);
   const int r = wave * R + col;
   if (r >= u.rows) return;
   if (cut >= 0) {
@@ -357,7 +391,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
     for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
       for (int e = 0; e < kSums; e += 4)
-        *(f32x4*)(parts.sums + row * D + dim_of(i, e)) = f32x4{sum[i][e], sum[i][e + 1], sum[i][e + 2], sum[i][e + 3]} * back;
+        *(f32x4*)(parts.sums + row * D + dim_of(i, e, part)) = f32x4{sum[i][e], sum[i][e + 1], sum[i][e + 2], sum[i][e + 3]} * (EIGHT ? back / kPartUnit : 1.0f);
     if (part == 0) {
       parts.stats[row * 2] = m;
       parts.stats[row * 2 + 1] = l;
@@ -371,7 +405,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_many(KvCache c, KvBatch b
 #pragma unroll
     for (int e = 0; e < kSums; e += 4) {
       const f32x4 x = f32x4{sum[i][e], sum[i][e + 1], sum[i][e + 2], sum[i][e + 3]} * inverse;
-      *(u32x2*)(out + dim_of(i, e)) = u32x2{pack<HALF>(x[0], x[1]), pack<HALF>(x[2], x[3])};
+      *(u32x2*)(out + dim_of(i, e, part)) = u32x2{pack<HALF>(x[0], x[1]), pack<HALF>(x[2], x[3])};
     }
   if (a.lse && part == 0)
     a.lse[(int64_t)(q.row + token) * a.q_heads + head] = q.bad ? __builtin_nanf("") : l == 0 ? -kInf : ((m - kLift) + __builtin_amdgcn_logf(l)) * kLn2;
@@ -422,7 +456,7 @@ hipError_t launch_waves(const KvCache& c, const KvBatch& b, const KvAttend& a, b
     attend_many<D, false, false, W, R><<<grid, kThreads, 0, stream>>>(c, b, a, parts);
   }
   if (hipError_t e = hipGetLastError(); e != hipSuccess || parts.splits == 1) return e;
-  return launch_join(c, b, a, parts, W * R, half || eight ? 8.0f : 0.0f, D, half, stream);
+  return launch_join(c, b, a, parts, W * R, half || eight ? 8.0f : 0.0f, eight ? kPartUnit : 1.0f, D, half, stream);
 }
 
 template <int D>

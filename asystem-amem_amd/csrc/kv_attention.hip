@@ -16,7 +16,7 @@ constexpr int kJoinThreads = 256;
 // turn; B parts are loaded at once, the first of them before the lengths are known, which say how many there are, where all units have
 // as many rows. `rows`: those that a unit can have.
 template <int D, bool HALF, int W, int B>
-__global__ __launch_bounds__(kJoinThreads) void join_stretches(KvCache c, KvBatch b, KvAttend a, Parts parts, int tile, int rows, float lift) {
+__global__ __launch_bounds__(kJoinThreads) void join_stretches(KvCache c, KvBatch b, KvAttend a, Parts parts, int tile, int rows, float lift, float sum_unit) {
   constexpr int kItems = kJoinThreads / W;
   const int blocks = (rows * (D / 4) + kItems - 1) / kItems, pair = blockIdx.x / blocks, turn = threadIdx.x / kItems;
   const int item = blockIdx.x % blocks * kItems + threadIdx.x % kItems, r = item / (D / 4), d = item % (D / 4) * 4;
@@ -84,20 +84,20 @@ __global__ __launch_bounds__(kJoinThreads) void join_stretches(KvCache c, KvBatc
     x = f32x4{0, 0, 0, 0};
     l = q.bad ? __builtin_nanf("") : 0;
   }
-  const float inverse = l == 0 ? 0.0f : 1.0f / l;
+  const float inverse = l == 0 ? 0.0f : sum_unit / l;
   *(u32x2*)(a.out + (q.row + token) * a.out_token + head * a.out_head + d) =
       u32x2{pack<HALF>(x[0] * inverse, x[1] * inverse), pack<HALF>(x[2] * inverse, x[3] * inverse)};
   if (a.lse && d == 0) a.lse[(int64_t)(q.row + token) * a.q_heads + head] = l == 0 ? -kInf : ((m - lift) + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 template <int D, bool HALF>
-hipError_t join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int tile, float lift, hipStream_t stream) {
+hipError_t join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int tile, float lift, float sum_unit, hipStream_t stream) {
   const int pairs = parts.units * c.kv_heads - parts.whole;
   const int rows = b.cu_tokens ? tile : (int)std::min<int64_t>(tile, (int64_t)b.uniform * (a.q_heads / c.kv_heads)), items = rows * (D / 4);
   auto blocks = [&](int each) { return pairs * ((items + each - 1) / each); };
-  if (parts.splits > 8) join_stretches<D, HALF, 4, 8><<<blocks(kJoinThreads / 4), kJoinThreads, 0, stream>>>(c, b, a, parts, tile, rows, lift);
-  else if (parts.splits > 4) join_stretches<D, HALF, 1, 8><<<blocks(kJoinThreads), kJoinThreads, 0, stream>>>(c, b, a, parts, tile, rows, lift);
-  else join_stretches<D, HALF, 1, 4><<<blocks(kJoinThreads), kJoinThreads, 0, stream>>>(c, b, a, parts, tile, rows, lift);
+  if (parts.splits > 8) join_stretches<D, HALF, 4, 8><<<blocks(kJoinThreads / 4), kJoinThreads, 0, stream>>>(c, b, a, parts, tile, rows, lift, sum_unit);
+  else if (parts.splits > 4) join_stretches<D, HALF, 1, 8><<<blocks(kJoinThreads), kJoinThreads, 0, stream>>>(c, b, a, parts, tile, rows, lift, sum_unit);
+  else join_stretches<D, HALF, 1, 4><<<blocks(kJoinThreads), kJoinThreads, 0, stream>>>(c, b, a, parts, tile, rows, lift, sum_unit);
   return hipGetLastError();
 }
 
@@ -110,10 +110,10 @@ bool few_rows(int q_heads, int kv_heads, int max_tokens, int head_dim) {
 
 }  // namespace
 
-hipError_t launch_join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int tile, float lift, int head_dim, bool half, hipStream_t stream) {
-  if (head_dim == 64) return half ? join<64, true>(c, b, a, parts, tile, lift, stream) : join<64, false>(c, b, a, parts, tile, lift, stream);
-  if (head_dim == 128) return half ? join<128, true>(c, b, a, parts, tile, lift, stream) : join<128, false>(c, b, a, parts, tile, lift, stream);
-  return half ? join<256, true>(c, b, a, parts, tile, lift, stream) : join<256, false>(c, b, a, parts, tile, lift, stream);
+hipError_t launch_join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int tile, float lift, float sum_unit, int head_dim, bool half, hipStream_t stream) {
+  if (head_dim == 64) return half ? join<64, true>(c, b, a, parts, tile, lift, sum_unit, stream) : join<64, false>(c, b, a, parts, tile, lift, sum_unit, stream);
+  if (head_dim == 128) return half ? join<128, true>(c, b, a, parts, tile, lift, sum_unit, stream) : join<128, false>(c, b, a, parts, tile, lift, sum_unit, stream);
+  return half ? join<256, true>(c, b, a, parts, tile, lift, sum_unit, stream) : join<256, false>(c, b, a, parts, tile, lift, sum_unit, stream);
 }
 
 uint64_t kv_attend_workspace(const KvCache& c, const KvBatch& b, int q_heads, int max_tokens, int head_dim) {

@@ -51,22 +51,39 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {  // 32 x 
   else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Eight e4m3 codes as 16-bit numbers, exactly (both types hold every one of them).
+// Eight e4m3 codes as 16-bit numbers, those of the first word times `first` and of the second times `second`, powers of two. Both types hold
+// every code exactly, and fp16 its product with 2^-15 to 2^7.
 template <bool HALF>
-__device__ __forceinline__ u32x4 widen(u32x2 x) {
+__device__ __forceinline__ u32x4 widen(u32x2 x, float first = 1.0f, float second = 1.0f) {
   u32x4 y;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
+    const float f = i ? second : first;
     if constexpr (HALF) {
-      y[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[i], 1.0f, false));
-      y[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[i], 1.0f, true));
+      y[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[i], f, false));
+      y[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[i], f, true));
     } else {
-      y[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], 1.0f, false));
-      y[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], 1.0f, true));
+      y[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], f, false));
+      y[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], f, true));
     }
   }
   return y;
 }
+
+// Scales of e4m3 values meet the weights in fp16. While those that a workgroup (or a wave) meets are within 2^kNear of the largest of its first
+// tile, codes are widened in multiples of 2^kNear times that one, exactly, and so are the sums. From the first tile on where one is not ("far"), codes
+// are widened as they are, and each row's weights take the scales, in multiples of a power of two of the row's own: its sums are in
+// multiples of 2^far_unit(h), where 2^h is at least its largest product of weight and scale so far. Those products are at most 2^15 in it,
+// and a large scale costs small ones no bits unless it comes with a weight. h falls as m grows and the weights so far shrink. Parts
+// leave a workgroup in multiples of kPartUnit, in which 32 bits hold sums of every scale from 2^-64 to 2^119.
+constexpr int kNear = 4;
+constexpr int kPartExponent = 40;
+constexpr float kPartUnit = 0x1p40f;
+constexpr float kNothing = -1000.0f;  // h of a row that has seen nothing
+
+__device__ __forceinline__ int exponent_of(float x) { return (int)(__builtin_bit_cast(uint32_t, x) >> 23 & 0xff) - 127; }
+__device__ __forceinline__ int far_unit(float h) { return (int)ceilf(h) - 15; }  // its exponent
+
 
 template <bool HALF>  // nearest, ties to even
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {

@@ -14,7 +14,7 @@ struct Parts {
   // Pairs of a unit and a kv head are numbered heads first and the last units first. The first `whole` of them are not cut, each of
   // the others is, into at most `splits` stretches.
   int whole, splits;
-  float* sums;   // [pair - whole][split][row][dim]
+  float* sums;   // [pair - whole][split][row][dim]; in multiples of kPartUnit where the cache has 8 bits
   float* stats;  // [pair - whole][split][row]{m, l}, m in units of log 2
 };
 
@@ -76,8 +76,8 @@ inline uint32_t workgroups(const KvCache& c, const Parts& parts) {
 
 }  // namespace
 
-// Joins the stretches of every row: kv_attention.hip. `tile`: a unit's rows; `lift`: what the kernel added to m.
-hipError_t launch_join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int tile, float lift, int head_dim, bool half, hipStream_t stream);
+// Joins the stretches of every row: kv_attention.hip. `tile`: a unit's rows; `lift`: what the kernel added to m; `sum_unit`: what the sums are multiples of.
+hipError_t launch_join(const KvCache& c, const KvBatch& b, const KvAttend& a, const Parts& parts, int tile, float lift, float sum_unit, int head_dim, bool half, hipStream_t stream);
 
 }  // namespace amem
 #endif

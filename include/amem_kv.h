@@ -113,7 +113,10 @@ int amem_kv_append(const amem_kv_cache* cache, const amem_kv_batch* batch, const
  * if causal, and p > i - window if window > 0. lse, where given, is the natural logarithm of the sum of
  * exp(scale q.k_p). A row that sees nothing, or nothing but scores of -infinity, gives zeros and lse
  * -infinity. What is hidden from a row does not reach it, infinities and NaN included. Weights are rounded to 16 bits
- * (bf16 where the cache is bf16, else fp16) before they meet the values; sums have 32. `out` may be q itself.
+ * (bf16 where the cache is bf16, else fp16) before they meet the values; sums have 32. 8 bits: where the scales of the values
+ * lie further apart than 2^4 from the first ones, the products of weights and scales are rounded in place of the weights, so that only
+ * products far below a row's largest lose bits. Weights below 2^-126 of the largest count as zero, which asks for scales within 2^100 of each other.
+ * Sums of bf16 values stay finite while 2^7 * context * |v| does. `out` may be q itself.
  * The queries' rows have to be in the cache already: append first, then attend, on one stream. */
 typedef struct amem_kv_attention_args {
   uint64_t q, out;               /* [token][head][dim], like k in append */

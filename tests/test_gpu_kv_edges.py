@@ -8,7 +8,7 @@ import pytest
 from asystem_amem_amd import kv
 from tests import kv_oracle as O
 from tests.kv_case import KINDS, Arena, Case
-from tests.test_gpu_kv import TYPES, check_attend, poison
+from tests.test_gpu_kv import HALF, TYPES, check_attend, near, poison, run_attend
 
 pytestmark = pytest.mark.gpu
 
@@ -90,4 +90,111 @@ def test_the_widest_windows(arena, window, causal):
     for lengths in ([(4, 2), (1, 1300), (3, 1)], [(70, 33), (40, 1300), (300, 280)]):
         case = Case(arena, lengths, dim=64, q_heads=4, kv_heads=2, page=16, seed=34).upload()
         check_attend(case, case.rows(4), causal, window)
+        arena.reset()
+
+
+FAR, NEAR, LATE = 2.0 ** -33, 2.0 ** -25, 2.0 ** -25
+
+
+def check_scaled(case, q, step):
+    """Values in e4m3 of scales that may be far apart. Beside the roundings of weights, scores and result: a product of weight and scale far below
+    the largest loses bits, to steps of 2^-33 of the largest at most, as fp16 has them for numbers whose largest is at least 2^8; or, while all scales
+    are within 2^8 of each other (NEAR), a weight does, whose scale may be 2^8 of the largest product's; times codes of up to 448, for each
+    position. Where near scales go before far ones the largest product is known within 2^15 at first: 2^8 of scales, and 2^7 of weights (LATE)."""
+    got, lse = run_attend(case, q)
+    group, d = case.q_heads // case.kv_heads, case.dim
+    for s, (n, c) in enumerate(case.lengths):
+        rows, seen = slice(case.cu[s], case.cu[s] + n), case.visible(s, True, 0)
+        p = np.arange(c)
+        page, block = case.table[s, p // case.page], p % case.page // case.block
+        for h in range(case.q_heads):
+            k, v = case.gathered(s, h // group)
+            x = O.decode(q[rows, h], case.kind)
+            out, l, size, top = O.attend(x, k, v, d ** -0.5, seen)
+            with np.errstate(all="ignore"):
+                weight = np.where(seen, np.exp(x @ k.T * d ** -0.5 - l[:, None]), 0)
+            most = (weight * case.v_scale[page, h // group, block].astype(np.float64)).max(1)
+            lost = c * 448 * step * most
+            score = d * 2.0 ** -23 * top + 2.0 ** -18
+            near(got[rows, h], out, case.kind, (HALF["f16"] + score)[:, None] * size + lost[:, None])
+            assert (np.abs(lse[rows, h] - l) <= score + 2.0 ** -22 * np.abs(l)).all()
+    return got
+
+
+def scaled_case(arena, lengths, dim, kind, exponents, bias, seed=35, **more):
+    """Blocks take the scales 2^e in turn, and keys make the first of them lose `bias` (of the natural logarithm of a weight) to the others."""
+    case = Case(arena, lengths, dim=dim, q_heads=4, kv_heads=2, kind=kind, eight=True, page=32, block=16, seed=seed, **more)
+    case.v &= 0xDF                                    # codes of at most 28, so that weighted means stay inside the types
+    case.k_scale[:] = 2.0 ** -6
+    case.k[..., 0] = O.e4m3_code(np.float64(448))
+    for s, (n, c) in enumerate(case.lengths):
+        for i, p in enumerate(range(0, c, 16)):
+            page, at = case.table[s, p // 32], p % 32
+            case.v_scale[page, :, at // 16] = 2.0 ** exponents[i % len(exponents)]
+            if i % len(exponents) == 0:
+                case.k[page, :, at:at + 16, 0] = O.e4m3_code(np.float64(-448))
+    case.upload()
+    q = case.r.standard_normal((case.tokens, 4, dim)) * 0.5
+    q[..., 0] = bias * dim ** 0.5 / 14                # the first dim's part of a score is bias / 2, or - bias / 2
+    return case, O.encode(q, kind)
+
+
+FORMS = {"token": [(1, 700)], "draft": [(5, 330)], "prompt": [(100, 700)], "long": [(1, 5000), (2, 900)], "long prompt": [(300, 1300)]}
+
+
+@pytest.mark.parametrize("dim,kind", [(64, "bf16"), (64, "f16"), (128, "bf16"), (128, "f16"), (256, "bf16"), (256, "f16")])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("exponents,bias", [((0, -14), 0), ((0, -14), 9.7), ((0, -14), 30), ((-14, 0), 5), ((9, -3, -9, 2), 12), ((-3, -7), 4), ((-3, -11), 4), ((-3, -12), 4), ((-7, -7, -7, -7, -3), 2),
+                                            ((-7, -7, -7, -7, -2), 2)])
+def test_scales_of_values_far_apart(arena, form, dim, kind, exponents, bias):
+    """A large scale takes no bits of small ones that have the weight, on either side of the border between scales that are near and far."""
+    case, q = scaled_case(arena, FORMS[form], dim, kind, exponents, bias)
+    check_scaled(case, q, NEAR if max(exponents) - min(exponents) <= 8 else FAR)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("exponents,bias", [((0, -30), 0), ((0, -30), 21), ((0, -30), 60), ((50, -50), 80), ((-50, 50), 3), ((119, 119), 1), ((119, 30), 40),
+                                            ((-64, -64), 1), ((-64, 0), 30), ((30, -30, 0, 5, -64, 10), 30)])
+def test_scales_of_the_whole_range(arena, form, dim, exponents, bias):
+    case, q = scaled_case(arena, FORMS[form], dim, "bf16", exponents, bias)
+    check_scaled(case, q, NEAR if max(exponents) - min(exponents) <= 8 else FAR)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("form", ["draft", "prompt", "long prompt"])
+def test_hidden_scales_and_bad_values_among_scales_far_apart(arena, form, kind):
+    """A scale of rows that come later is of no account to those before; NaN that some rows see, in a cache whose scales are far apart."""
+    case, q = scaled_case(arena, FORMS[form], 128, kind, (0, -14), 12, seed=36)
+    n, c = case.lengths[0]
+    last = c - 1
+    page, block = case.table[0, last // 32], last % 32 // 16
+    case.v_scale[page, :, block] = 2.0 ** 100
+    case.v[page, :, last % 32] = 0                     # the last position's block is huge; but for that position it holds zeros
+    for p in range(last // 16 * 16, last):
+        case.v[page, :, p % 32] = 0
+    case.v[page, 1, last % 32, 7] = 0x7F
+    poison(case, 0, c - n + 1, v=0x7F)
+    case.upload()
+    got = O.decode(check_scaled(case, q, FAR), kind)
+    assert np.isfinite(got[0]).all() and np.isnan(got[1]).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("far", [-40, 40])
+def test_scales_that_part_late(arena, form, dim, far):
+    """Near ones for half of the context, then one block far from them: with little weight, and with all of it for the last rows."""
+    for value in (-448, 448):
+        lengths = FORMS[form]
+        case, q = scaled_case(arena, lengths, dim, "bf16", (0, -3), 6, seed=37)
+        for s, (n, c) in enumerate(lengths):
+            p = c // 2 // 16 * 16
+            page, at = case.table[s, p // 32], p % 32
+            case.v_scale[page, :, at // 16] = 2.0 ** far
+            case.k[page, :, at:at + 16, 1] = O.e4m3_code(np.float64(value))
+        case.upload()
+        x = O.decode(q, "bf16")
+        x[..., 1] = 4 * dim ** 0.5
+        check_scaled(case, O.encode(x, "bf16"), LATE)
         arena.reset()
