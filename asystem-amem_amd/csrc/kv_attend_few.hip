@@ -479,25 +479,12 @@ int blocks_of(int group, int max_tokens, int head_dim) {
   return rows <= 16 ? 1 : rows <= 32 || head_dim > 64 ? 2 : rows <= 48 ? 3 : 4;
 }
 
-// Workgroups are bound by what a compute unit can load, or all of them by the memory. The figures are fitted to times of 25
-// calls with 1 to 32 stretches (8 to 512 pairs, contexts of 2000 to 131072, equal and not), 4 % above the best on average. Uncut, and
-// cut (us): 128 dims of e4m3, 33 sequences of 1000 to 4000 positions 50 and 44; 65 of 4000 126 and 102; 3 of 30000 270 and 40.
-Cut cut_of(int head_dim, bool eight, int blocks) {
-  const int fit = head_dim == 256 && (!eight || blocks > 1) ? 256 : head_dim == 64 && !eight && blocks == 1 ? 768 : 512;
-  const int bytes = head_dim * (eight ? 2 : 4);  // of a position
-  // Stretches of what four waves take at once: with 256 everywhere a token of 1000 positions takes 10.4 us instead of 9.7, 16.6 instead of 14.0 with 256
-  // dims in 16 bits; multiples of 256 for longer stretches: 24 tokens of 4000 positions 45 us, and 49 in multiples of 128.
-  // One token of 256 positions takes 6.9 us uncut and 8.4 cut, of 300 9.0 and 9.5, of 500 10.4 in two stretches and 9.2 in four.
-  const int least = head_dim == 64 && eight && blocks == 1 ? 256 : 128;
-  return {fit, 4, 2, least, 256, 37, 39, 33, 79, 5500 / bytes, 12000 / bytes, 34 * blocks * (head_dim + 2) / bytes, 384};
-}
-
 void plan(const KvCache& c, const KvBatch& b, int group, int head_dim, bool eight, int blocks, const KvAttend& a, Parts* few) {
   int64_t span = b.max_context;
   const int64_t seen = (int64_t)a.window + (16 * blocks) / group + 1 + 64;
   if (a.causal && a.window && seen < span) span = seen;  // else a window has no far end
   few->units = units_of(b, group, 16 * blocks);
-  cut_pairs(cut_of(head_dim, eight, blocks), c, span, true, few);
+  cut_pairs(cut_of_few(head_dim, eight, blocks), c, span, true, few);
 }
 
 template <int D, bool HALF, bool EIGHT, int NB>
@@ -531,7 +518,7 @@ hipError_t launch_dims(const KvCache& c, const KvBatch& b, const KvAttend& a, bo
 
 uint64_t kv_attend_few_workspace(const KvCache& c, const KvBatch& b, int q_heads, int max_tokens, int head_dim) {
   const int group = q_heads / c.kv_heads, blocks = blocks_of(group, max_tokens, head_dim);
-  return parts_bytes(cut_of(head_dim, c.block_shift > 0, blocks), (int64_t)units_of(b, group, 16 * blocks) * c.kv_heads, b.max_context, 16 * blocks, head_dim);
+  return parts_bytes(cut_of_few(head_dim, c.block_shift > 0, blocks), (int64_t)units_of(b, group, 16 * blocks) * c.kv_heads, b.max_context, 16 * blocks, head_dim);
 }
 
 hipError_t launch_kv_attend_few(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream) {

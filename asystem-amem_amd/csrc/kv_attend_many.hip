@@ -428,11 +428,6 @@ Shape shape_of(const KvCache& c, const KvBatch& b, int group, int head_dim) {
   return {128, 512, false};
 }
 
-// Two workgroups of a compute unit take 4/3 of the time of one, three 5/3; a part of 128 rows costs about a position's work
-// once all compute units write theirs. Uncut, and cut (us): 32 heads over 8, 128 dims, 16 bits, 1200 rows of 8192 positions 254 and
-// 226; 4500 of 16384 1262 and 1062; 256 dims, 8 bits, 1100 rows of 16000 positions 1290 and 674.
-Cut cut_of(const Shape& shape) { return {shape.fit, 2, 0, 512, kTile, 66, 33, 0, 100, 0, 150, shape.rows * 100 / 128}; }
-
 void plan(const KvCache& c, const KvBatch& b, int group, const Shape& shape, const KvAttend& a, Parts* parts) {
   parts->units = units_of(b, group, shape.rows);
   int64_t span = b.max_context;
@@ -440,7 +435,7 @@ void plan(const KvCache& c, const KvBatch& b, int group, const Shape& shape, con
   if (a.causal && a.window && seen < span) span = seen;  // else a window has no far end
   // the last rows of a prompt see more than the first ones
   const bool even = !a.causal || a.window || 2 * (int64_t)a.max_tokens <= b.max_context;
-  cut_pairs(cut_of(shape), c, span, even, parts);
+  cut_pairs(cut_of_many(shape.rows, shape.fit), c, span, even, parts);
 }
 
 template <int D, int W, int R>
@@ -476,7 +471,7 @@ hipError_t launch(const KvCache& c, const KvBatch& b, const KvAttend& a, bool ha
 uint64_t kv_attend_many_workspace(const KvCache& c, const KvBatch& b, int q_heads, int head_dim) {
   const int group = q_heads / c.kv_heads;
   const Shape shape = shape_of(c, b, group, head_dim);
-  return parts_bytes(cut_of(shape), (int64_t)units_of(b, group, shape.rows) * c.kv_heads, b.max_context, shape.rows, head_dim);
+  return parts_bytes(cut_of_many(shape.rows, shape.fit), (int64_t)units_of(b, group, shape.rows) * c.kv_heads, b.max_context, shape.rows, head_dim);
 }
 
 hipError_t launch_kv_attend_many(const KvCache& c, const KvBatch& b, const KvAttend& a, int head_dim, bool half, bool eight, hipStream_t stream) {

@@ -21,6 +21,24 @@ struct Cut {
   int shorter = 0;       // positions: what is shorter is not cut
 };
 
+// Few rows, `blocks` of 16 of them. Workgroups are bound by what a compute unit can load, or all of them by the memory. The figures are fitted to times of 25
+// calls with 1 to 32 stretches (8 to 512 pairs, contexts of 2000 to 131072, equal and not), 4 % above the best on average. Uncut, and
+// cut (us): 128 dims of e4m3, 33 sequences of 1000 to 4000 positions 50 and 44; 65 of 4000 126 and 102; 3 of 30000 270 and 40.
+inline Cut cut_of_few(int head_dim, bool eight, int blocks) {
+  const int fit = head_dim == 256 && (!eight || blocks > 1) ? 256 : head_dim == 64 && !eight && blocks == 1 ? 768 : 512;
+  const int bytes = head_dim * (eight ? 2 : 4);  // of a position
+  // Stretches of what four waves take at once: with 256 everywhere a token of 1000 positions takes 10.4 us instead of 9.7, 16.6 instead of 14.0 with 256
+  // dims in 16 bits; multiples of 256 for longer stretches: 24 tokens of 4000 positions 45 us, and 49 in multiples of 128.
+  // One token of 256 positions takes 6.9 us uncut and 8.4 cut, of 300 9.0 and 9.5, of 500 10.4 in two stretches and 9.2 in four.
+  const int least = head_dim == 64 && eight && blocks == 1 ? 256 : 128;
+  return {fit, 4, 2, least, 256, 37, 39, 33, 79, 5500 / bytes, 12000 / bytes, 34 * blocks * (head_dim + 2) / bytes, 384};
+}
+
+// Many rows, `rows` of a unit. Two workgroups of a compute unit take 4/3 of the time of one, three 5/3; a part of 128 rows costs about a position's work
+// once all compute units write theirs. Uncut, and cut (us): 32 heads over 8, 128 dims, 16 bits, 1200 rows of 8192 positions 254 and
+// 226; 4500 of 16384 1262 and 1062; 256 dims, 8 bits, 1100 rows of 16000 positions 1290 and 674.
+inline Cut cut_of_many(int rows, int fit) { return {fit, 2, 0, 512, 64, 66, 33, 0, 100, 0, 150, rows * 100 / 128}; }
+
 // The first `whole` pairs stay whole, each of the others becomes at most `splits` stretches of `stretch` positions.
 struct CutInto {
   int whole, splits, stretch;

@@ -16,3 +16,7 @@ def run_driver(tmp_path, source):
 
 def test_units_of_any_offsets_stay_inside_the_tensors(tmp_path):
     run_driver(tmp_path, "unit_driver.cpp")
+
+
+def test_cuts_with_the_kernels_own_figures(tmp_path):
+    run_driver(tmp_path, "cut_rules_driver.cpp")
