@@ -85,7 +85,7 @@ int check_batch(const char* what, const amem_kv_batch* b, const KvCache& c, bool
     NEED(b->context && b->context % 4 == 0 && b->cu_tokens % 4 == 0, "addresses of the lengths");
     NEED(b->table_pages == 0 || (b->page_table && b->page_table % 4 == 0), "address of the page table");
   }
-  if (!b->cu_tokens && addresses)
+  if (!b->cu_tokens)
     NEED((int64_t)b->sequences * b->max_tokens == b->tokens, "without cu_tokens there are sequences * max_tokens rows");
   *out = {(const int*)(uintptr_t)b->page_table, (const int*)(uintptr_t)b->context, (const int*)(uintptr_t)b->cu_tokens,
           b->table_stride, b->sequences, b->table_pages, b->tokens, b->max_tokens, b->max_context};

@@ -190,3 +190,15 @@ def test_packed_arguments_are_the_structures():
     numbers = list(range(1, 16))
     a = kv.AttentionArgs.from_buffer_copy(kv._attention_args(*numbers))
     assert [getattr(a, f[0]) for f in a._fields_] == numbers and C.sizeof(a) == len(kv._attention_args(*numbers))
+
+
+@pytest.mark.parametrize("sequences,tokens,max_tokens", [(3, 20, 7), (1 << 15, 1 << 15, 1 << 15), (1 << 16, 1 << 19, 1 << 19)])
+def test_the_workspace_of_rows_that_do_not_add_up_is_refused(lib, sequences, tokens, max_tokens):
+    """As by the call itself; their number of units can pass 32 bits."""
+    cache, batch, app, att = valid()
+    batch.sequences, batch.tokens, batch.max_tokens = sequences, tokens, max_tokens
+    kv.load()
+    n = C.c_uint64()
+    assert lib.amem_kv_attention_workspace(C.byref(cache), C.byref(batch), 16, C.byref(n)) == 0       # with offsets: a guide
+    batch.cu_tokens = 0
+    assert lib.amem_kv_attention_workspace(C.byref(cache), C.byref(batch), 16, C.byref(n)) == INVALID
