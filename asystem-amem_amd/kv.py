@@ -15,6 +15,7 @@ for instance. Arguments that do not fit raise ValueError before anything is enqu
 raises KvError.
 """
 import ctypes as C
+import operator
 import struct
 
 from . import binding
@@ -121,6 +122,19 @@ def _is(t, dtype, device, what):
         raise ValueError("%s is on another device than the cache" % what)
 
 
+def _int32(**numbers):
+    """The numbers as they are, which ctypes would cut to 32 bits without a word."""
+    out = []
+    for what, x in numbers.items():
+        try:
+            x = operator.index(x)
+        except TypeError:
+            raise ValueError("%s is no whole number" % what) from None
+        _need(-1 << 31 <= x < 1 << 31, "%s does not fit 32 bits" % what)
+        out.append(x)
+    return out
+
+
 class Cache:
     """Keys and values [pages, heads, slots, dim], with equal strides and contiguous dims; e4m3 with their scales, float32
     [pages, heads, blocks], blocks contiguous."""
@@ -131,6 +145,7 @@ class Cache:
         kind, block = _kind(k), 0
         _need(kind >= 0, "k is not bfloat16, float16 or float8_e4m3fn")
         pages, heads, slots, dim = k.shape
+        _int32(pages=pages, heads=heads, slots=slots, dim=dim)
         at = k.stride()
         _need(at[3] == 1 or dim == 1, "the dims of k are not contiguous")
         device = _device(k)
@@ -178,6 +193,7 @@ class Batch:
             _need(page_slots, "max_context or page_slots is needed")
             max_context = page_table.shape[1] * page_slots
         pages = page_table.shape[1]
+        n, pages, tokens, max_tokens, max_context = _int32(sequences=n, pages=pages, tokens=tokens, max_tokens=max_tokens, max_context=max_context)
         stride = page_table.stride()[0] if n > 1 else pages
         _need(stride >= pages, "the rows of page_table overlap")
         self.info = BatchInfo(page_table.data_ptr(), context.data_ptr(), cu_tokens.data_ptr() if cu_tokens is not None else 0,
@@ -271,7 +287,7 @@ def append(cache, batch, k, v, q=None, q_out=None, rotation=None, positions=None
 def attention_workspace(cache, batch, q_heads):
     """Bytes of workspace that `attention` needs for these sizes."""
     n = C.c_uint64()
-    _call("amem_kv_attention_workspace", cache._ref, batch._ref, q_heads, C.byref(n))
+    _call("amem_kv_attention_workspace", cache._ref, batch._ref, *_int32(q_heads=q_heads), C.byref(n))
     return n.value
 
 

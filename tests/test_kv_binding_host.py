@@ -151,3 +151,29 @@ def test_cuts_fit_the_workspace(tmp_path):
     r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, r.stdout + r.stderr
     assert "ok" in r.stdout
+
+
+@pytest.mark.parametrize("changed", [
+    dict(max_context=(1 << 32) + 64), dict(max_context=1 << 31), dict(max_tokens=(1 << 32) + 2), dict(tokens=(1 << 32) + 5), dict(tokens=-(1 << 32)), dict(max_context=64.0),
+    dict(max_tokens="2"), dict(max_context=None, page_slots=1 << 30)])
+def test_numbers_of_a_batch_are_not_cut_to_32_bits(changed):
+    with pytest.raises(ValueError):
+        batch(**changed)
+
+
+def test_numbers_of_a_batch_arrive():
+    b = batch(tokens=5, max_tokens=2, max_context=(1 << 31) - 1)
+    assert (b.info.tokens, b.info.max_tokens, b.info.max_context, b.info.sequences, b.info.table_pages) == (5, 2, (1 << 31) - 1, 3, 4)
+
+
+def test_a_cache_of_too_many_pages_is_refused():
+    k = Tensor(((1 << 32) + 9, 2, 16, 64))
+    with pytest.raises(ValueError):
+        kv.Cache(k, k)
+
+
+@pytest.mark.parametrize("q_heads", [(1 << 32) + 4, 4.0, None])
+def test_the_workspace_of_heads_that_are_no_number_is_refused(lib, q_heads):
+    assert kv.attention_workspace(cache(), batch(), 4) >= 0
+    with pytest.raises(ValueError):
+        kv.attention_workspace(cache(), batch(), q_heads)
