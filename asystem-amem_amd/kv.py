@@ -260,6 +260,8 @@ def append(cache, batch, k, v, q=None, q_out=None, rotation=None, positions=None
                 or q.device != device or q_out.device != device):
             _refuse_rows(shape, dtype, device, q=q, q_out=q_out)
         q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
+    elif q_out is not None:
+        raise ValueError("q_out without q")
     cos = sin = where = apart = dim = interleaved = rows = axes = 0
     sections = (0, 0, 0, 0)
     if rotation is not None:

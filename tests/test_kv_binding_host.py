@@ -177,3 +177,8 @@ def test_the_workspace_of_heads_that_are_no_number_is_refused(lib, q_heads):
     assert kv.attention_workspace(cache(), batch(), 4) >= 0
     with pytest.raises(ValueError):
         kv.attention_workspace(cache(), batch(), q_heads)
+
+
+def test_a_place_for_queries_without_queries_is_refused():
+    with pytest.raises(ValueError):
+        kv.append(cache(), batch(), Tensor((5, 2, 64)), Tensor((5, 2, 64)), q_out=Tensor((5, 4, 64)))
