@@ -23,6 +23,14 @@ namespace {
 
 constexpr int kTile = 64;  // positions
 
+template <bool HALF>
+__device__ __forceinline__ u32x4 times_zero(u32x4 x) {  // zeros, NaN where an element is not finite
+  constexpr uint32_t e = HALF ? 0x7c00 : 0x7f80;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = ((x[i] & e) == e ? 0x7fffu : 0) | ((x[i] >> 16 & e) == e ? 0x7fff0000u : 0);
+  return x;
+}
+
 // D dims, 16 bits of fp16 (HALF) or bf16, a cache of e4m3 (EIGHT).
 // W waves with R rows each, 32 or 16.
 template <int D, bool HALF, bool EIGHT, int W, int R>
@@ -85,11 +93,14 @@ __global__ __launch_bounds__(W * kWave, (D == 64 ? 3 : 2)) void attend_many(KvCa
     row_range(a, q, token, row_from, row_to);
     const uint16_t* p = a.q + (q.row + token) * a.q_token + head * a.q_head;
 #pragma unroll
-    for (int t = 0; t < D / kSteps; ++t) qr[t] = *(const u32x4*)(p + dim_at(t * kSteps + part * 8)) ^ (a.scale < 0 ? 0x80008000u : 0u);
+    for (int t = 0; t < D / kSteps; ++t) {
+      qr[t] = *(const u32x4*)(p + dim_at(t * kSteps + part * 8));
+      qr[t] = a.scale == 0 ? times_zero<HALF>(qr[t]) : qr[t] ^ (a.scale < 0 ? 0x80008000u : 0u);
+    }
   }
   // weights are exp2(score * factor - top), so the factor has to be above zero for the largest score to give the largest
-  // product: its sign is in the queries, and a scale of zero becomes one that is as good as zero
-  const float factor = fmaxf(fabsf(a.scale) * kLog2e, 0x1p-100f);
+  // product: the scale's sign, and a scale of zero, are in the queries
+  const float factor = a.scale == 0 ? 1.0f : fabsf(a.scale) * kLog2e;
 
   float m = -kInf, l = 0;
   Result sum[kBlocks];

@@ -198,3 +198,22 @@ def test_scales_that_part_late(arena, form, dim, far):
         x[..., 1] = 4 * dim ** 0.5
         check_scaled(case, O.encode(x, "bf16"), LATE)
         arena.reset()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, 2.0 ** -140, -2.0 ** -110])
+def test_a_scale_of_zero_or_hardly_more(arena, scale):
+    """All weights are equal, whatever the size of the scores; an infinite one times zero is NaN."""
+    for lengths in ([(1, 90)], [(5, 200)], [(70, 200)], [(300, 700)]):
+        n, c = lengths[0]
+        for infinite in (False, True):
+            case = Case(arena, lengths, dim=64, q_heads=2, kv_heads=1, page=16, seed=38)
+            case.k = O.encode(O.decode(case.k, "bf16") * 2.0 ** 100, "bf16")
+            if infinite:
+                page, slot = case.table[0, (c - 1) // 16], (c - 1) % 16
+                case.k[page, 0, slot, 0] = 0x7F80                      # the last row sees it
+            case.upload()
+            got, _ = check_attend(case, case.rows(2), scale=scale)
+            assert np.isfinite(O.decode(got, "bf16")[:n - 1]).all()
+            if infinite and scale == 0:
+                assert np.isnan(O.decode(got, "bf16")[n - 1]).all()
+            arena.reset()
