@@ -98,11 +98,51 @@ int check_rows(const char* what, const char* why, uint64_t at, int64_t token, in
   return 0;
 }
 
-// Runs `launch` with the cache's device current, unless the process is paused. The registry's lock is held
-// meanwhile: a pause takes it for its whole length and waits for the device before it releases anything, so what
-// gets enqueued here has run by then, and a call made during a pause finds the process paused.
-template <class Launch>
-int on_device(const char* what, int device, hipStream_t stream, Launch launch) {
+// What a call may touch: bytes from `at` on.
+struct Span {
+  uint64_t at, bytes;
+};
+struct Spans {  // of one call, at most 14
+  Span of[16];
+  int count = 0;
+  void add(const Span& span) {
+    if (span.bytes) of[count++] = span;
+  }
+};
+
+// Of a tensor of three outer dimensions, strides in bytes, with `inner` contiguous bytes; nothing if it is empty or absent.
+Span span_of(const void* at, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t inner) {
+  if (!at || n0 < 1 || n1 < 1 || n2 < 1 || inner < 1) return {0, 0};
+  return {(uint64_t)(uintptr_t)at, (uint64_t)((n0 - 1) * s0 + (n1 - 1) * s1 + (n2 - 1) * s2 + inner)};
+}
+
+bool tracked(const Ctx& c, const Span& span) {
+  for (const auto& table : c.allocTable) {  // regions are apart, so the last one that begins before the span's end decides
+    auto it = table.lower_bound(span.at + span.bytes);
+    if (it != table.begin() && (--it)->first + it->second.allocSz > span.at) return true;
+  }
+  return false;
+}
+
+void cache_spans(const KvCache& c, const KvBatch& b, int head_dim, bool eight, Spans* out) {
+  const int64_t slots = (int64_t)1 << c.page_shift, element = eight ? 1 : 2;
+  for (const uint8_t* at : {c.k, c.v}) out->add(span_of(at, c.pages, c.page_stride, c.kv_heads, c.head_stride, slots, c.slot_stride, head_dim * element));
+  for (const float* at : {c.k_scale, c.v_scale})
+    out->add(span_of(at, c.pages, c.scale_page_stride * 4, c.kv_heads, c.scale_head_stride * 4, 1, 0, 4 * (slots >> c.block_shift)));
+  out->add(span_of(b.page_table, b.sequences, b.table_stride * 4, 1, 0, 1, 0, (int64_t)b.table_pages * 4));
+  out->add(span_of(b.context, 1, 0, 1, 0, 1, 0, (int64_t)b.sequences * 4));
+  out->add(span_of(b.cu_tokens, 1, 0, 1, 0, 1, 0, ((int64_t)b.sequences + 1) * 4));
+}
+
+Span rows_span(const uint16_t* at, int64_t token, int64_t head, int tokens, int heads, int head_dim) {
+  return span_of(at, tokens, token * 2, heads, head * 2, 1, 0, head_dim * 2);
+}
+
+// Runs `launch` with the cache's device current, unless the process is paused and some of `spans()` lies in memory that the
+// engine tracks. The registry's lock is held meanwhile: a pause takes it for its whole length and waits for the device before it
+// releases anything, so what gets enqueued here has run by then, and a call made during a pause finds the process paused.
+template <class MakeSpans, class Launch>
+int on_device(const char* what, int device, hipStream_t stream, MakeSpans spans, Launch launch) {
   if (!gpu_present()) {
     LOGGER(ERROR, "%s: no HIP device", what);
     return (int)hipErrorNoDevice;
@@ -120,8 +160,13 @@ int on_device(const char* what, int device, hipStream_t stream, Launch launch) {
     lk = std::unique_lock<std::mutex>(c->structure);
     std::lock_guard<std::mutex> lf(c->fields);
     if (c->paused) {
-      LOGGER(WARN, "%s: groupID:%d pid:%d is paused: refused", what, amem_groupID_value(), getpid());
-      return (int)hipErrorInvalidValue;
+      const Spans s = spans();
+      for (int i = 0; i < s.count; ++i)
+        if (tracked(*c, s.of[i])) {
+          LOGGER(WARN, "%s: groupID:%d pid:%d is paused, and the tensor at %llx lies in tracked memory: refused", what, amem_groupID_value(),
+                 getpid(), (unsigned long long)s.of[i].at);
+          return (int)hipErrorInvalidValue;
+        }
     }
   }
   if (device != current)
@@ -185,7 +230,21 @@ int amem_kv_append(const amem_kv_cache* cache, const amem_kv_batch* batch, const
     p.axes = a->axes;
   }
   if (!b.tokens || !b.sequences) return 0;
-  return on_device(what, cache->device, (hipStream_t)stream, [&] {
+  auto spans = [&] {
+    Spans s;
+    const int dim = cache->head_dim;
+    cache_spans(c, b, dim, eight, &s);
+    s.add(rows_span(p.k, p.k_token, p.k_head, b.tokens, c.kv_heads, dim));
+    s.add(rows_span(p.v, p.v_token, p.v_head, b.tokens, c.kv_heads, dim));
+    s.add(rows_span(p.q, p.q_token, p.q_head, b.tokens, p.q_heads, dim));
+    s.add(rows_span(p.q_out, p.qo_token, p.qo_head, b.tokens, p.q_heads, dim));
+    if (pairs) {
+      for (const float* at : {p.cos, p.sin}) s.add(span_of(at, p.table_rows, pairs * 4, 1, 0, 1, 0, pairs * 4));
+      s.add(span_of(p.positions, p.axes, p.positions_stride * 4, 1, 0, 1, 0, (int64_t)b.tokens * 4));
+    }
+    return s;
+  };
+  return on_device(what, cache->device, (hipStream_t)stream, spans, [&] {
     return launch_kv_append(c, b, p, cache->head_dim, a->type == AMEM_KV_F16, eight, (hipStream_t)stream);
   });
 }
@@ -229,7 +288,17 @@ int amem_kv_attention(const amem_kv_cache* cache, const amem_kv_batch* batch, co
   const KvAttend p = {(const uint16_t*)(uintptr_t)a->q, (uint16_t*)(uintptr_t)a->out, (float*)(uintptr_t)a->lse,
                       (uint8_t*)(uintptr_t)a->workspace, a->q_token_stride, a->q_head_stride, a->out_token_stride,
                       a->out_head_stride, a->scale, a->q_heads, a->causal != 0, a->window, batch->max_tokens};
-  return on_device(what, cache->device, (hipStream_t)stream, [&] {
+  auto spans = [&] {
+    Spans s;
+    const int dim = cache->head_dim;
+    cache_spans(c, b, dim, eight, &s);
+    s.add(rows_span(p.q, p.q_token, p.q_head, b.tokens, p.q_heads, dim));
+    s.add(rows_span(p.out, p.out_token, p.out_head, b.tokens, p.q_heads, dim));
+    s.add(span_of(p.lse, 1, 0, 1, 0, 1, 0, (int64_t)b.tokens * p.q_heads * 4));
+    if (need) s.add(span_of(p.workspace, 1, 0, 1, 0, 1, 0, (int64_t)need));
+    return s;
+  };
+  return on_device(what, cache->device, (hipStream_t)stream, spans, [&] {
     return launch_kv_attend(c, b, p, cache->head_dim, a->type == AMEM_KV_F16, eight, (hipStream_t)stream);
   });
 }

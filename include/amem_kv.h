@@ -6,16 +6,16 @@
  *
  * The cache may lie in any device memory. In memory that the engine tracks (amem_vmm_alloc +
  * amem_add_alloc_info) a pause releases it and a resume brings back the same bytes at the same
- * addresses; with 8 bits there is half as much to park. While the process is paused the calls
- * below are refused, since their pages may have no memory behind them, and a pause waits for those
- * already enqueued. A captured graph is the caller's: it must not be replayed while paused.
+ * addresses; with 8 bits there is half as much to park. While the process is paused, calls that name
+ * an address in tracked memory are refused, since there may be no memory behind it; a pause waits for those
+ * already enqueued. A captured graph is the caller's: one that uses tracked memory must not be replayed while paused.
  *
  * Conventions. Device addresses are uint64_t. Every call only enqueues work on `stream` (a
  * hipStream_t of the cache's device, NULL for its default stream) and may be captured; nothing is
  * allocated, copied to the host or kept, so that tensors have to live until the stream is done with them. Everything that addresses name has to lie on the cache's
  * device, which need not be the current one. Results are the same, bit for bit, from call to call. Returns
- * 0, hipErrorInvalidValue (1) for arguments that are refused (one ERROR line says which) and while
- * paused, or another HIP error. Two calls that may run at the same time need different workspaces,
+ * 0, hipErrorInvalidValue (1) for arguments that are refused (one ERROR line says which) and for tracked
+ * memory while paused, or another HIP error. Two calls that may run at the same time need different workspaces,
  * and must not write the same pages or read pages that the other writes.
  *
  * Lengths, positions, page numbers and rows live in device memory and cannot be refused on the host. Where they

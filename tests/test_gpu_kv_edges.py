@@ -5,10 +5,11 @@ import ctypes as C
 import numpy as np
 import pytest
 
+from asystem_amem_amd import binding as B
 from asystem_amem_amd import kv
 from tests import kv_oracle as O
 from tests.kv_case import KINDS, Arena, Case
-from tests.test_gpu_kv import HALF, TYPES, check_attend, near, poison, run_attend
+from tests.test_gpu_kv import HALF, TYPES, check_append, check_attend, near, poison, run_attend
 
 pytestmark = pytest.mark.gpu
 
@@ -217,3 +218,28 @@ def test_a_scale_of_zero_or_hardly_more(arena, scale):
             if infinite and scale == 0:
                 assert np.isnan(O.decode(got, "bf16")[n - 1]).all()
             arena.reset()
+
+
+def test_memory_that_is_not_tracked_is_used_while_paused(gpu, fresh):
+    """A pause takes the communication buffers; a cache elsewhere is written and read meanwhile, with the same results."""
+    lib = fresh
+    arena, buffers = Arena(lib, 16 << 20), Arena(lib, 8 << 20)
+    try:
+        assert lib.amem_add_alloc_info(buffers.va, buffers.alloc, B.TYPE_LOCAL, 0, buffers.handle, -1, 0, None, B.CALLER_P2P) == 0
+        case = Case(arena, [(1, 2000), (40, 70)], dim=128, q_heads=4, kv_heads=2, eight=True, page=32, block=32, seed=39).upload()
+        q = case.rows(4)
+        one, l1 = run_attend(case, q)
+        assert lib.ncclPause(None) == 0
+        check_append(case, case.rows(2), case.rows(2), q, rotary=128)
+        check_attend(case, q)
+        case.args.workspace = buffers.va
+        case.args.workspace_bytes = 8 << 20
+        n = C.c_uint64()
+        assert lib.amem_kv_attention_workspace(C.byref(case.cache), C.byref(case.batch), 4, C.byref(n)) == 0 and n.value
+        assert lib.amem_kv_attention(C.byref(case.cache), C.byref(case.batch), C.byref(case.args), None) == 1
+        assert lib.ncclResume(None) == 0
+        assert lib.amem_kv_attention(C.byref(case.cache), C.byref(case.batch), C.byref(case.args), None) == 0
+        assert lib.amem_del_alloc_info(buffers.va, 0, 0) == 0
+    finally:
+        arena.free()
+        buffers.free()
