@@ -86,10 +86,12 @@ def load():
     """The library, with the entry points of include/amem_kv.h declared."""
     lib = binding.load()
     if not _entry:
+        found = {}
         for name, (res, args) in _SIGNATURES.items():
             fn = getattr(lib, name)
             fn.restype, fn.argtypes = res, args
-            _entry[name] = fn
+            found[name] = fn
+        _entry.update(found)     # all at once: another thread may be about to call
     return lib
 
 

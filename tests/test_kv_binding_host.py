@@ -182,3 +182,16 @@ def test_the_workspace_of_heads_that_are_no_number_is_refused(lib, q_heads):
 def test_a_place_for_queries_without_queries_is_refused():
     with pytest.raises(ValueError):
         kv.append(cache(), batch(), Tensor((5, 2, 64)), Tensor((5, 2, 64)), q_out=Tensor((5, 4, 64)))
+
+
+def test_entry_points_are_there_all_at_once(monkeypatch):
+    """Another thread that makes its first call meanwhile finds none of them, or all."""
+    class Library:
+        def __getattr__(self, name):
+            assert not kv._entry, "some of the entry points are already there"
+            return lambda *a: 0
+
+    monkeypatch.setattr(kv, "_entry", {})
+    monkeypatch.setattr(kv.binding, "load", Library)
+    kv.load()
+    assert sorted(kv._entry) == kv.kv_abi_names()
