@@ -13,9 +13,9 @@
 // by wave, to become operands. A tile's registers are loaded again for the next tile as soon as LDS has them.
 //
 // Measured, where reading alone reaches 6.6 TB/s: 64 single tokens of 2048 to 8192 positions, 32 heads over 8, 128 dims, e4m3: 704 MB in
-// 124 us, 5.7 TB/s; four of 32768 to 131072: 683 MB in 118 us, 5.8; 32 of 1024 to 4096, 16 heads each with its own keys, bf16: 675 MB in
-// 111 us, 6.1; five drafted tokens of 24 sequences, 64 heads over 8, 64 dims, fp16: 190 MB in 44 us, 4.3; one token of 1000 positions:
-// 9.7 us, 3 of them in the join: latency, of the length, then page numbers, then keys.
+// 127 us, 5.6 TB/s (136 where the scales of values are far apart); four of 32768 to 131072: 683 MB in 119 us, 5.7; 32 of 1024 to 4096, 16 heads each with
+// its own keys, bf16: 675 MB in 111 us, 6.1; five drafted tokens of 24 sequences, 64 heads over 8, 64 dims, fp16: 190 MB in 44 us, 4.3; one token
+// of 1000 positions: 9.2 us, 3 of them in the join: latency, of the length, then page numbers, then keys.
 #include <algorithm>
 
 #include "kv_parts.h"

@@ -10,9 +10,9 @@
 // values are read from LDS as columns.
 //
 // Measured, where a large product of matrices reaches 1209 TFLOP/s: a chunk of 4096 rows over 16384 positions, 32 heads over 8, 128 dims,
-// e4m3: 962 GFLOP in 0.91 ms, 1060 TFLOP/s; four prompts of up to 3500 rows, bf16: 428 GFLOP in 0.48 ms, 890; a window of 1024 over
-// 2 x 3001 rows, 8 heads over one, 256 dims, fp16: 39 GFLOP in 91 us, 430. The matrix unit is busy 48 and 42 % of the cycles of the
-// first two; the softmax's vector instructions take most of the others, and do not run beside it. 256 dims: 28 %, LDS 36 %.
+// e4m3: 962 GFLOP in 0.92 ms, 1050 TFLOP/s (warm 0.99; 1.23 where the scales of values are far apart); four prompts of up to 3500 rows, bf16: 428 GFLOP
+// in 0.50 ms, 860; a window of 1024 over 2 x 3001 rows, 8 heads over one, 256 dims, fp16: 39 GFLOP in 92 us, 420. The matrix unit is busy 46 and
+// 41 % of the cycles of the first two; the softmax's vector instructions take most of the others, and do not run beside it. 256 dims: 27 %, LDS 36 %.
 #include <algorithm>
 #include <type_traits>
 

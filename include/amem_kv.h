@@ -71,7 +71,7 @@ typedef struct amem_kv_batch {
   int32_t sequences, table_pages;
   int32_t tokens;                /* rows of the token tensors */
   int32_t max_tokens;            /* most new tokens of one sequence; a guide where cu_tokens is given */
-  int32_t max_context;           /* no context[s] is above it */
+  int32_t max_context;           /* no context[s] is above it; work is dealt out by it, so that a limit far above costs few sequences time */
   int32_t reserved;              /* 0 */
 } amem_kv_batch;
 
