@@ -162,12 +162,6 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
     load_rows(keys, base, page, true, kreg);
     load_scales(base, page, ks, vs);
     load_rows(values, base, page, true, vreg);
-    if constexpr (EIGHT) {
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) unit_scale = fmaxf(unit_scale, seen(base + g * 16) ? lane_value(vs, g * 16) : 0);
-      unit_scale *= 1 << kNear;
-      inverse_unit = 1.0f / unit_scale;
-    }
   }
   for (; base < end; base += kStep) {
     const bool more = base + kStep < end;
@@ -262,6 +256,12 @@ __global__ __launch_bounds__(kWaves * kWave, (kOneWave<D, EIGHT, NB> ? 1 : 2)) v
 
     float f_scale[kGroups];  // scales of values, in multiples of unit_scale
     if constexpr (EIGHT) {
+      if (unit_scale == 0) {  // the first tile that some row sees: in front of a window's beginning others may lie
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) unit_scale = fmaxf(unit_scale, seen(base + g * 16) ? lane_value(vs, g * 16) : 0);
+        unit_scale *= 1 << kNear;
+        inverse_unit = 1.0f / unit_scale;
+      }
       float least = 1, most = 0;
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {

@@ -243,3 +243,20 @@ def test_memory_that_is_not_tracked_is_used_while_paused(gpu, fresh):
     finally:
         arena.free()
         buffers.free()
+
+
+@pytest.mark.parametrize("bad", [0.0, -1.0, 2.0 ** 120, float("nan"), float("inf"), 1e-45])
+@pytest.mark.parametrize("lengths,window", [([(1, 300)], 40), ([(1, 1500)], 1000), ([(6, 330)], 100), ([(100, 400)], 30), ([(300, 1300)], 200)])
+def test_scales_of_hidden_blocks_may_be_anything(arena, lengths, window, bad):
+    """In front of what a window lets the first row see, in tiles of their own and beside seen blocks, and behind the context."""
+    for dim in (64, 128):
+        case = Case(arena, lengths, dim=dim, q_heads=4, kv_heads=2, eight=True, page=32, block=16, seed=40)
+        (n, c), = lengths
+        for p in range(0, case.table_pages * 32, 16):
+            page = case.table[0, p // 32]
+            if page >= 0 and (p + 15 <= c - n - window or p >= c):
+                case.k_scale[page, :, p % 32 // 16] = case.v_scale[page, :, p % 32 // 16] = bad
+        case.upload()
+        got, lse = check_attend(case, case.rows(4), window=window)
+        assert np.isfinite(O.decode(got, "bf16")).all() and np.isfinite(lse).all()
+        arena.reset()
