@@ -140,10 +140,10 @@ def scaled_case(arena, lengths, dim, kind, exponents, bias, seed=35, **more):
     return case, O.encode(q, kind)
 
 
-FORMS = {"token": [(1, 700)], "draft": [(5, 330)], "prompt": [(100, 700)], "long": [(1, 5000), (2, 900)], "long prompt": [(300, 1300)]}
+FORMS = {"token": [(1, 700)], "draft": [(5, 330)], "prompt": [(100, 700)], "long": [(1, 2500), (2, 900)], "long prompt": [(300, 1300)]}
 
 
-@pytest.mark.parametrize("dim,kind", [(64, "bf16"), (64, "f16"), (128, "bf16"), (128, "f16"), (256, "bf16"), (256, "f16")])
+@pytest.mark.parametrize("dim,kind", [(64, "f16"), (128, "bf16"), (128, "f16"), (256, "bf16")])
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("exponents,bias", [((0, -14), 0), ((0, -14), 9.7), ((0, -14), 30), ((-14, 0), 5), ((9, -3, -9, 2), 12), ((-3, -7), 4), ((-3, -11), 4), ((-3, -12), 4), ((-7, -7, -7, -7, -3), 2),
                                             ((-7, -7, -7, -7, -2), 2)])
