@@ -36,7 +36,7 @@ def _kind(t):
 
 class KvError(RuntimeError):
     def __init__(self, what, code):
-        super().__init__("%s failed: %d (refused arguments, or paused, if 1; the library's log says why)" % (what, code))
+        super().__init__("%s failed: %d (refused arguments, or tracked memory while paused, if 1; the library's log says why)" % (what, code))
         self.code = code
 
 
