@@ -2,7 +2,10 @@
 #include <hip/hip_runtime_api.h>
 #include <unistd.h>
 
+#include <algorithm>
+#include <initializer_list>
 #include <mutex>
+#include <utility>
 
 #include "../../include/amem.h"
 #include "../../include/amem_kv.h"
@@ -96,6 +99,21 @@ int check_batch(const char* what, const amem_kv_batch* b, const KvCache& c, bool
 int check_rows(const char* what, const char* why, uint64_t at, int64_t token, int64_t head, int tokens, int heads) {
   NEED(at && at % 16 == 0 && stride_ok(token, 8) && stride_ok(head, 8) && fits(tokens, token) && fits(heads, head), why);
   return 0;
+}
+
+// Whether the elements of a tensor that a call writes are apart: each dimension, the smaller strides first, steps over all of those
+// before it. Holds for every view that slicing and permuting gives, not for one that repeats rows.
+bool apart(int64_t inner, std::initializer_list<std::pair<int64_t, int64_t>> sizes_and_strides) {
+  std::pair<int64_t, int64_t> dims[4];  // stride, size
+  int n = 0;
+  for (const auto& d : sizes_and_strides)
+    if (d.first > 1) dims[n++] = {d.second, d.first};
+  std::sort(dims, dims + n);
+  for (int i = 0; i < n; ++i) {
+    if (dims[i].first < inner) return false;
+    inner += (dims[i].second - 1) * dims[i].first;
+  }
+  return true;
 }
 
 // What a call may touch: bytes from `at` on.
@@ -194,6 +212,10 @@ int amem_kv_append(const amem_kv_cache* cache, const amem_kv_batch* batch, const
   NEED(a->type == AMEM_KV_BF16 || a->type == AMEM_KV_F16, "type is not 16 bits");
   const bool eight = cache->type == AMEM_KV_E4M3;
   NEED(eight || cache->type == a->type, "a 16-bit cache has another type than the rows");
+  NEED(apart(cache->head_dim, {{cache->pages, cache->page_stride}, {cache->kv_heads, cache->head_stride}, {cache->page_slots, cache->slot_stride}}),
+       "slots of the cache overlap");
+  NEED(!eight || apart(cache->page_slots / cache->block_slots, {{cache->pages, cache->scale_page_stride}, {cache->kv_heads, cache->scale_head_stride}}),
+       "scales of the cache overlap");
   if (b.tokens) {
     if (int e = check_rows(what, "address or strides of k", a->k, a->k_token_stride, a->k_head_stride, b.tokens, c.kv_heads)) return e;
     if (int e = check_rows(what, "address or strides of v", a->v, a->v_token_stride, a->v_head_stride, b.tokens, c.kv_heads)) return e;
@@ -203,6 +225,7 @@ int amem_kv_append(const amem_kv_cache* cache, const amem_kv_batch* batch, const
     NEED(a->q_heads >= 1 && a->q_heads <= 1024, "q_heads out of range");
     if (int e = check_rows(what, "address or strides of q", a->q, a->q_token_stride, a->q_head_stride, b.tokens, a->q_heads)) return e;
     if (int e = check_rows(what, "address or strides of q_out", a->q_out, a->q_out_token_stride, a->q_out_head_stride, b.tokens, a->q_heads)) return e;
+    NEED(apart(cache->head_dim, {{b.tokens, a->q_out_token_stride}, {a->q_heads, a->q_out_head_stride}}), "rows of q_out overlap");
   }
   const int pairs = a->rotary_dim / 2;
   NEED(a->rotary_dim >= 0 && a->rotary_dim <= cache->head_dim && a->rotary_dim % 16 == 0,
@@ -276,6 +299,7 @@ int amem_kv_attention(const amem_kv_cache* cache, const amem_kv_batch* batch, co
   if (b.tokens) {
     if (int e = check_rows(what, "address or strides of q", a->q, a->q_token_stride, a->q_head_stride, b.tokens, a->q_heads)) return e;
     if (int e = check_rows(what, "address or strides of out", a->out, a->out_token_stride, a->out_head_stride, b.tokens, a->q_heads)) return e;
+    NEED(apart(cache->head_dim, {{b.tokens, a->out_token_stride}, {a->q_heads, a->out_head_stride}}), "rows of out overlap");
   }
   NEED((int64_t)b.tokens * a->q_heads <= 1 << 27, "tokens * q_heads is above 2^27");
   NEED(a->lse % 4 == 0, "address of lse");

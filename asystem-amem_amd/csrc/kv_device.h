@@ -84,7 +84,6 @@ constexpr float kNothing = -1000.0f;  // h of a row that has seen nothing
 __device__ __forceinline__ int exponent_of(float x) { return (int)(__builtin_bit_cast(uint32_t, x) >> 23 & 0xff) - 127; }
 __device__ __forceinline__ int far_unit(float h) { return (int)ceilf(h) - 15; }  // its exponent
 
-
 template <bool HALF>  // nearest, ties to even
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   if constexpr (HALF) return __builtin_bit_cast(uint32_t, f16x2{(_Float16)lo, (_Float16)hi});

@@ -18,6 +18,8 @@
  * memory while paused, or another HIP error. Two calls that may run at the same time need different workspaces,
  * and must not write the same pages or read pages that the other writes.
  *
+ * What a call writes (q_out, out, the cache and its scales in append) must not overlap itself; strides that do are refused. What it only reads may.
+ *
  * Lengths, positions, page numbers and rows live in device memory and cannot be refused on the host. Where they
  * are out of range nothing outside the tensors is touched: see the notes below.
  */

@@ -202,3 +202,41 @@ def test_the_workspace_of_rows_that_do_not_add_up_is_refused(lib, sequences, tok
     assert lib.amem_kv_attention_workspace(C.byref(cache), C.byref(batch), 16, C.byref(n)) == 0       # with offsets: a guide
     batch.cu_tokens = 0
     assert lib.amem_kv_attention_workspace(C.byref(cache), C.byref(batch), 16, C.byref(n)) == INVALID
+
+
+@pytest.mark.parametrize("record,field,value,refused", [
+    (2, "q_out_token_stride", 0, (1, 0)), (2, "q_out_head_stride", 0, (1, 0)), (2, "q_out_token_stride", 512, (1, 0)), (2, "q_out_head_stride", 64, (1, 0)),
+    (3, "out_token_stride", 0, (0, 1)), (3, "out_head_stride", 0, (0, 1)), (3, "out_token_stride", 1016, (0, 1)), (3, "out_head_stride", 64, (0, 1)),
+    (0, "page_stride", 0, (1, 0)), (0, "head_stride", 0, (1, 0)), (0, "slot_stride", 0, (1, 0)), (0, "head_stride", 128, (1, 0)), (0, "page_stride", 3 * 64 * 128, (1, 0)),
+    (0, "scale_page_stride", 0, (1, 0)), (0, "scale_head_stride", 1, (1, 0)), (0, "scale_page_stride", 7, (1, 0)),
+    (2, "k_token_stride", 0, (0, 0)), (2, "v_head_stride", 0, (0, 0)), (2, "q_token_stride", 0, (0, 0)), (3, "q_head_stride", 0, (0, 0))])
+def test_what_is_written_must_not_overlap_itself(lib, record, field, value, refused):
+    """What is only read may: the same row for all, the same keys for all heads."""
+    if lib.amem_device_count():
+        pytest.skip("the addresses are made up: only where nothing can run")
+    args = valid(True)
+    setattr(args[record], field, value)
+    assert calls(lib, *args) == tuple(INVALID if r else NO_DEVICE for r in refused)
+
+
+def test_layouts_that_keep_rows_apart_are_taken(lib):
+    """Heads before tokens, slots before heads, a part of a wider tensor, one of each dimension with any stride."""
+    if lib.amem_device_count():
+        pytest.skip("the addresses are made up: only where nothing can run")
+    for change in ({"out_token_stride": 128, "out_head_stride": 20 * 128}, {"out_token_stride": 4096}, {"out_head_stride": 256, "out_token_stride": 2048}):
+        cache, batch, app, att = valid(True)
+        for k, v in change.items():
+            setattr(att, k, v)
+            setattr(app, "q_" + k, v)
+        assert calls(lib, cache, batch, app, att) == (NO_DEVICE, NO_DEVICE), change
+    cache, batch, app, att = valid(True)
+    cache.head_stride, cache.slot_stride = 128, 4 * 128                            # [page][slot][head][dim]
+    assert calls(lib, cache, batch, app, att) == (NO_DEVICE, NO_DEVICE)
+    cache.page_stride, cache.slot_stride = 128 * 4, 10 * 4 * 128                   # [slot][page][head][dim]
+    assert calls(lib, cache, batch, app, att) == (NO_DEVICE, NO_DEVICE)
+    cache, batch, app, att = valid(True)
+    cache.pages = cache.kv_heads = 1
+    cache.page_stride = cache.head_stride = cache.scale_page_stride = cache.scale_head_stride = 0
+    att.q_heads = app.q_heads = 1
+    att.out_head_stride = app.q_out_head_stride = 0
+    assert calls(lib, cache, batch, app, att) == (NO_DEVICE, NO_DEVICE)
